@@ -355,6 +355,57 @@ int zt_kv_append(float *k_cache, float *v_cache, int *n_keys, const float *k_new
                  const float *v_new, int *full_count, int batch, int n_ctx, int n_kv_heads, int dim,
                  zt_stream_t stream);
 
+/* Attention with a sliding window and a few first tokens that stay visible (sinks), over whole sequences: the query at
+ * position t sees key j where j <= t and (j > t - window or j < sinks).  window 0: no window, every key up to t.
+ * Layouts, lse, delta, the gradients and the backward's workspace (zt_attn_backward_workspace_bytes, the same rules) are
+ * those of zt_attn_forward_batched and zt_attn_backward_batched; out and lse handed to the backward are this forward's.
+ * Key tiles that no query of a tile sees are not visited, so the time goes with the pairs that are seen.  The forward takes
+ * no scratch.  Non-finite values: see "non-finite" in the notes on operands; a window's masks are masks in that sense.
+ * Refusals: those of the batched calls; window < 0; sinks < 0.
+ * No reference counterpart (src/attention.zig:60-153 sees the whole prefix). */
+int zt_attn_forward_window_batched(const float *q, const float *k, const float *v, float *out, float *lse, int batch,
+                                   int T, int n_heads, int n_kv_heads, int dim, int window, int sinks,
+                                   zt_stream_t stream);
+int zt_attn_backward_window_batched(const float *q, const float *k, const float *v, const float *out,
+                                    const float *lse, const float *dout, float *dq, float *dk, float *dv,
+                                    float *delta, void *workspace, size_t workspace_bytes, int batch, int T,
+                                    int n_heads, int n_kv_heads, int dim, int window, int sinks,
+                                    zt_stream_t stream);
+
+/* A KV cache of pages.  k_pages, v_pages are [n_pages, page_size, n_kv_heads*dim]; key slot j of sequence b is row
+ * j % page_size of page table[b, j / page_size] (table: [batch, max_pages]; a place without a page holds a negative number).
+ * n_keys[b] counts the filled slots.  New rows are ragged: sequence b has rows cu_rows[b] .. cu_rows[b + 1] - 1 of the new
+ * tensors (cu_rows: batch + 1 ascending numbers, device memory), of which there are `rows`; those from cu_rows[batch] on
+ * belong to nobody.  cu_rows NULL: one row a sequence, `rows` == batch.
+ *
+ * zt_kv_append_paged copies the new rows into slots n_keys[b], n_keys[b] + 1, ... and advances n_keys[b].  A sequence
+ * whose rows do not all have a place -- more than max_pages * page_size slots, a page number outside [0, n_pages), bounds
+ * that do not ascend within [0, rows] -- is left untouched and counted in *skipped (device int, may be NULL).  No two
+ * sequences of a call may append to the same page.
+ *
+ * zt_attn_paged: q, out [rows, n_heads*dim], lse [rows, n_heads] (may be NULL); the new rows, appended before, are the last of
+ * their sequence: row cu_rows[b] + i stands at position n_keys[b] - (cu_rows[b + 1] - cu_rows[b]) + i and sees slot j where
+ * j is at most its position and, where window > 0, also j > position - window or j < sinks.  Slots that no row sees are not
+ * read, nor are their places in the table, so a page that has left the window may be given to another sequence.  A row that
+ * sees a slot on a page number outside [0, n_pages) is NaN.  A sequence whose counts contradict each other (fewer keys
+ * than new rows, more than max_pages * page_size, bounds that do not ascend within [0, rows]) is not computed: its rows
+ * are NaN, and zt_attn_decode_status(workspace) counts it after a synchronisation.  Rows that belong to nobody are left as
+ * they are.  A non-finite key or value reaches the rows that see it, and no others.
+ * workspace: zt_attn_paged_workspace_bytes(batch, rows, max_keys, ...), 256-byte aligned, max_keys the most keys that a
+ * sequence holds (max_pages * page_size always does); a call with a smaller batch, fewer rows or keys may use it too.
+ * Refusals of both: batch outside 1 .. 65535; degenerate pages; a width (n_kv_heads * dim) that is no multiple of four, heads that
+ * are no group, a dim outside 32 .. 256 or no multiple of four; rows < 0; cu_rows NULL and rows != batch; null pointers; tensors off a 16-byte boundary; window or sinks < 0; a
+ * missing, short or misaligned workspace.  rows 0 is nothing to do.
+ * No reference counterpart (src/kv_cache.zig:60-95 keeps a sequence's rows contiguous). */
+int zt_kv_append_paged(float *k_pages, float *v_pages, const int *table, int *n_keys, const float *k_new,
+                       const float *v_new, const int *cu_rows, int *skipped, int batch, int rows, int n_pages,
+                       int page_size, int max_pages, int width, zt_stream_t stream);
+int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, const int *n_keys,
+                  const int *cu_rows, float *out, float *lse, void *workspace, size_t workspace_bytes, int batch,
+                  int rows, int n_pages, int page_size, int max_pages, int n_heads, int n_kv_heads, int dim,
+                  int window, int sinks, zt_stream_t stream);
+size_t zt_attn_paged_workspace_bytes(int batch, int rows, int max_keys, int n_heads, int n_kv_heads, int dim);
+
 /* Number of kernels this library has launched in this process (all threads);
  * benchmarks report the difference over their timed region. */
 unsigned long long zt_attn_launch_count(void);

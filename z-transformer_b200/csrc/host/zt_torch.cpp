@@ -198,6 +198,115 @@ PyObject *block_backward(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     return rc != 0 ? refused() : pack({dq, dk, dv});
 }
 
+// attention_forward_window(q, k, v, H, G, D, window, sinks, want_lse) -> (out, lse | None)
+PyObject *attention_forward_window(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    Qkv s;
+    int w[2];
+    if (n_args != 9 || !s.take(args) || !ints(args + 6, 2, w)) return none();
+    const int want_lse = PyObject_IsTrue(args[8]);
+    if (want_lse < 0) return nullptr;
+    const c10::cuda::CUDAGuard guard(s.q->device());
+    const at::Tensor out = at::empty(s.q->sizes(), s.q->options());
+    const at::Tensor lse = want_lse ? at::empty({s.B, s.T, s.H}, s.q->options()) : at::Tensor();
+    const zt_stream_t stream = stream_of(*s.q);
+    const int rc = without_gil([&] {
+        return zt_attn_forward_window_batched(in(s.q), in(s.k), in(s.v), out_of(out), lse.defined() ? out_of(lse) : nullptr, s.B, s.T, s.H, s.G,
+                                              s.D, w[0], w[1], stream);
+    });
+    return rc != 0 ? refused() : pack({out, lse});
+}
+
+// attention_backward_window(q, k, v, H, G, D, out, lse, dout, buffer | None, bytes, window, sinks) -> (dq, dk, dv)
+PyObject *attention_backward_window(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    Qkv s;
+    int w[2];
+    if (n_args != 13 || !s.take(args) || !ints(args + 11, 2, w)) return none();
+    const at::Tensor *out = f32(args[6], 3, s.q), *lse = f32(args[7], 3, s.q), *dout = f32(args[8], 3, s.q);
+    if (!out || !lse || !dout || out->sizes() != s.q->sizes() || dout->sizes() != s.q->sizes() || !is_shape(*lse, {s.B, s.T, s.H}))
+        return none();
+    const size_t bytes = PyLong_AsSize_t(args[10]);
+    if (PyErr_Occurred()) return nullptr;
+    bool ok;
+    void *ws = scratch(args[9], bytes, *s.q, &ok);
+    if (!ok) return none();
+    const c10::cuda::CUDAGuard guard(s.q->device());
+    const at::Tensor dq = at::empty(s.q->sizes(), s.q->options()), dk = at::empty(s.k->sizes(), s.k->options());
+    const at::Tensor dv = at::empty(s.v->sizes(), s.v->options()), delta = at::empty(lse->sizes(), lse->options());
+    const zt_stream_t stream = stream_of(*s.q);
+    const int rc = without_gil([&] {
+        return zt_attn_backward_window_batched(in(s.q), in(s.k), in(s.v), in(out), in(lse), in(dout), out_of(dq), out_of(dk), out_of(dv),
+                                               out_of(delta), bytes ? ws : nullptr, bytes, s.B, s.T, s.H, s.G, s.D, w[0], w[1], stream);
+    });
+    return rc != 0 ? refused() : pack({dq, dk, dv});
+}
+
+// A contiguous int32 CUDA tensor of this shape on q's device.
+const int *i32(PyObject *o, std::initializer_list<int64_t> shape, const at::Tensor &q) {
+    const at::Tensor *t = tensor(o);
+    if (!t || !t->is_cuda() || t->device() != q.device() || t->scalar_type() != at::kInt || !is_shape(*t, shape) || !t->is_contiguous()) return nullptr;
+    return t->const_data_ptr<int>();
+}
+// k_pages, v_pages [n_pages, page_size, width], table [B, max_pages], n_keys [B] and, where not None, cu_rows [B + 1].
+struct Paged {
+    const at::Tensor *k, *v;
+    const int *table, *n_keys, *cu;
+    int B, n_pages, page_size, max_pages, width;
+    bool take(PyObject *k_, PyObject *v_, PyObject *table_, PyObject *n_keys_, PyObject *cu_) {
+        const at::Tensor *t = tensor(table_);
+        if (!(k = f32(k_, 3)) || !(v = f32(v_, 3, k)) || k->sizes() != v->sizes() || !t || t->dim() != 2) return false;
+        for (const int64_t n : {k->size(0), k->size(1), k->size(2), t->size(0), t->size(1)})
+            if (n < 1 || n > 2147483647LL) return false;
+        n_pages = (int)k->size(0), page_size = (int)k->size(1), width = (int)k->size(2), B = (int)t->size(0), max_pages = (int)t->size(1);
+        table = i32(table_, {B, max_pages}, *k), n_keys = i32(n_keys_, {B}, *k), cu = cu_ == Py_None ? nullptr : i32(cu_, {(int64_t)B + 1}, *k);
+        return table && n_keys && (cu || cu_ == Py_None);
+    }
+};
+
+// paged_append(k_pages, v_pages, table, n_keys, k_new, v_new, cu_rows | None, skipped | None) -> True
+PyObject *paged_append(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    Paged p;
+    if (n_args != 8 || !p.take(args[0], args[1], args[2], args[3], args[6])) return none();
+    const at::Tensor *kn = f32(args[4], 2, p.k), *vn = f32(args[5], 2, p.k);
+    if (!kn || !vn || kn->sizes() != vn->sizes() || kn->size(1) != p.width || kn->size(0) > 2147483647LL) return none();
+    const int *skipped = args[7] == Py_None ? nullptr : i32(args[7], {1}, *p.k);
+    if (!skipped && args[7] != Py_None) return none();
+    const c10::cuda::CUDAGuard guard(p.k->device());
+    const zt_stream_t stream = stream_of(*p.k);
+    const int rc = without_gil([&] {
+        return zt_kv_append_paged(out_of(*p.k), out_of(*p.v), p.table, const_cast<int *>(p.n_keys), in(kn), in(vn), p.cu, const_cast<int *>(skipped), p.B,
+                                  (int)kn->size(0), p.n_pages, p.page_size, p.max_pages, p.width, stream);
+    });
+    if (rc != 0) return refused();
+    Py_RETURN_TRUE;
+}
+
+// attention_paged(q, k_pages, v_pages, table, n_keys, H, G, D, cu_rows | None, window, sinks, buffer, bytes, out | None, want_lse) -> (out, lse | None)
+PyObject *attention_paged(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    Paged p;
+    int n[3], w[2];
+    if (n_args != 15 || !ints(args + 5, 3, n) || !ints(args + 9, 2, w) || !p.take(args[1], args[2], args[3], args[4], args[8])) return none();
+    const int H = n[0], G = n[1], D = n[2];
+    const at::Tensor *q = f32(args[0], 2, p.k), *given = nullptr;
+    if (!q || H < 1 || G < 1 || D < 1 || H % G != 0 || (int64_t)G * D != p.width || q->size(1) != (int64_t)H * D || q->size(0) > 2147483647LL) return none();
+    if (args[13] != Py_None && (!(given = f32(args[13], 2, q)) || given->sizes() != q->sizes())) return none();
+    const size_t bytes = PyLong_AsSize_t(args[12]);
+    if (PyErr_Occurred()) return nullptr;
+    bool ok;
+    void *ws = scratch(args[11], bytes, *q, &ok);
+    if (!ok || !ws) return none();
+    const int want_lse = PyObject_IsTrue(args[14]);
+    if (want_lse < 0) return nullptr;
+    const c10::cuda::CUDAGuard guard(q->device());
+    const at::Tensor out = given ? *given : at::empty(q->sizes(), q->options());
+    const at::Tensor lse = want_lse ? at::empty({q->size(0), (int64_t)H}, q->options()) : at::Tensor();
+    const zt_stream_t stream = stream_of(*q);
+    const int rc = without_gil([&] {
+        return zt_attn_paged(in(q), in(p.k), in(p.v), p.table, p.n_keys, p.cu, out_of(out), lse.defined() ? out_of(lse) : nullptr, ws, bytes, p.B,
+                             (int)q->size(0), p.n_pages, p.page_size, p.max_pages, H, G, D, w[0], w[1], stream);
+    });
+    return rc != 0 ? refused() : pack({out, lse});
+}
+
 // forward_at(q, k, v, out (the holder's flat buffers), t, H, G, D, group_q, max_tile, q_offset, n_keys) -> True
 PyObject *forward_at(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     int n[8];
@@ -283,7 +392,9 @@ PyObject *guarded(PyObject *self, PyObject *const *args, Py_ssize_t n) {
 
 #define ZT_METHOD(f) {#f, (PyCFunction)(void *)guarded<f>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ZT_METHOD(attention_forward), ZT_METHOD(attention_backward), ZT_METHOD(block_forward), ZT_METHOD(block_backward),
-                         ZT_METHOD(forward_at), ZT_METHOD(decode), ZT_METHOD(kv_append), {nullptr, nullptr, 0, nullptr}};
+                         ZT_METHOD(forward_at), ZT_METHOD(decode), ZT_METHOD(kv_append),
+                         ZT_METHOD(attention_forward_window), ZT_METHOD(attention_backward_window), ZT_METHOD(paged_append),
+                         ZT_METHOD(attention_paged), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_zt_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,214 @@
+// A KV cache of pages: rows of keys and values in fixed-size pages of a pool that all sequences share, a table that names
+// every sequence's pages in order, and the kernels over it -- the append of new rows and the attention of new rows over
+// all rows so far.
+//
+// Key slot j of sequence b is row j % page_size of page table[b, j / page_size]; a page's row holds n_kv_heads * dim
+// floats.  New rows are ragged: sequence b has rows [cu_rows[b], cu_rows[b + 1]) of the new tensors (one each where
+// cu_rows is null).  They are appended first and attend then, so the last of them stands at slot n_keys[b] - 1, and the
+// query at position p sees slot j where j <= p and, with a window, where j > p - window or j < sinks.
+//
+// (The reference keeps a sequence's rows contiguous, src/kv_cache.zig:60-95, and appends one at a time.)
+#pragma once
+
+#include "zt_common.cuh"
+
+namespace zt {
+
+struct Pages {
+    const float *k, *v;  // [n_pages, page_size, width]
+    const int *table;    // [batch, max_pages]
+    int n_pages, page_size, max_pages, width;
+    // Elements from the pool's begin to the row of slot j of sequence b; negative where the table names no page for it.
+    __device__ __forceinline__ long long row(int b, int j) const {
+        const int slot = j / page_size, id = table[(long long)b * max_pages + slot];
+        return id < 0 || id >= n_pages ? -1 : ((long long)id * page_size + (j - slot * page_size)) * width;
+    }
+    __device__ __forceinline__ long long capacity() const { return (long long)max_pages * page_size; }
+};
+
+// What a query at position p sees; `window` 0: everything up to itself.
+struct Seen {
+    int window, sinks;
+    __device__ __forceinline__ bool operator()(int key, int pos) const { return key <= pos && (window == 0 || key > pos - window || key < sinks); }
+};
+
+// A sequence's new rows: [begin, begin + count) of `rows`, whose first stands at slot `pos`.
+struct NewRows {
+    int begin, count, pos;
+    bool bad;  // the counts contradict each other or the tensors: nothing is read for such a sequence
+};
+// n_keys: the rows of the sequence with the new ones (`appended`), or before them.
+__device__ __forceinline__ NewRows new_rows(const int *cu_rows, const int *n_keys, int b, int rows, const Pages &pg, bool appended) {
+    NewRows r;
+    r.begin = cu_rows ? cu_rows[b] : b;
+    const int end = cu_rows ? cu_rows[b + 1] : b + 1, nk = n_keys[b];
+    r.bad = r.begin < 0 || end < r.begin || end > rows;
+    r.count = r.bad ? 0 : end - r.begin;
+    r.pos = appended ? nk - r.count : nk;
+    r.bad = r.bad || nk < 0 || r.pos < 0 || (long long)r.pos + r.count > pg.capacity();
+    return r;
+}
+
+// ---- append ----------------------------------------------------------------------------------------------------------
+
+struct AppendParams {
+    Pages pg;
+    float *k_pages, *v_pages;
+    const float *k_new, *v_new;
+    int *n_keys, *skipped;
+    const int *cu_rows;
+    int batch, rows;
+};
+// Whether all of a sequence's new rows have a place (called by whole blocks): none is written otherwise.
+__device__ __forceinline__ bool rows_fit(const AppendParams &p, const NewRows &r, int b) {
+    bool fits = !r.bad;
+    if (fits && r.count > 0)
+        for (int s = r.pos / p.pg.page_size + (int)threadIdx.x; s <= (r.pos + r.count - 1) / p.pg.page_size; s += (int)blockDim.x) {
+            const int id = p.pg.table[(long long)b * p.pg.max_pages + s];
+            if (id < 0 || id >= p.pg.n_pages) fits = false;
+        }
+    return __syncthreads_and(fits);
+}
+// The sequence that row `row` belongs to, -1 if to none (called by whole blocks).
+__device__ __forceinline__ int sequence_of(const int *cu_rows, int batch, int row, int *found) {
+    if (!cu_rows) return row < batch ? row : -1;
+    if (threadIdx.x == 0) *found = -1;
+    __syncthreads();
+    for (int b = threadIdx.x; b < batch; b += blockDim.x)
+        if (cu_rows[b] <= row && row < cu_rows[b + 1]) atomicMax(found, b);
+    __syncthreads();
+    return *found;
+}
+
+// A block per new row.  Where a sequence has one row only (cu_rows null) its block also advances the count; elsewhere rows of
+// other blocks still read it, and advance_kernel follows.
+__global__ void __launch_bounds__(256) append_paged_kernel(const AppendParams p) {
+    __shared__ int found;
+    pdl_wait();
+    pdl_launch();
+    const int row = blockIdx.x;
+    const int b = sequence_of(p.cu_rows, p.batch, row, &found);
+    if (b < 0) return;
+    const NewRows r = new_rows(p.cu_rows, p.n_keys, b, p.rows, p.pg, false);
+    const bool fits = rows_fit(p, r, b);
+    if (fits) {
+        const long long at = p.pg.row(b, r.pos + (row - r.begin));
+        const float *ks = p.k_new + (long long)row * p.pg.width, *vs = p.v_new + (long long)row * p.pg.width;
+        float *kd = p.k_pages + at, *vd = p.v_pages + at;
+        for (int j = threadIdx.x * 4; j < p.pg.width; j += 1024) {
+            const float4 kx = *reinterpret_cast<const float4 *>(ks + j), vx = *reinterpret_cast<const float4 *>(vs + j);
+            *reinterpret_cast<float4 *>(kd + j) = kx, *reinterpret_cast<float4 *>(vd + j) = vx;
+        }
+    }
+    if (p.cu_rows) return;
+    __syncthreads();  // (every thread has read the count)
+    if (threadIdx.x == 0) {
+        if (fits) p.n_keys[b] = r.pos + 1;
+        else if (p.skipped) atomicAdd(p.skipped, 1);
+    }
+}
+// A block per sequence, behind append_paged_kernel: the counts take in the rows that it wrote.
+__global__ void __launch_bounds__(128) advance_kernel(const AppendParams p) {
+    pdl_wait();
+    pdl_launch();
+    const int b = blockIdx.x;
+    const NewRows r = new_rows(p.cu_rows, p.n_keys, b, p.rows, p.pg, false);
+    const bool fits = rows_fit(p, r, b);
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    if (fits) p.n_keys[b] = r.pos + r.count;
+    else if (p.skipped) atomicAdd(p.skipped, 1);
+}
+inline int launch_append_paged(const AppendParams &p, cudaStream_t stream) {
+    if (p.rows > 0 && launch_pdl("append_paged_kernel", append_paged_kernel, dim3((unsigned)p.rows), dim3(256), 0, stream, p)) return 1;
+    if (!p.cu_rows) return 0;
+    return launch_pdl("advance_kernel", advance_kernel, dim3((unsigned)p.batch), dim3(128), 0, stream, p);
+}
+
+// ---- attention -------------------------------------------------------------------------------------------------------
+
+constexpr int kPagedHeaderBytes = 256;  // of a workspace: how many sequences were bad
+
+struct PagedParams {
+    Pages pg;
+    const float *q;
+    const int *n_keys, *cu_rows;
+    float *out, *lse;  // lse may be null
+    int *bad_count;
+    int batch, rows, n_heads, n_kv_heads, dim;
+    Seen seen;
+    float scale_log2;
+};
+
+// Counted by one block, so that nothing has to be cleared beforehand.
+__device__ __forceinline__ void count_bad_rows(const PagedParams &p) {
+    __shared__ int total;
+    if (threadIdx.x == 0) total = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.batch; i += blockDim.x)
+        if (new_rows(p.cu_rows, p.n_keys, i, p.rows, p.pg, true).bad) atomicAdd(&total, 1);
+    __syncthreads();
+    if (threadIdx.x == 0) *p.bad_count = total;
+}
+
+// The formula as it stands: a block per (new row, head), whose four warps take the keys in turn, the head's columns across
+// a warp's lanes, and merge their partial softmaxes through shared memory.
+__global__ void __launch_bounds__(128) attn_paged_rows(const PagedParams p) {
+    constexpr int W = 4, C = 8;  // warps; columns a lane holds of a head of up to 256
+    __shared__ int found;
+    __shared__ float sm[W], sl[W], so[W][C * 32];
+    pdl_wait();
+    pdl_launch();
+    if (blockIdx.x == 0 && blockIdx.y == 0) count_bad_rows(p);
+    const int row = blockIdx.x, h = blockIdx.y, g = h / (p.n_heads / p.n_kv_heads);
+    const int b = sequence_of(p.cu_rows, p.batch, row, &found);
+    if (b < 0) return;
+    const NewRows r = new_rows(p.cu_rows, p.n_keys, b, p.rows, p.pg, true);
+    const long long head = (long long)row * p.n_heads + h;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float nan = __int_as_float(0x7fc00000);
+    if (r.bad) {
+        for (int j = threadIdx.x; j < p.dim; j += 128) p.out[head * p.dim + j] = nan;
+        if (p.lse && threadIdx.x == 0) p.lse[head] = nan;
+        return;
+    }
+    const int pos = r.pos + (row - r.begin);
+    float q[C], o[C], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) q[c] = lane + 32 * c < p.dim ? p.q[head * p.dim + lane + 32 * c] * p.scale_log2 : 0.f, o[c] = 0.f;
+    for (int key = warp; key <= pos; key += W) {
+        if (!p.seen(key, pos)) continue;
+        const long long at = p.pg.row(b, key);
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (lane + 32 * c < p.dim && at >= 0) s = fmaf(q[c], p.pg.k[at + g * p.dim + lane + 32 * c], s);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        if (at < 0) s = nan;  // a key on no page
+        const float top = fmaxf(m, s), keep = m == -INFINITY ? 0.f : ex2(m - top), w = ex2(s - top);
+        l = fmaf(l, keep, w), m = top;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (lane + 32 * c < p.dim) o[c] = fmaf(o[c], keep, at >= 0 ? w * p.pg.v[at + g * p.dim + lane + 32 * c] : w);
+    }
+    if (lane == 0) sm[warp] = m, sl[warp] = l;
+#pragma unroll
+    for (int c = 0; c < C; ++c) so[warp][lane + 32 * c] = o[c];
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+    for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w]);
+    for (int w = 0; w < W; ++w) sum += sm[w] == -INFINITY && sl[w] == 0.f ? 0.f : sl[w] * ex2(sm[w] - top);
+    for (int j = threadIdx.x; j < p.dim; j += 128) {
+        float x = 0.f;
+        for (int w = 0; w < W; ++w) x += sm[w] == -INFINITY && sl[w] == 0.f ? 0.f : so[w][j] * ex2(sm[w] - top);
+        p.out[head * p.dim + j] = x / sum;
+    }
+    if (p.lse && threadIdx.x == 0) p.lse[head] = (top + log2f(sum)) * kLn2;
+}
+inline int launch_paged_rows(const PagedParams &p, cudaStream_t stream) {
+    g_last_path = "paged-rows";
+    return launch_pdl("attn_paged_rows", attn_paged_rows, dim3((unsigned)p.rows, (unsigned)p.n_heads), dim3(128), 0, stream, p);
+}
+
+}  // namespace zt

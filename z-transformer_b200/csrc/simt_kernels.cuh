@@ -36,7 +36,22 @@ struct SimtFwdParams {
     // capacity; a count outside [1, capacity] yields a NaN row and bumps *bad_count.
     const int *n_keys_dev;
     int *bad_count;
+    int window, sinks;  // window > 0: key j takes part in the query at position t where j > t - window or j < sinks
 };
+// Whether key j lies in the window of the query at position t, or before it among the sinks.
+__device__ __forceinline__ bool in_window(int j, int t, int window, int sinks) { return window == 0 || j > t - window || j < sinks; }
+// The key tile behind the one at s0 that a tile of queries from position t0 on looks at: those between the sinks and the
+// first query's window are passed over.
+__device__ __forceinline__ int next_key_tile(int s0, int t0, int window, int sinks) {
+    const int next = s0 + kTile;
+    if (window == 0 || next < sinks) return next;
+    const int first = (t0 - window + 1) / kTile * kTile;  // (negative positions: a tile at or before 0)
+    return next > first ? next : first;
+}
+// Where the first of them is: at 0 where there are sinks.
+__device__ __forceinline__ int first_key_tile(int t0, int window, int sinks) {
+    return window == 0 || sinks > 0 || t0 < window ? 0 : (t0 - window + 1) / kTile * kTile;
+}
 
 struct SimtBwdParams {
     const float *q, *k, *v, *dout, *lse, *delta;
@@ -44,6 +59,7 @@ struct SimtBwdParams {
     int T, n_heads, n_kv_heads, dim;
     long long q_batch_stride, kv_batch_stride, lse_batch_stride;
     float scale, scale_log2;
+    int window, sinks;  // as in the forward
 };
 
 // Rows [row0, row0 + 32) of a [rows, ld_g] matrix, columns [col0, col0 + dim),
@@ -138,7 +154,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_fwd_simt(const SimtFwdParam
 #pragma unroll
     for (int i = 0; i < kMaxColsPerThread; ++i) o[i] = 0.f;
 
-    for (int s0 = 0; s0 < last_key; s0 += kTile) {
+    for (int s0 = first_key_tile(q_offset + t0, p.window, p.sinks); s0 < last_key; s0 = next_key_tile(s0, q_offset + t0, p.window, p.sinks)) {
         __syncthreads();  // previous tile's readers are done (also orders the Q load)
         load_tile(sK, k, s0, n_keys, kld, kvh * dim, dim);
         load_tile(sV, v, s0, n_keys, kld, kvh * dim, dim);
@@ -150,7 +166,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_fwd_simt(const SimtFwdParam
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int key = s0 + cg + 8 * i;
-            s[i] = ((key <= pos || ZT_DEFECT(1)) && key < n_keys) ? s[i] * p.scale_log2 : -INFINITY;
+            s[i] = ((key <= pos || ZT_DEFECT(1)) && key < n_keys && in_window(key, pos, p.window, p.sinks)) ? s[i] * p.scale_log2 : -INFINITY;
             tmax = fmaxf(tmax, s[i]);
         }
         tmax = row_max8(tmax);
@@ -252,7 +268,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_bwd_dq_simt(const SimtBwdPa
 #pragma unroll
     for (int i = 0; i < kMaxColsPerThread; ++i) acc[i] = 0.f;
 
-    for (int s0 = 0; s0 < last_key; s0 += kTile) {
+    for (int s0 = first_key_tile(t0, p.window, p.sinks); s0 < last_key; s0 = next_key_tile(s0, t0, p.window, p.sinks)) {
         __syncthreads();
         load_tile(sK, k, s0, p.T, kld, kvh * dim, dim);
         load_tile(sV, v, s0, p.T, kld, kvh * dim, dim);
@@ -263,7 +279,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_bwd_dq_simt(const SimtBwdPa
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int key = s0 + cg + 8 * i;
-            const float pe = ((key <= t || ZT_DEFECT(11)) && key < p.T) ? ex2(s[i] * p.scale_log2 - lse2) : 0.f;
+            const float pe = ((key <= t || ZT_DEFECT(11)) && key < p.T && in_window(key, t, p.window, p.sinks)) ? ex2(s[i] * p.scale_log2 - lse2) : 0.f;
             sS[r * (kTile + 1) + cg + 8 * i] = pe * (dp[i] - del);
         }
         __syncwarp();
@@ -324,6 +340,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_bwd_dkdv_simt(const SimtBwd
     for (int hh = 0; hh < group; ++hh) {
         const int h = kvh * group + hh;
         for (int t0 = s0; t0 < p.T; t0 += kTile) {  // s0 is a multiple of 32, so tiles align
+            if (p.window > 0 && s0 >= p.sinks && t0 >= s0 + kTile - 1 + p.window) break;  // (no query from here on sees one of the keys)
             __syncthreads();
             load_tile(sQ, q, t0, p.T, qld, h * dim, dim);
             load_tile(sG, g, t0, p.T, qld, h * dim, dim);
@@ -341,7 +358,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_bwd_dkdv_simt(const SimtBwd
             for (int i = 0; i < 4; ++i) {
                 const int rr = cg + 8 * i, t = t0 + rr;
                 const float pe =
-                    ((key <= t || ZT_DEFECT(11)) && t < p.T && key < p.T) ? ex2(st[i] * p.scale_log2 - sL[rr]) : 0.f;
+                    ((key <= t || ZT_DEFECT(11)) && t < p.T && key < p.T && in_window(key, t, p.window, p.sinks)) ? ex2(st[i] * p.scale_log2 - sL[rr]) : 0.f;
                 sP[kk * (kTile + 1) + rr] = pe;
                 sS[kk * (kTile + 1) + rr] = pe * (dpt[i] - sD[rr]);
             }

@@ -11,6 +11,7 @@
 #include "../../include/zt_attn.h"
 
 #include "decode_kernels.cuh"
+#include "paged_kernels.cuh"
 #include "simt_kernels.cuh"
 #include "zt_common.cuh"
 #ifndef ZT_NO_TC
@@ -301,16 +302,16 @@ static int backward_impl(const float *q, const float *k, const float *v, const f
                          float *delta, const float *dout, float *dq, float *dk, float *dv,
                          void *workspace, size_t workspace_bytes, int batch, int T, int n_heads,
                          int n_kv_heads, int dim, cudaStream_t stream, bool kept = false,
-                         const PeerList *dq_peers = nullptr) {
+                         const PeerList *dq_peers = nullptr, int window = 0, int sinks = 0) {
 #ifndef ZT_NO_TC
     const size_t least = backward_need(batch, T, n_heads, n_kv_heads, dim).least;
-    if (g_path.load() != 1 && workspace && workspace_bytes >= least &&
+    if (g_path.load() != 1 && window == 0 && workspace && workspace_bytes >= least &&
         (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
         n_kv_heads <= tcb::kPrepassMaxGroups && tcb::tc_bwd_supported(batch, T, dim, q, k, v, dout, dq, dk, dv)) {
         return launch_bwd_tc(q, k, v, out, dout, lse, delta, dq, dk, dv, workspace, workspace_bytes, batch, T, n_heads, n_kv_heads,
                              dim, stream, nullptr, nullptr, kept, dq_peers, g_path.load() == 8);
     }
-    if (g_path.load() != 1 && workspace && least > 0 && workspace_bytes >= least &&
+    if (g_path.load() != 1 && window == 0 && workspace && least > 0 && workspace_bytes >= least &&
         (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 && n_kv_heads <= tcb::kPrepassMaxGroups &&
         !(dq_peers && dq_peers->n > 0) &&
         tcw::tc_bwd_wide_supported(batch, T, n_heads, n_kv_heads, dim, q, k, v, dout, dq, dk, dv)) {
@@ -331,6 +332,7 @@ static int backward_impl(const float *q, const float *k, const float *v, const f
     p.lse_batch_stride = (long long)T * n_heads;
     p.scale = 1.0f / sqrtf((float)dim);
     p.scale_log2 = kLog2e / sqrtf((float)dim);
+    p.window = window, p.sinks = sinks;
     return launch_bwd_simt(p, batch, stream);
 }
 
@@ -677,7 +679,7 @@ static int backward_kept_impl(const float *q, const float *k, const float *v, co
                               const float *lse, const float *dout, float *dq, float *dk, float *dv,
                               float *delta, void *workspace, size_t workspace_bytes, int batch, int T,
                               int n_heads, int n_kv_heads, int dim, zt_stream_t stream,
-                              unsigned long long token, const PeerList *dq_peers) {
+                              unsigned long long token, const PeerList *dq_peers, int window = 0, int sinks = 0) {
     if (batch < 1 || batch > 65535) return refuse("batch %d is not launchable (1 .. 65535).", batch);
     if (check_geometry(T, n_heads, n_kv_heads, dim)) return 1;
     if (!q || !k || !v || !out || !lse || !dout || !dq || !dk || !dv || !delta)
@@ -697,7 +699,7 @@ static int backward_kept_impl(const float *q, const float *k, const float *v, co
                       "are gone (pass 0 to convert q, k, v again).", token);
     if (workspace) drop_kept_planes(workspace);
     return backward_impl(q, k, v, out, lse, delta, dout, dq, dk, dv, workspace, workspace_bytes, batch, T, n_heads,
-                         n_kv_heads, dim, s, kept, dq_peers);
+                         n_kv_heads, dim, s, kept, dq_peers, window, sinks);
 }
 
 int zt_attn_backward_batched_kept(const float *q, const float *k, const float *v, const float *out,
@@ -1146,6 +1148,108 @@ int zt_kv_append(float *k_cache, float *v_cache, int *n_keys, const float *k_new
     const bool vec = width % 4 == 0 && aligned16(k_cache) && aligned16(v_cache) && aligned16(k_new) && aligned16(v_new);
     return launch_pdl("kv_append_kernel", vec ? kv_append_kernel<true> : kv_append_kernel<false>, dim3((unsigned)batch), dim3(256), 0, s,
                       k_cache, v_cache, n_keys, k_new, v_new, full_count, n_ctx, width);
+}
+
+// ---- sliding windows over whole sequences ---------------------------------------------------------------------
+// A window, or sinks, as long as the sequence leave nothing out: the plain calls' case (window 0).
+static void normal_window(int T, int *window, int *sinks) {
+    if (*window == 0 || *window >= T || *sinks >= T) *window = 0, *sinks = 0;
+}
+static int check_window(int window, int sinks) {
+    if (window < 0) return refuse("a window of %d keys is refused (0: no window).", window);
+    if (sinks < 0) return refuse("%d sinks is refused.", sinks);
+    return 0;
+}
+
+int zt_attn_forward_window_batched(const float *q, const float *k, const float *v, float *out, float *lse, int batch,
+                                   int T, int n_heads, int n_kv_heads, int dim, int window, int sinks,
+                                   zt_stream_t stream) {
+    g_last_error[0] = 0;
+    if (batch < 1 || batch > 65535) return refuse("batch %d is not launchable (1 .. 65535).", batch);
+    if (check_geometry(T, n_heads, n_kv_heads, dim) || check_window(window, sinks)) return 1;
+    if (!q || !k || !v || !out) return refuse("a null device pointer was passed.");
+    if (need_device()) return 1;
+    normal_window(T, &window, &sinks);
+    if (window == 0) return forward_impl(q, k, v, out, lse, batch, T, n_heads, n_kv_heads, dim, 0, T, (cudaStream_t)stream);
+    SimtFwdParams p{};
+    p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
+    p.T = T, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.dim = dim, p.n_keys = T;
+    p.q_batch_stride = (long long)T * n_heads * dim, p.kv_batch_stride = (long long)T * n_kv_heads * dim;
+    p.lse_batch_stride = (long long)T * n_heads;
+    p.scale_log2 = kLog2e / sqrtf((float)dim);
+    p.window = window, p.sinks = sinks;
+    return launch_fwd_simt(p, batch, (cudaStream_t)stream);
+}
+
+int zt_attn_backward_window_batched(const float *q, const float *k, const float *v, const float *out,
+                                    const float *lse, const float *dout, float *dq, float *dk, float *dv,
+                                    float *delta, void *workspace, size_t workspace_bytes, int batch, int T,
+                                    int n_heads, int n_kv_heads, int dim, int window, int sinks, zt_stream_t stream) {
+    g_last_error[0] = 0;
+    if (check_window(window, sinks)) return 1;
+    normal_window(T, &window, &sinks);
+    return backward_kept_impl(q, k, v, out, lse, dout, dq, dk, dv, delta, workspace, workspace_bytes, batch, T, n_heads,
+                              n_kv_heads, dim, stream, 0ull, nullptr, window, sinks);
+}
+
+// ---- a paged cache -----------------------------------------------------------------------------------------------
+static int check_pages(int batch, int rows, const int *cu_rows, int n_pages, int page_size, int max_pages, long long width) {
+    if (batch < 1 || batch > 65535) return refuse("batch %d is not launchable (1 .. 65535).", batch);
+    if (n_pages < 1 || page_size < 1 || max_pages < 1 || (long long)max_pages * page_size > 2147483647LL)
+        return refuse("%d pages of %d rows, %d a sequence at most, are not a cache.", n_pages, page_size, max_pages);
+    if (width < 4 || width % 4 != 0 || width > 2147483647LL) return refuse("pages of %lld columns are refused: not a multiple of four.", width);
+    if (rows < 0) return refuse("%d new rows is refused.", rows);
+    if (!cu_rows && rows != batch) return refuse("%d new rows of %d sequences: without cu_rows every sequence has one.", rows, batch);
+    return 0;
+}
+
+int zt_kv_append_paged(float *k_pages, float *v_pages, const int *table, int *n_keys, const float *k_new,
+                       const float *v_new, const int *cu_rows, int *skipped, int batch, int rows, int n_pages,
+                       int page_size, int max_pages, int width, zt_stream_t stream) {
+    g_last_error[0] = 0;
+    if (check_pages(batch, rows, cu_rows, n_pages, page_size, max_pages, width)) return 1;
+    if (!k_pages || !v_pages || !table || !n_keys || (rows > 0 && (!k_new || !v_new))) return refuse("a null device pointer was passed.");
+    for (const void *t : {(const void *)k_pages, (const void *)v_pages, (const void *)k_new, (const void *)v_new})
+        if (!aligned16(t)) return refuse("the pages and the new rows must be 16-byte aligned.");
+    if (need_device()) return 1;
+    AppendParams p{};
+    p.pg = Pages{k_pages, v_pages, table, n_pages, page_size, max_pages, width};
+    p.k_pages = k_pages, p.v_pages = v_pages, p.k_new = k_new, p.v_new = v_new;
+    p.n_keys = n_keys, p.skipped = skipped, p.cu_rows = cu_rows, p.batch = batch, p.rows = rows;
+    g_last_path = "kv-append";
+    return launch_append_paged(p, (cudaStream_t)stream);
+}
+
+size_t zt_attn_paged_workspace_bytes(int batch, int rows, int max_keys, int n_heads, int n_kv_heads, int dim) {
+    if (batch < 1 || rows < 0 || max_keys < 1 || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || !zt_attn_dim_ok(dim) || dim % 4 != 0)
+        return 0;
+    return kPagedHeaderBytes;
+}
+
+int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, const int *n_keys,
+                  const int *cu_rows, float *out, float *lse, void *workspace, size_t workspace_bytes, int batch,
+                  int rows, int n_pages, int page_size, int max_pages, int n_heads, int n_kv_heads, int dim,
+                  int window, int sinks, zt_stream_t stream) {
+    g_last_error[0] = 0;
+    if (check_geometry(1, n_heads, n_kv_heads, dim)) return 1;
+    if (dim % 4 != 0) return refuse("head_dim %d is refused: pages take multiples of four columns.", dim);
+    if (check_pages(batch, rows, cu_rows, n_pages, page_size, max_pages, (long long)n_kv_heads * dim) || check_window(window, sinks)) return 1;
+    if (!k_pages || !v_pages || !table || !n_keys || (rows > 0 && (!q || !out))) return refuse("a null device pointer was passed.");
+    const size_t need = zt_attn_paged_workspace_bytes(batch, rows, max_pages * page_size, n_heads, n_kv_heads, dim);
+    if (!workspace || workspace_bytes < need) return refuse("paged attention needs %zu bytes of workspace, %zu were given.", need, workspace_bytes);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return refuse("the paged workspace must be 256-byte aligned.");
+    for (const void *t : {(const void *)q, (const void *)k_pages, (const void *)v_pages, (const void *)out})
+        if (!aligned16(t)) return refuse("q, out and the pages must be 16-byte aligned.");
+    if (need_device()) return 1;
+    if (rows == 0) return 0;
+    PagedParams p{};
+    p.pg = Pages{k_pages, v_pages, table, n_pages, page_size, max_pages, n_kv_heads * dim};
+    p.q = q, p.n_keys = n_keys, p.cu_rows = cu_rows, p.out = out, p.lse = lse;
+    p.bad_count = static_cast<int *>(workspace);
+    p.batch = batch, p.rows = rows, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.dim = dim;
+    p.seen = window == 0 || window >= max_pages * page_size ? Seen{0, 0} : Seen{window, sinks};
+    p.scale_log2 = kLog2e / sqrtf((float)dim);
+    return launch_paged_rows(p, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -16,7 +16,8 @@ from __future__ import annotations
 
 from . import lib as _lib
 from .device import ConfigRefused
-from .ops import DecodeWorkspace, DimensionMismatch, _need_cuda_f32, decode_attention
+from .ops import (DecodeWorkspace, DimensionMismatch, PagedWorkspace, _need_cuda_f32, attention_paged, decode_attention,
+                  paged_append)
 
 
 class Full(Exception):
@@ -133,3 +134,106 @@ def attn_step(q, layer: Layer, n_heads, n_kv_heads, head_dim, *, workspace: Deco
         raise DimensionMismatch("cache width disagrees with the head configuration")
     return decode_attention(q, layer.k, layer.v, layer.len, n_heads, n_kv_heads, head_dim,
                             workspace=workspace, want_lse=want_lse)
+
+
+class PagedLayer:
+    """A layer's cache for `batch` sequences whose rows lie in pages of a common pool: k, v [n_pages, page_size, width], a table
+    [batch, max_pages] of every sequence's pages (-1: none) and per-sequence len.  Which pages are whose is decided on the host, from
+    counts kept there; no step reads the device.  (kv_cache.Layer, src/kv_cache.zig:60-135, keeps n_ctx rows for each.)"""
+
+    def __init__(self, n_pages: int, page_size: int, width: int, batch: int, max_pages: int, device="cuda"):
+        import torch
+        if min(n_pages, page_size, width, batch, max_pages) < 1 or width % 4 != 0:
+            raise DimensionMismatch("kv_cache.PagedLayer")
+        self.n_pages, self.page_size, self.width, self.batch, self.max_pages = n_pages, page_size, width, batch, max_pages
+        self.k = torch.zeros((n_pages, page_size, width), dtype=torch.float32, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.table = torch.full((batch, max_pages), -1, dtype=torch.int32, device=device)
+        self.len = torch.zeros((batch,), dtype=torch.int32, device=device)
+        self.skipped = torch.zeros((1,), dtype=torch.int32, device=device)
+        self._table = torch.full((batch, max_pages), -1, dtype=torch.int32)
+        self._len = [0] * batch
+        self._free = list(range(n_pages - 1, -1, -1))
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _send_table(self):
+        # (a copy that is ours alone: the host's table may change before the device has read it)
+        self.table.copy_(self._table.clone(), non_blocking=True)
+
+    def append(self, k_rows, v_rows, counts=None):
+        """counts[b] new rows of each sequence, behind one another in k_rows, v_rows [N, width] (None: one each).  Refuses with
+        Full, writing nothing, when a sequence has no place left in the table or the pool no page.  Returns the rows' bounds
+        cu_rows on the device (None for one row each), which attn_rows takes."""
+        import torch
+        given = [1] * self.batch if counts is None else [int(n) for n in counts]
+        if len(given) != self.batch or min(given) < 0:
+            raise DimensionMismatch("kv_cache.PagedLayer.append takes a count for every sequence")
+        shape = (sum(given), self.width)
+        if tuple(k_rows.shape) != shape or tuple(v_rows.shape) != shape:
+            raise DimensionMismatch("kv_cache.PagedLayer.append")
+        _need_cuda_f32(k_rows, v_rows)
+        if k_rows.device != self.k.device or v_rows.device != self.k.device:
+            raise DimensionMismatch("the new rows must live on the cache's device")
+        self.reserve(given)
+        cu = None
+        if counts is not None:
+            cu = torch.zeros(self.batch + 1, dtype=torch.int32)
+            cu[1:] = torch.tensor(given, dtype=torch.int32).cumsum(0)
+            cu = cu.to(self.k.device, non_blocking=True)
+        paged_append(self.k, self.v, self.table, self.len, k_rows, v_rows, cu_rows=cu, skipped=self.skipped)
+        self._len = [n + m for n, m in zip(self._len, given)]
+        return cu
+
+    def reserve(self, counts) -> None:
+        """Pages for counts[b] more rows of each sequence, for all of them or (Full) for none."""
+        wanted = []
+        for b, n in enumerate(counts):
+            if n < 0:
+                raise DimensionMismatch("kv_cache.PagedLayer.reserve")
+            if self._len[b] + n > self.max_pages * self.page_size:
+                raise Full("kv_cache.PagedLayer: the sequence's table")
+            wanted += [(b, s) for s in range(self._len[b] // self.page_size, -(-(self._len[b] + n) // self.page_size))
+                       if self._table[b, s] < 0]
+        if len(wanted) > len(self._free):
+            raise Full("kv_cache.PagedLayer: the pool")
+        for b, s in wanted:
+            self._table[b, s] = self._free.pop()
+        if wanted:
+            self._send_table()
+
+    def release(self, b: int) -> None:
+        """The sequence ends: its pages go back to the pool and its place is empty again."""
+        self._give_back(b, range(self.max_pages))
+        self._len[b] = 0
+        self.len[b].zero_()
+
+    def trim(self, window: int, sinks: int = 0) -> int:
+        """Gives back the pages that no coming query of `window` and `sinks` sees; returns how many."""
+        if window < 1 or sinks < 0:
+            raise DimensionMismatch("kv_cache.PagedLayer.trim")
+        before, ps = len(self._free), self.page_size
+        for b, n in enumerate(self._len):
+            # the next query stands at n and sees slots from n - window + 1 on
+            self._give_back(b, range(-(-sinks // ps), max(0, n - window + 1) // ps))
+        return len(self._free) - before
+
+    def _give_back(self, b, slots) -> None:
+        held = [s for s in slots if self._table[b, s] >= 0]
+        self._free += [int(self._table[b, s]) for s in held]
+        self._table[b, held] = -1
+        if held:
+            self._send_table()
+
+    def bytes(self) -> int:
+        return 2 * self.n_pages * self.page_size * self.width * 4
+
+
+def attn_rows(q, layer: PagedLayer, n_heads, n_kv_heads, head_dim, *, cu_rows=None, window=0, sinks=0,
+              workspace: PagedWorkspace | None = None, want_lse=False):
+    """attn_step over pages, for the rows that layer.append took last (and whose bounds it returned): q [N, H*D]."""
+    if layer.width != n_kv_heads * head_dim:
+        raise DimensionMismatch("cache width disagrees with the head configuration")
+    return attention_paged(q, layer.k, layer.v, layer.table, layer.len, n_heads, n_kv_heads, head_dim, cu_rows=cu_rows,
+                           window=window, sinks=sinks, workspace=workspace, want_lse=want_lse)

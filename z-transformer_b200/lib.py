@@ -54,6 +54,11 @@ _SIGNATURES = {
     "zt_attn_decode_static_capacity": (_sz, []),
     "zt_attn_decode_status": (_i, [_vp, C.POINTER(_i)]),
     "zt_kv_append": (_i, [_vp] * 6 + [_i] * 4 + [_vp]),
+    "zt_attn_forward_window_batched": (_i, [_vp] * 5 + [_i] * 7 + [_vp]),
+    "zt_attn_backward_window_batched": (_i, [_vp] * 11 + [_sz] + [_i] * 7 + [_vp]),
+    "zt_kv_append_paged": (_i, [_vp] * 8 + [_i] * 6 + [_vp]),
+    "zt_attn_paged": (_i, [_vp] * 9 + [_sz] + [_i] * 10 + [_vp]),
+    "zt_attn_paged_workspace_bytes": (_sz, [_i] * 6),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

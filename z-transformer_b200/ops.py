@@ -235,6 +235,82 @@ def attention_backward_rope(q, k, v, out, lse, dout, n_heads, n_kv_heads, head_d
     return dq, dk, dv
 
 
+def _window_args(q, k, v, n_heads, n_kv_heads, head_dim, window, sinks):
+    _head_config(n_heads, n_kv_heads, head_dim)
+    _need_cuda_f32(q, k, v)
+    if q.dim() != 3:
+        raise DimensionMismatch("the window calls take [B, T, width] tensors")
+    B, T = q.shape[0], q.shape[1]
+    if (k.shape[:2] != (B, T) or v.shape != k.shape or k.dim() != 3 or k.shape[2] != n_kv_heads * head_dim
+            or q.shape[2] != n_heads * head_dim):
+        raise DimensionMismatch("q/k/v shapes disagree with the head configuration")
+    if k.device != q.device or v.device != q.device:
+        raise DimensionMismatch("q, k and v must live on one device")
+    return B, T, _counts(window, sinks)
+
+
+def _counts(window, sinks):
+    """window and sinks for the C calls, whose ints hold 31 bits: what is longer leaves nothing out either way."""
+    window, sinks = int(window), int(sinks)
+    return (min(window, 2**31 - 1) if window >= 0 else -1, min(sinks, 2**31 - 1) if sinks >= 0 else -1)
+
+
+def attention_forward_window(q, k, v, n_heads, n_kv_heads, head_dim, window, *, sinks=0, want_lse=False):
+    """Batched attention.forward with a sliding window: the query at position t sees key j where j <= t and (j > t - window or
+    j < sinks), the first `sinks` tokens staying visible to all.  window 0: no window.  q [B, T, H*D], k and v [B, T, Hkv*D];
+    returns out (and lse [B, T, H])."""
+    done = _lib.native().attention_forward_window(q, k, v, n_heads, n_kv_heads, head_dim, window, sinks, want_lse)
+    if done:
+        return done if want_lse else done[0]
+    # (whatever has to be refused)
+    import torch
+    B, T, (window, sinks) = _window_args(q, k, v, n_heads, n_kv_heads, head_dim, window, sinks)
+    out = torch.empty_like(q)
+    lse = torch.empty((B, T, n_heads), dtype=torch.float32, device=q.device) if want_lse else None
+    with torch.cuda.device(q.device):
+        rc = _lib.load().zt_attn_forward_window_batched(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None, B, T, n_heads,
+            n_kv_heads, head_dim, window, sinks, _stream(q))
+    if rc != 0:
+        raise ConfigRefused(_lib.last_error())
+    return (out, lse) if want_lse else out
+
+
+def attention_backward_window(q, k, v, out, lse, dout, n_heads, n_kv_heads, head_dim, window, *, sinks=0, workspace=None):
+    """dq, dk, dv of attention_forward_window from its out and lse, with its window and sinks.
+    workspace: a BackwardWorkspace of this shape (one is allocated per call otherwise)."""
+    if workspace is not None and workspace.shape == (*q.shape[:2], n_heads, n_kv_heads, head_dim):
+        done = _lib.native().attention_backward_window(q, k, v, n_heads, n_kv_heads, head_dim, out, lse, dout, workspace.buf,
+                                                       workspace.nbytes, window, sinks)
+        if done is not None:
+            workspace.token = 0
+            if not done:
+                raise ConfigRefused(_lib.last_error())
+            return done
+    import torch
+    B, T, (window, sinks) = _window_args(q, k, v, n_heads, n_kv_heads, head_dim, window, sinks)
+    _need_cuda_f32(out, lse, dout)
+    if dout.shape != q.shape or out.shape != q.shape or lse.shape != (B, T, n_heads):
+        raise DimensionMismatch("dout/out/lse shapes disagree with q")
+    if any(x.device != q.device for x in (out, lse, dout)):
+        raise DimensionMismatch("all tensors must live on one device")
+    if workspace is None:
+        workspace = BackwardWorkspace(B, T, n_heads, n_kv_heads, head_dim, q.device)
+    elif workspace.shape != (B, T, n_heads, n_kv_heads, head_dim):
+        raise DimensionMismatch("the workspace was sized for another shape")
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    delta = torch.empty_like(lse)
+    workspace.token = 0
+    with torch.cuda.device(q.device):
+        rc = _lib.load().zt_attn_backward_window_batched(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), workspace.buf.data_ptr() if workspace.nbytes else None,
+            workspace.nbytes, B, T, n_heads, n_kv_heads, head_dim, window, sinks, _stream(q))
+    if rc != 0:
+        raise ConfigRefused(_lib.last_error())
+    return dq, dk, dv
+
+
 class ProjWorkspace:
     """Caller-owned scratch of the projection calls for one (batch, T, k, n) shape."""
 
@@ -418,6 +494,118 @@ def decode_attention(q, k_cache, v_cache, n_keys, n_heads, n_kv_heads, head_dim,
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), n_keys.data_ptr(), out.data_ptr(),
             lse.data_ptr() if want_lse else None, workspace.buf.data_ptr(), workspace.nbytes, B, n_ctx,
             n_heads, n_kv_heads, head_dim, _stream(q))
+    if rc != 0:
+        raise ConfigRefused(_lib.last_error())
+    return (out, lse) if want_lse else out
+
+
+class PagedWorkspace:
+    """Caller-owned scratch of attention_paged for up to `batch` sequences, `rows` new rows together and `max_keys` keys a
+    sequence."""
+
+    def __init__(self, batch, rows, max_keys, n_heads, n_kv_heads, head_dim, device="cuda"):
+        import torch
+        self.shape = (batch, rows, max_keys, n_heads, n_kv_heads, head_dim)
+        self.nbytes = int(_lib.load().zt_attn_paged_workspace_bytes(*self.shape))
+        if self.nbytes == 0:
+            raise ConfigRefused("the paged shape is not admissible")
+        self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+
+    def bad_sequences(self) -> int:
+        """Sequences that the last call over this workspace found contradictory (waits for the GPU)."""
+        import ctypes
+        import torch
+        n = ctypes.c_int(0)
+        torch.cuda.synchronize(self.buf.device)
+        if _lib.load().zt_attn_decode_status(self.buf.data_ptr(), ctypes.byref(n)) != 0:
+            raise RuntimeError(_lib.last_error())
+        return n.value
+
+
+def _int32(t, shape, device, what):
+    import torch
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise DimensionMismatch(f"{what} must be a contiguous int32 tensor of shape {shape} on the pages' device")
+
+
+def _paged_args(k_pages, v_pages, table, n_keys, cu_rows):
+    _need_cuda_f32(k_pages, v_pages)
+    if k_pages.dim() != 3 or v_pages.shape != k_pages.shape or v_pages.device != k_pages.device:
+        raise DimensionMismatch("the pages are two tensors [n_pages, page_size, Hkv*D] on one device")
+    if table.dim() != 2:
+        raise DimensionMismatch("the table is [batch, max_pages]")
+    B = table.shape[0]
+    _int32(table, tuple(table.shape), k_pages.device, "the table")
+    _int32(n_keys, (B,), k_pages.device, "n_keys")
+    if cu_rows is not None:
+        _int32(cu_rows, (B + 1,), k_pages.device, "cu_rows")
+    return B
+
+
+def paged_append(k_pages, v_pages, table, n_keys, k_new, v_new, *, cu_rows=None, skipped=None):
+    """New rows into a cache of pages [n_pages, page_size, width]: sequence b's rows cu_rows[b] .. cu_rows[b + 1] - 1 of k_new,
+    v_new [N, width] go to its slots from n_keys[b] on, slot j being row j % page_size of page table[b, j // page_size], and
+    n_keys[b] moves on.  cu_rows None: one row a sequence.  A sequence whose rows do not all have a place is left untouched and
+    counted in `skipped` (int32 [1], may be None)."""
+    if _lib.native().paged_append(k_pages, v_pages, table, n_keys, k_new, v_new, cu_rows, skipped):
+        return
+    import torch
+    B = _paged_args(k_pages, v_pages, table, n_keys, cu_rows)
+    _need_cuda_f32(k_new, v_new)
+    if k_new.dim() != 2 or k_new.shape[1] != k_pages.shape[2] or v_new.shape != k_new.shape:
+        raise DimensionMismatch("the new rows are two tensors [N, width] of the pages' width")
+    if k_new.device != k_pages.device or v_new.device != k_pages.device:
+        raise DimensionMismatch("the new rows must live on the pages' device")
+    if skipped is not None:
+        _int32(skipped, (1,), k_pages.device, "skipped")
+    n_pages, page_size, width = k_pages.shape
+    with torch.cuda.device(k_pages.device):
+        rc = _lib.load().zt_kv_append_paged(
+            k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), n_keys.data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
+            cu_rows.data_ptr() if cu_rows is not None else None, skipped.data_ptr() if skipped is not None else None, B,
+            k_new.shape[0], n_pages, page_size, table.shape[1], width, _stream(k_pages))
+    if rc != 0:
+        raise ConfigRefused(_lib.last_error())
+
+
+def attention_paged(q, k_pages, v_pages, table, n_keys, n_heads, n_kv_heads, head_dim, *, cu_rows=None, window=0, sinks=0,
+                    workspace=None, want_lse=False, out=None):
+    """Attention of new rows over a paged cache that they have been appended to (paged_append): q [N, H*D], of which rows
+    cu_rows[b] .. cu_rows[b + 1] - 1 are the last of sequence b's n_keys[b]; each sees the slots up to its own and, with a
+    window, of those the last `window` and the first `sinks`.  cu_rows None: one row a sequence (a decode step).
+    Returns out [N, H*D] (and lse [N, H]); rows that belong to no sequence are left as they are.
+    workspace: a PagedWorkspace at least this large (one is allocated per call otherwise)."""
+    if workspace is not None:
+        done = _lib.native().attention_paged(q, k_pages, v_pages, table, n_keys, n_heads, n_kv_heads, head_dim, cu_rows, window,
+                                             sinks, workspace.buf, workspace.nbytes, out, want_lse)
+        if done:
+            return done if want_lse else done[0]
+    import torch
+    _head_config(n_heads, n_kv_heads, head_dim)
+    B = _paged_args(k_pages, v_pages, table, n_keys, cu_rows)
+    _need_cuda_f32(q, out)
+    n_pages, page_size, width = k_pages.shape
+    if width != n_kv_heads * head_dim or q.dim() != 2 or q.shape[1] != n_heads * head_dim:
+        raise DimensionMismatch("q and the pages disagree with the head configuration")
+    if q.device != k_pages.device:
+        raise DimensionMismatch("q must live on the pages' device")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.device != q.device:
+        raise DimensionMismatch("out must be a tensor of q's shape on q's device")
+    N = q.shape[0]
+    if workspace is None:
+        workspace = PagedWorkspace(B, N, table.shape[1] * page_size, n_heads, n_kv_heads, head_dim, q.device)
+    elif workspace.buf.device != q.device:
+        raise DimensionMismatch("the workspace must live on q's device")
+    lse = torch.empty((N, n_heads), dtype=torch.float32, device=q.device) if want_lse else None
+    window, sinks = _counts(window, sinks)
+    with torch.cuda.device(q.device):
+        rc = _lib.load().zt_attn_paged(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), n_keys.data_ptr(),
+            cu_rows.data_ptr() if cu_rows is not None else None, out.data_ptr(), lse.data_ptr() if want_lse else None,
+            workspace.buf.data_ptr(), workspace.nbytes, B, N, n_pages, page_size, table.shape[1], n_heads, n_kv_heads, head_dim,
+            window, sinks, _stream(q))
     if rc != 0:
         raise ConfigRefused(_lib.last_error())
     return (out, lse) if want_lse else out
