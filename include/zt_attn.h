@@ -391,8 +391,8 @@ int zt_attn_backward_window_batched(const float *q, const float *k, const float 
  * than new rows, more than max_pages * page_size, bounds that do not ascend within [0, rows]) is not computed: its rows
  * are NaN, and zt_attn_decode_status(workspace) counts it after a synchronisation.  Rows that belong to nobody are left as
  * they are.  A non-finite key or value reaches the rows that see it, and no others.
- * workspace: zt_attn_paged_workspace_bytes(batch, rows, max_keys, ...), 256-byte aligned, max_keys the most keys that a
- * sequence holds (max_pages * page_size always does); a call with a smaller batch, fewer rows or keys may use it too.
+ * workspace: zt_attn_paged_workspace_bytes(batch, rows, max_keys, ...), 256-byte aligned, max_keys = max_pages * page_size; a call
+ * with a smaller batch, fewer rows or a smaller table may use it too.  Calls that may overlap on the GPU take one each.
  * Refusals of both: batch outside 1 .. 65535; degenerate pages; a width (n_kv_heads * dim) that is no multiple of four, heads that
  * are no group, a dim outside 32 .. 256 or no multiple of four; rows < 0; cu_rows NULL and rows != batch; null pointers; tensors off a 16-byte boundary; window or sinks < 0; a
  * missing, short or misaligned workspace.  rows 0 is nothing to do.

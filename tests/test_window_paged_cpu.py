@@ -76,6 +76,17 @@ def test_paged_workspace_size(zt, L):
             assert size(5, 200, keys if keys > 50 else 50, H, G, D) >= worst
 
 
+@pytest.mark.parametrize("H,G,D", [(32, 8, 128), (4, 2, 32), (16, 16, 64), (8, 2, 256), (12, 4, 96), (64, 1, 64), (300, 1, 32)])
+def test_paged_workspace_holds_a_step_over_any_part_of_the_keys(zt, L, H, G, D):
+    """A step over a window is planned for the keys that it sees: the plan of every smaller step fits."""
+    for B in (1, 2, 7, 30, 64, 300):
+        for keys in (1, 64, 129, 1000, 2047, 6145, 20000, 131072):
+            room = L.zt_attn_paged_workspace_bytes(B, B, keys, H, G, D)
+            for n in {keys, *(k for k in (1, 100, 128, 500, 769, 1025, 3000, 8000, 16385, 100000) if k < keys)}:
+                for b in {B, max(1, B // 2), 1}:
+                    assert L.zt_attn_decode_workspace_bytes(b, n, H, G, D) <= room, (b, n, keys)
+
+
 def test_python_calls_refuse_what_is_not_on_a_gpu(zt):
     x = torch.zeros(1, 4, 64)
     with pytest.raises(RuntimeError, match="no CPU path"):

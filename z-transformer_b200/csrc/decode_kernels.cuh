@@ -22,6 +22,7 @@
 // once each) plus q and out.
 #pragma once
 
+#include "paged_kernels.cuh"
 #include "zt_common.cuh"
 
 namespace zt {
@@ -42,6 +43,21 @@ struct DecodeParams {
     int cluster;  // blocks per cluster in the one-launch form
     long long cache_batch_stride;  // elements between two sequences' caches
     float scale_log2;
+    // Over pages (k_cache, v_cache are the pool's, n_ctx the most slots that the table holds), and where window > 0 over the
+    // sinks and the window alone.
+    Pages pg;
+    int window, sinks;
+};
+
+// The keys that a step over `nk` rows looks at, which are numbered through: the first `sinks` of them, then those from `skip` on.
+struct KeysSeen {
+    int n, sinks, skip;  // (key i stands at i, or from `sinks` on at i + skip)
+    __device__ __forceinline__ KeysSeen(const DecodeParams &p, int nk) {
+        const int low = p.window > 0 && nk > p.window ? nk - p.window : 0;
+        sinks = p.sinks < low ? p.sinks : low;
+        skip = low - sinks, n = nk - skip;
+    }
+    __device__ __forceinline__ int slot(int i) const { return i < sinks ? i : i + skip; }
 };
 
 // How many sequences name no valid prefix: counted by one block, so that nothing has to be cleared beforehand.
@@ -85,7 +101,9 @@ struct DecodeCfg {
 // The U GP dots of a step are summed over the lane group by exchanging halves -- V - 1 + log2(LPK / V) shuffles instead of
 // V log2(LPK) -- which leaves each lane the sum of one (key, head) pair; that lane alone takes the exponential and keeps
 // the head's maximum and its share of the denominator, and hands P out to the others.
-template <int LPK, int NCH, int GP, bool CLUSTER>
+// PAGED: the keys' rows lie in pages.  A lane group looks up its keys' pages a step before it asks for their rows: the look-up
+// is then never waited for.  A key on a page that is none makes its scores NaN: its slot is filled in place of a copy.
+template <int LPK, int NCH, int GP, bool CLUSTER, bool PAGED>
 __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<LPK, NCH, GP>::kMinBlocks)
     decode_splitk_kernel(const DecodeParams p) {
     using Cfg = DecodeCfg<LPK, NCH, GP>;
@@ -104,7 +122,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<LPK, NCH, GP>::kMinB
     pdl_wait();
     pdl_launch();
     const bool counts = CLUSTER && blockIdx.x == 0 && blockIdx.y == 0 && b == 0;  // (last of all: off every row's path)
-    const int nk = p.n_keys ? p.n_keys[b] : p.n_keys_all;
+    int nk = p.n_keys ? p.n_keys[b] : p.n_keys_all;
     if (nk < 1 || nk > p.n_ctx) {
         // decode.attnStep refuses an empty prefix (src/decode.zig:350); on the device the refusal is a NaN row plus
         // a count the host can read.  (Two launches: the combine kernel writes the rows.)
@@ -115,6 +133,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<LPK, NCH, GP>::kMinB
         if (counts) count_bad_sequences(p);
         return;  // (the whole cluster)
     }
+    const KeysSeen seen(p, nk);
+    if (PAGED) nk = seen.n;
     const int chunk = CLUSTER ? (nk + p.cluster - 1) / p.cluster : p.chunk;
     const int c0 = blockIdx.x * chunk;
     if (!CLUSTER && c0 >= nk) return;
@@ -131,20 +151,38 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<LPK, NCH, GP>::kMinB
     const int n_steps = c1 > c0 ? (c1 - c0 + NG * U - 1) / (NG * U) : 0;
     const float4 *ring = reinterpret_cast<const float4 *>(smem) + threadIdx.x;  // [S][U][NCH][2][threads]
     const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
+    // (PAGED) elements from the pool's begin to the rows of the next step to be fetched; -1: no page
+    long long rows[U];
+    const auto look_up = [&](int step) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (step * U + u) * NG;
+            rows[u] = i < n_mine ? p.pg.row(b, seen.slot(c0 + gi + i)) : 0;
+        }
+    };
     const auto fetch = [&](int step) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = (step * U + u) * NG;
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                const bool in = i < n_mine && li + LPK * c < n_chunks4;
-                const long long off = (long long)i * kvw + LPK * c * 4;
-                const uint32_t dst = ring_u32 + (uint32_t)((((step % S) * U + u) * NCH + c) * 2 * kDecodeThreads * 16);
-                copy16_async(dst, in ? kb + off : p.k_cache, in);
-                copy16_async(dst + kDecodeThreads * 16, in ? vb + off : p.v_cache, in);
+                const bool in = i < n_mine && li + LPK * c < n_chunks4 && !(PAGED && rows[u] < 0);
+                const long long off = PAGED ? rows[u] + (long long)g * dim + li * 4 + LPK * c * 4 : (long long)i * kvw + LPK * c * 4;
+                const float *kx = PAGED ? p.k_cache : kb, *vx = PAGED ? p.v_cache : vb;
+                const int at = (((step % S) * U + u) * NCH + c) * 2 * kDecodeThreads;
+                const uint32_t dst = ring_u32 + (uint32_t)(at * 16);
+                if (PAGED && rows[u] < 0) {
+                    const float nan = __int_as_float(0x7fc00000);
+                    reinterpret_cast<float4 *>(smem)[threadIdx.x + at] = make_float4(nan, nan, nan, nan);
+                } else {
+                    copy16_async(dst, in ? kx + off : p.k_cache, in);
+                }
+                copy16_async(dst + kDecodeThreads * 16, in ? vx + off : p.v_cache, in);
             }
         }
+        if (PAGED) look_up(step + 1);
     };
+    if (PAGED) look_up(0);
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) {
         if (i < n_steps) fetch(i);
@@ -362,7 +400,7 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const DecodeParams 
     pdl_wait();
     pdl_launch();
     const bool counts = h == 0 && b == 0;
-    const int nk = p.n_keys ? p.n_keys[b] : p.n_keys_all;
+    int nk = p.n_keys ? p.n_keys[b] : p.n_keys_all;
     float *orow = p.out + ((long long)b * p.n_heads + h) * p.dim;
     if (nk < 1 || nk > p.n_ctx) {
         for (int j = threadIdx.x; j < p.dim; j += blockDim.x) orow[j] = __int_as_float(0x7fc00000);
@@ -370,6 +408,7 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const DecodeParams 
         if (counts) count_bad_sequences(p);
         return;
     }
+    nk = KeysSeen(p, nk).n;
     const int nchunks = (nk + p.chunk - 1) / p.chunk;
     const long long slot0 = ((long long)b * p.n_heads + h) * p.max_chunks;
     float mx = -INFINITY;
@@ -479,13 +518,27 @@ inline DecodePlan decode_plan(int batch, int n_ctx, int n_heads, int n_kv_heads,
     return pl;
 }
 
+// The most bytes of a plan's workspace over all calls of at most `batch` sequences and `n_ctx` keys: a chunk holds 128 keys at least, and
+// where it holds fewer than 1024 there are no more blocks than decode_plan aims at, with one over for every sequence.
+inline size_t decode_bytes_bound(int batch, int n_ctx, int n_heads, int n_kv_heads, int dim) {
+    const DecodePlan one = decode_plan(1, 1, n_heads, n_kv_heads, dim);
+    const DeviceInfo *di = device_info();
+    const long long sms = di && di->sm_count > 0 ? di->sm_count : 148, passes = (long long)n_kv_heads * one.n_sub;
+    const long long by_keys = (long long)batch * ((n_ctx + 127) / 128), long_chunks = (long long)batch * ((n_ctx + 1023) / 1024);
+    long long chunks = (8 * sms + passes - 1) / passes + 2LL * batch;
+    if (chunks < long_chunks) chunks = long_chunks;
+    if (chunks > by_keys) chunks = by_keys;
+    return kDecodeHeaderBytes + 256 + (size_t)chunks * n_heads * (sizeof(float2) + (size_t)dim * sizeof(float));
+}
+
 template <int LPK, int NCH, int GP>
 inline int launch_decode_inst(const DecodeParams &p, cudaStream_t stream) {
     using Cfg = DecodeCfg<LPK, NCH, GP>;
     size_t smem = (size_t)Cfg::kStages * Cfg::kStageBytes;
     const size_t merge = (size_t)(kDecodeThreads / 32 + 1) * GP * (p.dim + 4) * sizeof(float);
     if (smem < merge) smem = merge;
-    const auto kernel = p.cluster ? decode_splitk_kernel<LPK, NCH, GP, true> : decode_splitk_kernel<LPK, NCH, GP, false>;
+    const auto kernel = p.pg.table ? (p.cluster ? decode_splitk_kernel<LPK, NCH, GP, true, true> : decode_splitk_kernel<LPK, NCH, GP, false, true>)
+                                   : (p.cluster ? decode_splitk_kernel<LPK, NCH, GP, true, false> : decode_splitk_kernel<LPK, NCH, GP, false, false>);
     if (optin_smem((const void *)kernel, smem)) return 1;
     const dim3 grid((unsigned)(p.cluster ? p.cluster : p.max_chunks), (unsigned)(p.n_kv_heads * p.n_sub), (unsigned)p.batch);
     if (p.cluster) return launch_pdl_cluster("decode_splitk_kernel", kernel, grid, dim3(kDecodeThreads), smem, stream, p.cluster, p);

@@ -18,13 +18,25 @@ struct Pages {
     const float *k, *v;  // [n_pages, page_size, width]
     const int *table;    // [batch, max_pages]
     int n_pages, page_size, max_pages, width;
+    uint32_t per;  // j / page_size is j * per >> shift for every j below 2^31
+    int shift;
     // Elements from the pool's begin to the row of slot j of sequence b; negative where the table names no page for it.
     __device__ __forceinline__ long long row(int b, int j) const {
-        const int slot = j / page_size, id = table[(long long)b * max_pages + slot];
+        const int slot = page_of(j), id = table[(long long)b * max_pages + slot];
         return id < 0 || id >= n_pages ? -1 : ((long long)id * page_size + (j - slot * page_size)) * width;
     }
+    __device__ __forceinline__ int page_of(int j) const { return (int)(((uint64_t)(uint32_t)j * per) >> shift); }
     __device__ __forceinline__ long long capacity() const { return (long long)max_pages * page_size; }
 };
+
+// With L bits to hold page_size - 1 and `per` 2^(31 + L) / page_size rounded up, per page_size is at most 2^L over 2^(31 + L), so
+// that j times the excess stays below one quotient's worth for 31 bits of j; `per` itself is below 2^32.
+inline Pages make_pages(const float *k, const float *v, const int *table, int n_pages, int page_size, int max_pages, int width) {
+    Pages p{k, v, table, n_pages, page_size, max_pages, width, 0, 31};
+    while ((1LL << (p.shift - 31)) < page_size) ++p.shift;
+    p.per = (uint32_t)(((1ull << p.shift) + (uint64_t)page_size - 1) / (uint64_t)page_size);
+    return p;
+}
 
 // What a query at position p sees; `window` 0: everything up to itself.
 struct Seen {

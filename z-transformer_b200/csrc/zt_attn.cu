@@ -1213,7 +1213,7 @@ int zt_kv_append_paged(float *k_pages, float *v_pages, const int *table, int *n_
         if (!aligned16(t)) return refuse("the pages and the new rows must be 16-byte aligned.");
     if (need_device()) return 1;
     AppendParams p{};
-    p.pg = Pages{k_pages, v_pages, table, n_pages, page_size, max_pages, width};
+    p.pg = make_pages(k_pages, v_pages, table, n_pages, page_size, max_pages, width);
     p.k_pages = k_pages, p.v_pages = v_pages, p.k_new = k_new, p.v_new = v_new;
     p.n_keys = n_keys, p.skipped = skipped, p.cu_rows = cu_rows, p.batch = batch, p.rows = rows;
     g_last_path = "kv-append";
@@ -1223,7 +1223,7 @@ int zt_kv_append_paged(float *k_pages, float *v_pages, const int *table, int *n_
 size_t zt_attn_paged_workspace_bytes(int batch, int rows, int max_keys, int n_heads, int n_kv_heads, int dim) {
     if (batch < 1 || rows < 0 || max_keys < 1 || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || !zt_attn_dim_ok(dim) || dim % 4 != 0)
         return 0;
-    return kPagedHeaderBytes;
+    return decode_bytes_bound(batch, max_keys, n_heads, n_kv_heads, dim);
 }
 
 int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, const int *n_keys,
@@ -1242,12 +1242,25 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
         if (!aligned16(t)) return refuse("q, out and the pages must be 16-byte aligned.");
     if (need_device()) return 1;
     if (rows == 0) return 0;
+    const int capacity = max_pages * page_size;
+    if (window == 0 || window >= capacity) window = sinks = 0;
+    if (!cu_rows) {
+        // one row a sequence: split over the keys that it sees
+        const int seen = window > 0 && sinks < capacity - window ? window + sinks : capacity;
+        DecodeParams d{};
+        d.q = q, d.k_cache = k_pages, d.v_cache = v_pages, d.n_keys = n_keys, d.out = out, d.lse = lse;
+        d.batch = batch, d.n_ctx = capacity, d.n_heads = n_heads, d.n_kv_heads = n_kv_heads, d.dim = dim;
+        d.scale_log2 = kLog2e / sqrtf((float)dim);
+        d.pg = make_pages(k_pages, v_pages, table, n_pages, page_size, max_pages, n_kv_heads * dim);
+        d.window = window, d.sinks = sinks;
+        return launch_decode(d, decode_plan(batch, seen, n_heads, n_kv_heads, dim), workspace, (cudaStream_t)stream);
+    }
     PagedParams p{};
-    p.pg = Pages{k_pages, v_pages, table, n_pages, page_size, max_pages, n_kv_heads * dim};
+    p.pg = make_pages(k_pages, v_pages, table, n_pages, page_size, max_pages, n_kv_heads * dim);
     p.q = q, p.n_keys = n_keys, p.cu_rows = cu_rows, p.out = out, p.lse = lse;
     p.bad_count = static_cast<int *>(workspace);
     p.batch = batch, p.rows = rows, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.dim = dim;
-    p.seen = window == 0 || window >= max_pages * page_size ? Seen{0, 0} : Seen{window, sinks};
+    p.seen = Seen{window, sinks};
     p.scale_log2 = kLog2e / sqrtf((float)dim);
     return launch_paged_rows(p, (cudaStream_t)stream);
 }
