@@ -1,6 +1,6 @@
 // A KV cache of pages: rows of keys and values in fixed-size pages of a pool that all sequences share, a table that names
-// every sequence's pages in order, and the kernels over it -- the append of new rows and the attention of new rows over
-// all rows so far.
+// every sequence's pages in order, and the append of new rows.  (Their attention: decode_kernels.cuh for one new row a sequence,
+// tc_rows.cuh for more.)
 //
 // Key slot j of sequence b is row j % page_size of page table[b, j / page_size]; a page's row holds n_kv_heads * dim
 // floats.  New rows are ragged: sequence b has rows [cu_rows[b], cu_rows[b + 1]) of the new tensors (one each where
@@ -135,92 +135,6 @@ inline int launch_append_paged(const AppendParams &p, cudaStream_t stream) {
     if (p.rows > 0 && launch_pdl("append_paged_kernel", append_paged_kernel, dim3((unsigned)p.rows), dim3(256), 0, stream, p)) return 1;
     if (!p.cu_rows) return 0;
     return launch_pdl("advance_kernel", advance_kernel, dim3((unsigned)p.batch), dim3(128), 0, stream, p);
-}
-
-// ---- attention -------------------------------------------------------------------------------------------------------
-
-constexpr int kPagedHeaderBytes = 256;  // of a workspace: how many sequences were bad
-
-struct PagedParams {
-    Pages pg;
-    const float *q;
-    const int *n_keys, *cu_rows;
-    float *out, *lse;  // lse may be null
-    int *bad_count;
-    int batch, rows, n_heads, n_kv_heads, dim;
-    Seen seen;
-    float scale_log2;
-};
-
-// Counted by one block, so that nothing has to be cleared beforehand.
-__device__ __forceinline__ void count_bad_rows(const PagedParams &p) {
-    __shared__ int total;
-    if (threadIdx.x == 0) total = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.batch; i += blockDim.x)
-        if (new_rows(p.cu_rows, p.n_keys, i, p.rows, p.pg, true).bad) atomicAdd(&total, 1);
-    __syncthreads();
-    if (threadIdx.x == 0) *p.bad_count = total;
-}
-
-// The formula as it stands: a block per (new row, head), whose four warps take the keys in turn, the head's columns across
-// a warp's lanes, and merge their partial softmaxes through shared memory.
-__global__ void __launch_bounds__(128) attn_paged_rows(const PagedParams p) {
-    constexpr int W = 4, C = 8;  // warps; columns a lane holds of a head of up to 256
-    __shared__ int found;
-    __shared__ float sm[W], sl[W], so[W][C * 32];
-    pdl_wait();
-    pdl_launch();
-    if (blockIdx.x == 0 && blockIdx.y == 0) count_bad_rows(p);
-    const int row = blockIdx.x, h = blockIdx.y, g = h / (p.n_heads / p.n_kv_heads);
-    const int b = sequence_of(p.cu_rows, p.batch, row, &found);
-    if (b < 0) return;
-    const NewRows r = new_rows(p.cu_rows, p.n_keys, b, p.rows, p.pg, true);
-    const long long head = (long long)row * p.n_heads + h;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float nan = __int_as_float(0x7fc00000);
-    if (r.bad) {
-        for (int j = threadIdx.x; j < p.dim; j += 128) p.out[head * p.dim + j] = nan;
-        if (p.lse && threadIdx.x == 0) p.lse[head] = nan;
-        return;
-    }
-    const int pos = r.pos + (row - r.begin);
-    float q[C], o[C], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) q[c] = lane + 32 * c < p.dim ? p.q[head * p.dim + lane + 32 * c] * p.scale_log2 : 0.f, o[c] = 0.f;
-    for (int key = warp; key <= pos; key += W) {
-        if (!p.seen(key, pos)) continue;
-        const long long at = p.pg.row(b, key);
-        float s = 0.f;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (lane + 32 * c < p.dim && at >= 0) s = fmaf(q[c], p.pg.k[at + g * p.dim + lane + 32 * c], s);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        if (at < 0) s = nan;  // a key on no page
-        const float top = fmaxf(m, s), keep = m == -INFINITY ? 0.f : ex2(m - top), w = ex2(s - top);
-        l = fmaf(l, keep, w), m = top;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (lane + 32 * c < p.dim) o[c] = fmaf(o[c], keep, at >= 0 ? w * p.pg.v[at + g * p.dim + lane + 32 * c] : w);
-    }
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-    for (int c = 0; c < C; ++c) so[warp][lane + 32 * c] = o[c];
-    __syncthreads();
-    float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w]);
-    for (int w = 0; w < W; ++w) sum += sm[w] == -INFINITY && sl[w] == 0.f ? 0.f : sl[w] * ex2(sm[w] - top);
-    for (int j = threadIdx.x; j < p.dim; j += 128) {
-        float x = 0.f;
-        for (int w = 0; w < W; ++w) x += sm[w] == -INFINITY && sl[w] == 0.f ? 0.f : so[w][j] * ex2(sm[w] - top);
-        p.out[head * p.dim + j] = x / sum;
-    }
-    if (p.lse && threadIdx.x == 0) p.lse[head] = (top + log2f(sum)) * kLn2;
-}
-inline int launch_paged_rows(const PagedParams &p, cudaStream_t stream) {
-    g_last_path = "paged-rows";
-    return launch_pdl("attn_paged_rows", attn_paged_rows, dim3((unsigned)p.rows, (unsigned)p.n_heads), dim3(128), 0, stream, p);
 }
 
 }  // namespace zt

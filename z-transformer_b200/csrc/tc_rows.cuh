@@ -1,0 +1,628 @@
+// Attention of rows over the keys that they see -- the last rows of sequences whose keys lie in pages (attention_paged), or
+// whole sequences with a window (attention_forward_window) -- on the tensor cores, straight from the f32 keys and values.
+//
+//     S = q k^T / sqrt(dim),  P = softmax over the seen keys of each row,  out = P v,  lse = max + ln(denominator)
+//
+// with the arithmetic of tc_fwd16.cuh: every operand is split into two f16 pieces and every product is three MMAs.  What is
+// different:
+//   rows    A tile's 128 rows are (token, head of the KV group) pairs, token by token: sixteen tokens of eight heads see the
+//           same keys, so a short chunk fills a tile, and a window of W keys costs a tile W + 128 / group keys and not W + 128.
+//   keys    come as they are.  Four warps copy a tile's rows into shared memory (cp.async, row by row: each has its page),
+//           find the tile's largest magnitude and write the pieces, scaled by a power of two of the tile's own, as the
+//           operand tiles that the MMAs read.  No launch before this one converts anything and nothing is kept in memory.
+//   scales  K's goes into the tile's scores; V's, and the reference maximum of the tile's exponentials, into the factor with
+//           which the row threads add the tile's P V to the row: O leaves TMEM after every tile and is summed in registers,
+//           with rounding (the tensor core adds with truncation, 2.3e-7 of O for every 64 keys: over a long prefix that is the
+//           largest error of all; see kFlushKeyTiles).
+//   masks   Which key tiles a CTA visits follows from its first and last position: the sinks' and the window's.  A key that
+//           no row of the tile sees is not read and counts as zero.  A value that is not finite does not enter the product,
+//           where a weight of zero would not keep it from a row that does not see it: the row threads add it to those that do.
+// Roles, 16 warps: two sets of four row warps -- set j & 1 makes P of tile j, each set sums one half of the columns of every
+// tile --, four converting warps, a warp that issues S and one that issues P V (a thread issues an MMA of N <= 64 every 50
+// clocks, the pipe takes one every 32), two idle ones that make the four a group for setmaxnreg.
+// TMEM: up to 128 columns Q hi, Q lo, two O and two S/P buffers; above, Q hi, one O and two S/P buffers of 32 keys, Q lo in
+// shared memory.
+#pragma once
+
+#include "paged_kernels.cuh"
+#include "tc_fwd16.cuh"
+
+namespace zt {
+namespace tcr {
+
+using namespace tc;
+using tcb::block_mult;
+using tcb::split_pack;
+using tcb::floats2;
+using tcb::fma2;
+using tcb::mul2;
+using tcf16::max_abs4;
+using tcf16::row_exp32;
+using tcf16::row_max32;
+using tcf16::split_q32;
+using tcf16::store_q_piece;
+
+constexpr int kThreads = 512, kConvert = 128;  // threads of a CTA; of them those that convert
+
+template <int TD>
+struct Cfg {
+    static constexpr bool kWide = TD > 128;
+    static constexpr int BN = kWide ? 32 : 64;      // keys of a tile
+    static constexpr int OB = kWide ? 1 : 2;        // O buffers
+    static constexpr int KS = TD == 256 ? 1 : 2, VS = KS;  // slots of converted K and V tiles
+    static constexpr int SU = 2;                    // slots of tiles as they come
+    static constexpr int KP = BN * TD * 2;          // bytes of one piece of a tile
+    static constexpr int RAW = BN * TD * 4;
+    static constexpr int QL = kWide ? 128 * TD * 2 : 0;
+    static constexpr int CHUNKS = BN * TD / 4 / kConvert;  // 16-byte chunks a converting thread has of a tile
+    // registers a thread: the launch gives 512 threads 128 each
+    static constexpr int kRowRegs = kWide ? 200 : 184, kConvertRegs = kWide ? 72 : 104, kIssueRegs = 40;
+    static_assert(256 * kRowRegs + 128 * (kConvertRegs + kIssueRegs) <= kThreads * 128, "the groups share what the launch has");
+    static constexpr int cQh = 0, cQl = TD / 2, cO = kWide ? 128 : TD, cS = kWide ? 384 : 3 * TD;
+    static constexpr int kData = KS * 2 * KP + VS * 2 * KP + SU * RAW + QL;
+    static_assert(128 * (TD * 4 + 16) <= kData, "the finished rows are staged where the tiles were");
+};
+
+struct Shared {
+    uint64_t k_full[2], k_free[2], v_full[2], v_free[2], a_ready, s_full[2], p_full[2], pv_done[2], o_full[2], o_free[2];
+    uint32_t tmem_base;
+    volatile int abort;
+    int found;
+    float mk[4], mv[4];         // the scales of tiles j & 3
+    uint32_t odd[8][2];         // which values' rows of tile j & 7 hold something that is not finite
+    uint32_t top[2][4];         // per converting warp: max |x| of the unit
+    float m_ref[4][128];        // the rows' reference maxima of tile j & 3
+    float fin_m[2][128], fin_l[2][128], q_top[2][128];
+    long long row[4][64];       // of tile j & 3: elements to every key's row; kNone: counts as zero; kNoPage: NaN
+};
+constexpr long long kNone = -1, kNoPage = -2;
+
+struct Params {
+    const float *q, *k, *v;  // k, v: the pool's, or [batch, T, width]
+    Pages pg;                // (table null: whole sequences of T rows)
+    const int *n_keys, *cu_rows;
+    int *bad_count;
+    float *out, *lse;        // with parts: the parts', out_part and lse_part elements from one to the next
+    long long out_part, lse_part;
+    int batch, rows, T, n_heads, n_kv_heads, dim, parts;
+    Seen seen;
+    float scale_log2;
+};
+
+__device__ __forceinline__ bool rwait(uint64_t *bar, uint32_t parity, Shared *sh) {
+    for (uint32_t i = 0; i < (1u << 20); ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255u) == 255u && sh->abort) return false;
+    }
+    return false;
+}
+__device__ __forceinline__ void rgive_up(Shared *sh, int code) {
+    sh->abort = code;
+    atomicMax(&g_tc_status, code);
+}
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// The key tiles that the rows at positions [first, last] visit, numbered through: those with sinks, then the window's.
+struct Tiles {
+    int n, sink_tiles, skip;
+    __device__ __forceinline__ Tiles(const Seen &s, int first, int last, int BN) {
+        const int end = last / BN + 1;
+        const int low = s.window > 0 && first >= s.window ? (first - s.window + 1) / BN : 0;
+        const int sinks = s.window > 0 ? (int)(((long long)s.sinks + BN - 1) / BN) : 0;
+        sink_tiles = sinks < low ? sinks : low;
+        skip = low - sink_tiles, n = end - skip;
+    }
+    __device__ __forceinline__ int at(int j) const { return j < sink_tiles ? j : j + skip; }
+};
+
+// The rows of a tile: flat rows [f0, f0 + 128) of a sequence's (token, head of the group) pairs.
+struct RowTile {
+    int b, begin, count, pos;  // sequence; its first row in q, its rows, the first one's position
+    int f0;
+    bool bad;
+};
+
+template <int TD, bool PAGED>
+__global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
+    using C = Cfg<TD>;
+    constexpr int BN = C::BN, KP = C::KP, KS = C::KS, VS = C::VS, OB = C::OB, SU = C::SU;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *sK = smem, *sV = sK + KS * 2 * KP, *sRaw = sV + VS * 2 * KP, *sQl = sRaw + SU * C::RAW;
+    Shared *sh = reinterpret_cast<Shared *>(sQl + C::QL);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = p.n_heads / p.n_kv_heads;
+    const int g = blockIdx.y, part = blockIdx.z;
+    const int slot = (int)(gridDim.x - 1 - blockIdx.x);  // (of whole sequences the late tiles, which see the most, start first)
+
+    pdl_wait();
+    RowTile t{};
+    if (PAGED) {
+        if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && warp == 15) {
+            int bad = 0;
+            for (int i = lane; i < p.batch; i += 32) bad += new_rows(p.cu_rows, p.n_keys, i, p.rows, p.pg, true).bad;
+            bad = __reduce_add_sync(0xffffffffu, bad);
+            if (lane == 0) *p.bad_count = bad;
+        }
+        // Sequence b has the tiles from floor(cu_rows[b] group / 128) + b on: as many as it needs, or one more.
+        if (threadIdx.x == 0) sh->found = -1;
+        __syncthreads();
+        const auto clipped = [&](int i) { const int c = p.cu_rows[i]; return c < 0 ? 0 : (c > p.rows ? p.rows : c); };
+        const auto first_tile = [&](int i) { return (int)((long long)clipped(i) * group / 128) + i; };
+        for (int i = threadIdx.x; i < p.batch; i += kThreads)
+            if (first_tile(i) <= slot && slot < first_tile(i + 1)) atomicMax(&sh->found, i);
+        __syncthreads();
+        t.b = sh->found;
+        if (t.b < 0) return;
+        const NewRows r = new_rows(p.cu_rows, p.n_keys, t.b, p.rows, p.pg, true);
+        t.begin = clipped(t.b), t.count = clipped(t.b + 1) - t.begin, t.pos = r.pos, t.bad = r.bad;
+        t.f0 = (slot - first_tile(t.b)) * 128;
+    } else {
+        const int per = (int)(((long long)p.T * group + 127) / 128);
+        t.b = slot / per, t.begin = t.b * p.T, t.count = p.T, t.f0 = (slot - t.b * per) * 128;
+    }
+    const long long flat = (long long)t.count * group;
+    if (t.f0 >= flat) return;
+    const int n_rows = flat - t.f0 < 128 ? (int)(flat - t.f0) : 128;
+    // a row's place in q, out and lse
+    const auto row_head = [&](int r) -> long long {
+        const int f = t.f0 + r, i = f / group;
+        return (long long)(t.begin + i) * p.n_heads + g * group + (f - i * group);
+    };
+    if (PAGED && t.bad) {
+        const float nan = __int_as_float(0x7fc00000);
+        for (int i = threadIdx.x; i < n_rows * p.dim; i += kThreads) {
+            const int r = i / p.dim;
+            p.out[part * p.out_part + row_head(r) * p.dim + (i - r * p.dim)] = nan;
+        }
+        if (p.lse && threadIdx.x < n_rows) p.lse[part * p.lse_part + row_head(threadIdx.x)] = nan;
+        return;
+    }
+    const int pos_first = t.pos + t.f0 / group, pos_last = t.pos + (t.f0 + n_rows - 1) / group;
+    const Tiles tiles(p.seen, pos_first, pos_last, BN);
+    int n = tiles.n, jb = 0;  // key tiles of this CTA, and the first of them
+    if (p.parts > 1) {
+        const int per = (n + p.parts - 1) / p.parts;
+        jb = part * per;
+        n = n - jb < per ? n - jb : per;
+        if (n <= 0) {
+            if (threadIdx.x < n_rows) p.lse[part * p.lse_part + row_head(threadIdx.x)] = -INFINITY;
+            return;
+        }
+    }
+    const auto key0 = [&](int j) { return tiles.at(jb + j) * BN; };
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->k_full[i], kConvert / 32), mbar_init(&sh->k_free[i], 1);
+            mbar_init(&sh->v_full[i], kConvert / 32), mbar_init(&sh->v_free[i], 1);
+            mbar_init(&sh->s_full[i], 1), mbar_init(&sh->p_full[i], 4), mbar_init(&sh->pv_done[i], 1);
+            mbar_init(&sh->o_full[i], 1), mbar_init(&sh->o_free[i], 8);
+        }
+        mbar_init(&sh->a_ready, 8);
+        sh->abort = (smem_u32(smem) & 1023u) ? 100 : 0;
+        if (sh->abort) atomicMax(&g_tc_status, 100);
+        mbar_fence_init();
+    }
+    if (warp == 12) tmem_alloc(&sh->tmem_base, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem_base;
+    const int steps = head_steps(p.dim);
+
+    if (warp >= 12) {
+        fewer_registers<C::kIssueRegs>();
+        if (warp == 12) {
+            // -------------------------------------------------------------- S(j) = Q K^T into buffer j & 1
+            if (elect_one()) {
+                constexpr uint32_t id_s = idesc_f16(128, BN, false, false);
+                bool ok = rwait(&sh->a_ready, 0, sh);
+                if (!ok) rgive_up(sh, 101);
+                const uint32_t k_u32 = smem_u32(sK), ql_u32 = smem_u32(sQl);
+                for (int j = 0; ok && j < n; ++j) {
+                    const int s = j % KS;
+                    // (over P(j - 2), which its product has read)
+                    if (!rwait(&sh->k_full[s], (uint32_t)((j / KS) & 1), sh) ||
+                        (j >= 2 && !rwait(&sh->pv_done[j & 1], (uint32_t)(((j >> 1) - 1) & 1), sh))) { rgive_up(sh, 102); break; }
+                    tc_fence_after();
+                    const uint32_t cS = C::cS + (j & 1) * BN;
+                    const uint64_t bkh = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP)), bkl = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP + KP));
+                    const uint64_t bql = desc_kmajor(ql_u32);
+#pragma unroll
+                    for (int kk = 0; kk < TD / 16; ++kk) {
+                        if (kk >= steps) break;
+                        const uint32_t bo = (uint32_t)((kk >> 2) * (BN * 128) + (kk & 3) * 32);
+                        const uint64_t dkh = desc_advance(bkh, bo), dkl = desc_advance(bkl, bo);
+                        mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, dkh, id_s, kk > 0);
+                        mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, dkl, id_s, 1);
+                        if (C::kWide) mma_ss_f16(tmem + cS, desc_advance(bql, (uint32_t)((kk >> 2) * (128 * 128) + (kk & 3) * 32)), dkh, id_s, 1);
+                        else mma_ts_f16(tmem + cS, tmem + C::cQl + kk * 8, dkh, id_s, 1);
+                    }
+                    mma_commit(&sh->k_free[s]);
+                    mma_commit(&sh->s_full[j & 1]);
+                }
+            }
+            __syncwarp();
+        } else if (warp == 13) {
+            // -------------------------------------------------------------- O(j) = P(j) V
+            if (elect_one()) {
+                const uint32_t id_o = idesc_f16(128, 16 * steps, false, true);
+                const uint32_t v_u32 = smem_u32(sV);
+                for (int j = 0; j < n; ++j) {
+                    const int s = j % VS, ob = j % OB;
+                    if (!rwait(&sh->p_full[j & 1], (uint32_t)((j >> 1) & 1), sh) || !rwait(&sh->v_full[s], (uint32_t)((j / VS) & 1), sh) ||
+                        (j >= OB && !rwait(&sh->o_free[ob], (uint32_t)((j / OB - 1) & 1), sh))) { rgive_up(sh, 103); break; }
+                    tc_fence_after();
+                    const uint32_t vh = v_u32 + (uint32_t)(s * 2 * KP);
+                    const uint64_t mvh = desc_mnmajor_16b(vh, BN * 128), mvl = desc_mnmajor_16b(vh + KP, BN * 128);
+                    const uint32_t cS = C::cS + (j & 1) * BN, cO = C::cO + ob * TD;
+#pragma unroll
+                    for (int kk = 0; kk < BN / 16; ++kk) {
+                        const uint32_t ac = (uint32_t)(32 * (kk >> 1) + (kk & 1) * 8);
+                        const uint64_t dvh = desc_advance(mvh, kk * 2048), dvl = desc_advance(mvl, kk * 2048);
+                        mma_ts_f16(tmem + cO, tmem + cS + ac, dvh, id_o, kk > 0);
+                        mma_ts_f16(tmem + cO, tmem + cS + ac, dvl, id_o, 1);
+                        mma_ts_f16(tmem + cO, tmem + cS + ac + 16, dvh, id_o, 1);
+                    }
+                    mma_commit(&sh->v_free[s]);
+                    mma_commit(&sh->o_full[ob]);
+                    mma_commit(&sh->pv_done[j & 1]);
+                }
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 8) {
+        // ------------------------------------------------------------------ keys and values: copied, scaled, split.  The units
+        // go in the order in which the MMAs ask for them: K0, K1, V0, K2, V1, ...
+        fewer_registers<C::kConvertRegs>();
+        const int ct = threadIdx.x - 256, cw = warp - 8;
+        constexpr int CPR = TD / 4;  // chunks of a row
+        const int n_units = 2 * n;
+        const long long width = PAGED ? p.pg.width : (long long)p.n_kv_heads * p.dim;
+        const auto tile_of = [&](int u, bool &is_k) {
+            is_k = u == 0 || ((u & 1) && u != n_units - 1);
+            return u == 0 ? 0 : (is_k ? (u + 1) >> 1 : (u == n_units - 1 ? n - 1 : (u >> 1) - 1));
+        };
+        // where the keys of tile j lie; one that no row of this CTA sees counts as zero
+        const auto look_up = [&](int j) {
+            if (ct >= BN || j >= n) return;
+            const int key = key0(j) + ct;
+            long long at = kNone;
+            if (key <= pos_last && (p.seen.window == 0 || key > pos_first - p.seen.window || key < p.seen.sinks)) {
+                at = PAGED ? p.pg.row(t.b, key) : ((long long)t.b * p.T + key) * width;
+                if (at < 0) at = kNoPage;
+            }
+            sh->row[j & 3][ct] = at;
+        };
+        const auto copy_unit = [&](int u) {
+            if (u < n_units) {
+                bool is_k;
+                const int j = tile_of(u, is_k);
+                const float *base = is_k ? p.k : p.v;
+                const uint32_t dst = smem_u32(sRaw + (u % SU) * C::RAW) + (uint32_t)ct * 16;
+#pragma unroll
+                for (int i = 0; i < C::CHUNKS; ++i) {
+                    const int f = i * kConvert + ct, r = f / CPR, c = f - r * CPR;
+                    const long long at = sh->row[j & 3][r];
+                    const bool in = at >= 0 && c * 4 < p.dim;
+                    copy16_async(dst + i * (kConvert * 16), in ? base + at + (long long)g * p.dim + c * 4 : base, in);
+                }
+            }
+            copy_async_commit();
+        };
+        look_up(0), look_up(1);
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+        for (int u = 0; u < SU; ++u) copy_unit(u);
+        bool ok = true;
+        for (int u = 0; u < n_units; ++u) {
+            bool is_k;
+            const int j = tile_of(u, is_k);
+            copy_async_wait<SU - 1>();
+            const float4 *raw = reinterpret_cast<const float4 *>(sRaw + (u % SU) * C::RAW) + ct;
+            if (ct < 2 && is_k) sh->odd[j & 7][ct] = 0;  // (of V, whose unit comes later)
+            uint32_t top = 0, seen_bits = 0;
+#pragma unroll
+            for (int i = 0; i < C::CHUNKS; ++i) {
+                const float4 x = raw[i * kConvert];
+                top = max(max(top, __float_as_uint(x.x) & 0x7fffffffu), __float_as_uint(x.y) & 0x7fffffffu);
+                top = max(max(top, __float_as_uint(x.z) & 0x7fffffffu), __float_as_uint(x.w) & 0x7fffffffu);
+            }
+            seen_bits = top;
+            if (seen_bits >= 0x7f800000u) {  // something is not finite: the largest of what is; rows of V are noted
+                top = 0;
+#pragma unroll 1
+                for (int i = 0; i < C::CHUNKS; ++i) {
+                    const float4 x = raw[i * kConvert];
+                    const int r = (i * kConvert + ct) / CPR;
+                    for (const float e : {x.x, x.y, x.z, x.w}) {
+                        if (finite(e)) top = max(top, __float_as_uint(e) & 0x7fffffffu);
+                        else if (!is_k) atomicOr(&sh->odd[j & 7][r >> 5], 1u << (r & 31));
+                    }
+                }
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) sh->top[u & 1][cw] = top;
+            if (u & 1) look_up(((u + 1) >> 1) + (SU + 1) / 2);
+            asm volatile("bar.sync 2, 128;" ::: "memory");
+            const float m = block_mult(max(max(sh->top[u & 1][0], sh->top[u & 1][1]), max(sh->top[u & 1][2], sh->top[u & 1][3])));
+            const int s = is_k ? j % KS : j % VS, S = is_k ? KS : VS;
+            if (ok && j >= S && !__all_sync(0xffffffffu, rwait(is_k ? &sh->k_free[s] : &sh->v_free[s], (uint32_t)((j / S - 1) & 1), sh))) {
+                rgive_up(sh, 104);
+                ok = false;
+            }
+            if (!ok) continue;  // (on to the barriers that the other warps wait at)
+            uint8_t *dst = (is_k ? sK : sV) + s * 2 * KP;
+            if (ct == 0) (is_k ? sh->mk : sh->mv)[j & 3] = m;
+#pragma unroll
+            for (int i = 0; i < C::CHUNKS; ++i) {
+                const int f = i * kConvert + ct, r = f / CPR, c = f - r * CPR;
+                float4 x = raw[i * kConvert];
+                if (is_k) {
+                    if (sh->row[j & 3][r] == kNoPage) x.x = __int_as_float(0x7fc00000);
+                } else if (seen_bits >= 0x7f800000u) {
+                    x.x = finite(x.x) ? x.x : 0.f, x.y = finite(x.y) ? x.y : 0.f, x.z = finite(x.z) ? x.z : 0.f, x.w = finite(x.w) ? x.w : 0.f;
+                }
+                const float2 mm = make_float2(m, m);
+                uint2 h, l;
+                split_pack(mul2(make_float2(x.x, x.y), mm), h.x, l.x);
+                split_pack(mul2(make_float2(x.z, x.w), mm), h.y, l.y);
+                // 64-column block, row, 16-byte chunk of eight halves with the 128-byte swizzle, its first or second half
+                uint8_t *at = dst + (c >> 4) * (BN * 128) + r * 128 + ((((c & 15) >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
+                *reinterpret_cast<uint2 *>(at) = h;
+                *reinterpret_cast<uint2 *>(at + KP) = l;
+            }
+            fence_async_smem();
+            mbar_arrive_warp(is_k ? &sh->k_full[s] : &sh->v_full[s]);
+            copy_unit(u + SU);  // (into the slot that this thread has just read its own chunks out of)
+        }
+        copy_async_wait<0>();
+    } else {
+        // ------------------------------------------------------------------ rows
+        more_registers<C::kRowRegs>();
+        const int tid = threadIdx.x & 127, set = threadIdx.x >> 7;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const bool mine = tid < n_rows;
+        const int pos = t.pos + (t.f0 + (mine ? tid : n_rows - 1)) / group;  // (rows past the last repeat it, with q zero)
+        const long long rh = mine ? row_head(tid) : 0;
+        bool ok = true;
+        float cs0;  // scale_log2 over the row's scale
+        {
+            float4 x[TD / 8];
+            float top = 0.f;
+#pragma unroll
+            for (int c = 0; c < TD / 8; ++c) {
+                const int col = set * (TD / 2) + c * 4;
+                x[c] = mine && col < p.dim ? *reinterpret_cast<const float4 *>(p.q + rh * p.dim + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                top = fmaxf(top, max_abs4(x[c]));
+            }
+            sh->q_top[set][tid] = top;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            top = fmaxf(top, sh->q_top[set ^ 1][tid]);
+            const float m = block_mult(__float_as_uint(top));
+            cs0 = p.scale_log2 / m;
+#pragma unroll
+            for (int cb = 0; cb < TD / 64; ++cb) {
+                uint32_t qh[16], ql[16];
+                split_q32([&](int c) { return x[cb * 8 + c]; }, m, qh, ql);
+                tmem_st16(tmem + lane_base + C::cQh + set * (TD / 4) + cb * 16, qh);
+                if (C::kWide) store_q_piece(sQl, tid, set * (TD / 64) + cb, ql);
+                else tmem_st16(tmem + lane_base + C::cQl + set * (TD / 4) + cb * 16, ql);
+            }
+            tmem_wait_st();
+            if (C::kWide) fence_async_smem();
+            tc_fence_before();
+            mbar_arrive_warp(&sh->a_ready);
+        }
+        float2 o[TD / 4];  // this set's half of the row's columns, relative to m_o
+#pragma unroll
+        for (int c = 0; c < TD / 4; ++c) o[c] = make_float2(0.f, 0.f);
+        float m_o = -INFINITY, m_ref = -INFINITY, l = 0.f;
+        // adds tile j's P V to the row
+        const auto add_tile = [&](int j) -> bool {
+            const int ob = j % OB;
+            if (!__all_sync(0xffffffffu, rwait(&sh->o_full[ob], (uint32_t)((j / OB) & 1), sh))) {
+                rgive_up(sh, 106);
+                return false;
+            }
+            tc_fence_after();
+            const float mj = sh->m_ref[j & 3][tid];
+            if (__any_sync(0xffffffffu, mj > m_o)) {
+                const float f = mj > m_o ? ex2(m_o - mj) : 1.f;
+                m_o = fmaxf(m_o, mj);
+#pragma unroll
+                for (int c = 0; c < TD / 4; ++c) o[c] = mul2(o[c], make_float2(f, f));
+            }
+            // (no key of the tile or before it is seen: P is zero)
+            const float w = mj == -INFINITY ? 0.f : ex2(mj - m_o) / sh->mv[j & 3];
+            const uint32_t from = tmem + lane_base + C::cO + ob * TD + set * (TD / 2);
+#pragma unroll
+            for (int c = 0; c < TD / 2; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(from + c, r);
+                tmem_wait_ld();
+                if (c + 32 >= TD / 2) {
+                    tc_fence_before();
+                    mbar_arrive_warp_relaxed(&sh->o_free[ob]);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) o[(c + i) >> 1] = fma2(floats2(r[i], r[i + 1]), make_float2(w, w), o[(c + i) >> 1]);
+            }
+            const uint32_t odd[2] = {sh->odd[j & 7][0], sh->odd[j & 7][1]};
+            if (odd[0] | odd[1]) {  // values that are not finite, added to the rows that see them
+                for (int i = 0; i < BN; ++i) {
+                    const int key = key0(j) + i;
+                    if (!(odd[i >> 5] >> (i & 31) & 1u) || !p.seen(key, pos)) continue;
+                    const long long at = PAGED ? p.pg.row(t.b, key) : ((long long)t.b * p.T + key) * ((long long)p.n_kv_heads * p.dim);
+                    if (at < 0) continue;
+#pragma unroll
+                    for (int c = 0; c < TD / 4; ++c) {
+                        const int col = set * (TD / 2) + 2 * c;
+                        if (col >= p.dim) continue;
+                        const float2 x = *reinterpret_cast<const float2 *>(p.v + at + (long long)g * p.dim + col);
+                        if (!finite(x.x)) o[c].x += x.x;
+                        if (!finite(x.y)) o[c].y += x.y;
+                    }
+                }
+                __syncwarp();
+            }
+            return true;
+        };
+        int added = 0;
+        // positions of this warp's rows: which tiles need a mask
+        const int warp_first = __shfl_sync(0xffffffffu, pos, 0), warp_last = __shfl_sync(0xffffffffu, pos, 31);
+        for (int j = set; ok && j < n; j += 2) {
+            if (!__all_sync(0xffffffffu, rwait(&sh->s_full[set], (uint32_t)((j >> 1) & 1), sh))) {
+                rgive_up(sh, 105);
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const int s0 = key0(j);
+            const float cs = fmaxf(cs0 / sh->mk[j & 3], 1.17549435e-38f);
+            const uint32_t cS = tmem + lane_base + C::cS + set * BN;
+            uint32_t r[BN];
+            tmem_ld32(cS, reinterpret_cast<uint32_t(&)[32]>(r[0]));
+            if (BN > 32) tmem_ld32(cS + 32, reinterpret_cast<uint32_t(&)[32]>(r[BN - 32]));
+            tmem_wait_ld();
+            const Seen &v = p.seen;
+            if (s0 + BN - 1 > warp_first || (v.window > 0 && s0 <= warp_last - v.window && s0 + BN > v.sinks)) {
+#pragma unroll
+                for (int i = 0; i < BN; ++i)
+                    if (!v(s0 + i, pos)) r[i] = 0xff800000u;
+            }
+            float mt = row_max32(reinterpret_cast<uint32_t(&)[32]>(r[0]), -INFINITY);
+            if (BN > 32) mt = row_max32(reinterpret_cast<uint32_t(&)[32]>(r[BN - 32]), mt);
+            mt *= cs;  // cs > 0
+            if ((mt > m_ref + tcf16::kRescaleThreshold || m_ref == -INFINITY) && mt != -INFINITY) {
+                l *= m_ref == -INFINITY ? 0.f : ex2(m_ref - mt);
+                m_ref = mt;
+            }
+            sh->m_ref[j & 3][tid] = m_ref;
+            const float off = ((m_ref == -INFINITY) ? 0.f : m_ref) - 7.0f;  // log2 kPScale: l and O are in P's units
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) {
+                uint32_t ph[16], pl[16];
+                l += row_exp32(reinterpret_cast<uint32_t(&)[32]>(r[c]), cs, off, ph, pl);
+                tmem_st16(cS + c, ph);
+                tmem_st16(cS + c + 16, pl);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive_warp(&sh->p_full[set]);
+            for (; ok && added <= j; ++added) ok = add_tile(added);
+        }
+        for (; ok && added < n; ++added) ok = add_tile(added);
+        // ---- the two sets' sums of exponentials; every thread then has its half of the row
+        sh->fin_m[set][tid] = m_ref, sh->fin_l[set][tid] = l;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (ok) {
+            const float m0 = sh->fin_m[0][tid], m1 = sh->fin_m[1][tid], mm = fmaxf(m0, m1);
+            // (a part may hold no key that the row sees)
+            const float w0 = m0 == -INFINITY ? 0.f : ex2(m0 - mm), w1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
+            const float sum = w0 * sh->fin_l[0][tid] + w1 * sh->fin_l[1][tid];
+            const float f = m_o == -INFINITY ? sum : ex2(m_o - mm) / sum;  // (sum: zero, or NaN)
+            constexpr int RS = TD * 4 + 16;
+            const int c0 = set * (TD / 2), cols = p.dim - c0 < TD / 2 ? p.dim - c0 : TD / 2;
+            uint8_t *srow = smem + tid * RS + c0 * 4;
+#pragma unroll
+            for (int c = 0; c < TD / 4; c += 2)
+                *reinterpret_cast<float4 *>(srow + c * 8) = make_float4(o[c].x * f, o[c].y * f, o[c + 1].x * f, o[c + 1].y * f);
+            tcf16::send_row<false>(p.out + part * p.out_part + rh * p.dim + c0, srow, cols, mine);
+            if (set == 0 && p.lse && mine) p.lse[part * p.lse_part + rh] = (mm + log2f(sum) - 7.0f) * kLn2;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// out, lse <- the parts'.  A warp per (row, head); a row that belongs to no sequence is left as it is.
+__global__ void __launch_bounds__(256) rows_join_kernel(const Params p, float *out, float *lse) {
+    pdl_wait();
+    pdl_launch();
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= p.lse_part) return;
+    const int lane = threadIdx.x & 31, token = (int)(row / p.n_heads), n4 = p.dim >> 2;
+    bool owned = false;
+    for (int b = lane; b < p.batch; b += 32) owned |= p.cu_rows[b] <= token && token < p.cu_rows[b + 1];
+    if (!__any_sync(0xffffffffu, owned)) return;
+    const float mine = lane < p.parts ? p.lse[lane * p.lse_part + row] : -INFINITY;
+    float top = mine;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    float w = (mine == -INFINITY) ? 0.f : ex2((mine - top) * kLog2e), sum = w;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    w /= sum;
+    for (int c = lane; c - lane < n4; c += 32) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < p.parts; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            if (wi == 0.f || c >= n4) continue;
+            const float4 x = *(reinterpret_cast<const float4 *>(p.out + i * p.out_part + row * p.dim) + c);
+            a.x = fmaf(wi, x.x, a.x), a.y = fmaf(wi, x.y, a.y), a.z = fmaf(wi, x.z, a.z), a.w = fmaf(wi, x.w, a.w);
+        }
+        if (c < n4) *(reinterpret_cast<float4 *>(out + row * p.dim) + c) = a;
+    }
+    if (lse && lane == 0) lse[row] = top + log2f(sum) * kLn2;
+}
+
+// The register shares are taken from what the kernel was compiled to be launched with: less than their sum, and a group that asks
+// for its share would wait for good.
+template <int TD, bool PAGED>
+inline bool registers_suffice() {
+    cudaFuncAttributes a{};
+    if (cudaFuncGetAttributes(&a, attn_rows_tc<TD, PAGED>) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return a.numRegs * kThreads >= 256 * Cfg<TD>::kRowRegs + 128 * (Cfg<TD>::kConvertRegs + Cfg<TD>::kIssueRegs);
+}
+template <int TD>
+inline int launch_td(const Params &p, long long slots, cudaStream_t stream) {
+    static const bool suffice = registers_suffice<TD, true>() && registers_suffice<TD, false>();
+    if (!suffice) return refuse("attn_rows_tc was not compiled for the registers that its warps share out.");
+    const size_t smem = (size_t)Cfg<TD>::kData + sizeof(Shared);
+    const auto kernel = p.pg.table ? attn_rows_tc<TD, true> : attn_rows_tc<TD, false>;
+    if (optin_smem((const void *)kernel, smem)) return 1;
+    const dim3 grid((unsigned)slots, (unsigned)p.n_kv_heads, (unsigned)p.parts);
+    return launch_after("attn_rows_tc", kernel, grid, dim3(kThreads), smem, stream, 1, p);
+}
+inline int launch(const Params &p, long long slots, cudaStream_t stream) {
+    g_last_path = "tcgen05";
+    switch (tc_tile_dim(p.dim)) {
+        case 64: return launch_td<64>(p, slots, stream);
+        case 128: return launch_td<128>(p, slots, stream);
+        case 192: return launch_td<192>(p, slots, stream);
+        default: return launch_td<256>(p, slots, stream);
+    }
+}
+
+inline int launch_join(const Params &p, float *out, float *lse, cudaStream_t stream) {
+    return launch_pdl("rows_join_kernel", rows_join_kernel, dim3((unsigned)((p.lse_part + 7) / 8)), dim3(256), 0, stream, p, out, lse);
+}
+
+// Row tiles, at most, of `rows` new rows of `batch` sequences.
+inline long long row_slots(int batch, int rows, int group) { return (long long)rows * group / 128 + batch; }
+// How many parts the keys of a row tile are split into, where a CTA an SM is more than there are row tiles: a part keeps
+// 256 keys of the longest sequence at least.
+inline int row_parts(int batch, int rows, int max_seen, int n_heads, int n_kv_heads) {
+    const int group = n_heads / n_kv_heads;
+    // (sequences share the rows: a tile each, and one more for every 128 rows)
+    const long long full = (long long)rows * group, tiles = full / 128 + (full < batch ? full : batch);
+    long long n = split_sm_count() / (tiles * n_kv_heads < 1 ? 1 : tiles * n_kv_heads);
+    if (n > max_seen / 256) n = max_seen / 256;
+    return n < 2 ? 1 : (n > 32 ? 32 : (int)n);
+}
+// The most floats of the parts' rows, of a call of at most so many rows: what row_parts splits is at most a CTA's 128 rows an SM.
+inline size_t row_parts_bound(int rows, int n_heads, int dim) {
+    const size_t by_rows = (size_t)32 * rows * n_heads, by_blocks = (size_t)split_sm_count() * 128;
+    return (by_rows < by_blocks ? by_rows : by_blocks) * ((size_t)dim + 1);
+}
+
+}  // namespace tcr
+}  // namespace zt

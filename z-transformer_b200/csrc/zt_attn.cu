@@ -22,6 +22,7 @@
 #include "tc_fwd16n.cuh"
 #include "tc_fwd16x.cuh"
 #include "tc_fwd_short.cuh"
+#include "tc_rows.cuh"
 #include "tc_gemm.cuh"
 #include "tc_bwd_wide.cuh"
 #include "tc_bwd_fused.cuh"
@@ -1170,7 +1171,15 @@ int zt_attn_forward_window_batched(const float *q, const float *k, const float *
     if (!q || !k || !v || !out) return refuse("a null device pointer was passed.");
     if (need_device()) return 1;
     normal_window(T, &window, &sinks);
-    if (window == 0) return forward_impl(q, k, v, out, lse, batch, T, n_heads, n_kv_heads, dim, 0, T, (cudaStream_t)stream);
+    const DeviceInfo *d = device_info();
+    if (g_path.load() != 1 && tc_takes_dim(dim) && d->cc_major == 10 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out)) {
+        tcr::Params p{};
+        p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
+        p.batch = batch, p.T = T, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.dim = dim, p.parts = 1;
+        p.seen = Seen{window, sinks};
+        p.scale_log2 = kLog2e / sqrtf((float)dim);
+        return tcr::launch(p, (long long)batch * (((long long)T * (n_heads / n_kv_heads) + 127) / 128), (cudaStream_t)stream);
+    }
     SimtFwdParams p{};
     p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
     p.T = T, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.dim = dim, p.n_keys = T;
@@ -1223,7 +1232,7 @@ int zt_kv_append_paged(float *k_pages, float *v_pages, const int *table, int *n_
 size_t zt_attn_paged_workspace_bytes(int batch, int rows, int max_keys, int n_heads, int n_kv_heads, int dim) {
     if (batch < 1 || rows < 0 || max_keys < 1 || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || !zt_attn_dim_ok(dim) || dim % 4 != 0)
         return 0;
-    return decode_bytes_bound(batch, max_keys, n_heads, n_kv_heads, dim);
+    return most(decode_bytes_bound(batch, max_keys, n_heads, n_kv_heads, dim), kDecodeHeaderBytes + tcr::row_parts_bound(rows, n_heads, dim) * sizeof(float));
 }
 
 int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, const int *n_keys,
@@ -1241,28 +1250,37 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     for (const void *t : {(const void *)q, (const void *)k_pages, (const void *)v_pages, (const void *)out})
         if (!aligned16(t)) return refuse("q, out and the pages must be 16-byte aligned.");
     if (need_device()) return 1;
+    const DeviceInfo *d = device_info();
+    if (d->cc_major != 10 || !tc_takes_dim(dim)) return refuse("paged attention needs an sm_100 device.");
     if (rows == 0) return 0;
     const int capacity = max_pages * page_size;
-    if (window == 0 || window >= capacity) window = sinks = 0;
+    if (window == 0 || window >= capacity || sinks >= capacity) window = sinks = 0;
     if (!cu_rows) {
         // one row a sequence: split over the keys that it sees
         const int seen = window > 0 && sinks < capacity - window ? window + sinks : capacity;
-        DecodeParams d{};
-        d.q = q, d.k_cache = k_pages, d.v_cache = v_pages, d.n_keys = n_keys, d.out = out, d.lse = lse;
-        d.batch = batch, d.n_ctx = capacity, d.n_heads = n_heads, d.n_kv_heads = n_kv_heads, d.dim = dim;
-        d.scale_log2 = kLog2e / sqrtf((float)dim);
-        d.pg = make_pages(k_pages, v_pages, table, n_pages, page_size, max_pages, n_kv_heads * dim);
-        d.window = window, d.sinks = sinks;
-        return launch_decode(d, decode_plan(batch, seen, n_heads, n_kv_heads, dim), workspace, (cudaStream_t)stream);
+        DecodeParams s{};
+        s.q = q, s.k_cache = k_pages, s.v_cache = v_pages, s.n_keys = n_keys, s.out = out, s.lse = lse;
+        s.batch = batch, s.n_ctx = capacity, s.n_heads = n_heads, s.n_kv_heads = n_kv_heads, s.dim = dim;
+        s.scale_log2 = kLog2e / sqrtf((float)dim);
+        s.pg = make_pages(k_pages, v_pages, table, n_pages, page_size, max_pages, n_kv_heads * dim);
+        s.window = window, s.sinks = sinks;
+        return launch_decode(s, decode_plan(batch, seen, n_heads, n_kv_heads, dim), workspace, (cudaStream_t)stream);
     }
-    PagedParams p{};
+    tcr::Params p{};
+    p.q = q, p.k = k_pages, p.v = v_pages, p.out = out, p.lse = lse;
     p.pg = make_pages(k_pages, v_pages, table, n_pages, page_size, max_pages, n_kv_heads * dim);
-    p.q = q, p.n_keys = n_keys, p.cu_rows = cu_rows, p.out = out, p.lse = lse;
-    p.bad_count = static_cast<int *>(workspace);
+    p.n_keys = n_keys, p.cu_rows = cu_rows, p.bad_count = static_cast<int *>(workspace);
     p.batch = batch, p.rows = rows, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.dim = dim;
     p.seen = Seen{window, sinks};
     p.scale_log2 = kLog2e / sqrtf((float)dim);
-    return launch_paged_rows(p, (cudaStream_t)stream);
+    const long long keys = window > 0 ? (long long)window + sinks + rows : capacity;
+    p.parts = tcr::row_parts(batch, rows, (int)(keys < capacity ? keys : capacity), n_heads, n_kv_heads);
+    const long long slots = tcr::row_slots(batch, rows, n_heads / n_kv_heads);
+    if (p.parts == 1) return tcr::launch(p, slots, (cudaStream_t)stream);
+    p.lse_part = (long long)rows * n_heads, p.out_part = p.lse_part * dim;
+    p.out = reinterpret_cast<float *>(static_cast<char *>(workspace) + kDecodeHeaderBytes), p.lse = p.out + p.parts * p.out_part;
+    if (tcr::launch(p, slots, (cudaStream_t)stream)) return 1;
+    return tcr::launch_join(p, out, lse, (cudaStream_t)stream);
 }
 
 }  // extern "C"
