@@ -7,9 +7,11 @@
 // different:
 //   rows    A tile's 128 rows are (token, head of the KV group) pairs, token by token: sixteen tokens of eight heads see the
 //           same keys, so a short chunk fills a tile, and a window of W keys costs a tile W + 128 / group keys and not W + 128.
-//   keys    come as they are.  Four warps copy a tile's rows into shared memory (cp.async, row by row: each has its page),
-//           find the tile's largest magnitude and write the pieces, scaled by a power of two of the tile's own, as the
-//           operand tiles that the MMAs read.  No launch before this one converts anything and nothing is kept in memory.
+//   keys    come as they are.  Converting warps copy a tile's rows into shared memory (cp.async, row by row: each has its
+//           page) and write the pieces, scaled by a power of two of the tile's own, as the operand tiles that the MMAs
+//           read.  No launch before this one converts anything and nothing is kept in memory.  The power of two is the one that
+//           the tile before would have had, so that a row is converted as soon as it is there; where it turns out to be off by
+//           more than the pieces can bear, or something is not finite, the tile is converted again with care.
 //   scales  K's goes into the tile's scores; V's, and the reference maximum of the tile's exponentials, into the factor with
 //           which the row threads add the tile's P V to the row: O leaves TMEM after every tile and is summed in registers,
 //           with rounding (the tensor core adds with truncation, 2.3e-7 of O for every 64 keys: over a long prefix that is the
@@ -17,9 +19,10 @@
 //   masks   Which key tiles a CTA visits follows from its first and last position: the sinks' and the window's.  A key that
 //           no row of the tile sees is not read and counts as zero.  A value that is not finite does not enter the product,
 //           where a weight of zero would not keep it from a row that does not see it: the row threads add it to those that do.
-// Roles, 16 warps: two sets of four row warps -- set j & 1 makes P of tile j, each set sums one half of the columns of every
-// tile --, four converting warps, a warp that issues S and one that issues P V (a thread issues an MMA of N <= 64 every 50
-// clocks, the pipe takes one every 32), two idle ones that make the four a group for setmaxnreg.
+// Roles: two sets of four row warps -- set j & 1 makes P of tile j, each set sums one half of the columns of every tile --,
+// four warps that convert K and four that convert V (above 128 columns the same four), a warp that issues S and one that
+// issues P V (a thread issues an MMA of N <= 64 every 50 clocks, the pipe takes one every 32), two idle ones that make the
+// four a group for setmaxnreg.
 // TMEM: up to 128 columns Q hi, Q lo, two O and two S/P buffers; above, Q hi, one O and two S/P buffers of 32 keys, Q lo in
 // shared memory.
 #pragma once
@@ -42,7 +45,7 @@ using tcf16::row_max32;
 using tcf16::split_q32;
 using tcf16::store_q_piece;
 
-constexpr int kThreads = 512, kConvert = 128;  // threads of a CTA; of them those that convert
+constexpr int kConvert = 128;  // threads that convert a tile
 
 template <int TD>
 struct Cfg {
@@ -50,17 +53,22 @@ struct Cfg {
     static constexpr int BN = kWide ? 32 : 64;      // keys of a tile
     static constexpr int OB = kWide ? 1 : 2;        // O buffers
     static constexpr int KS = TD == 256 ? 1 : 2, VS = KS;  // slots of converted K and V tiles
-    static constexpr int SU = 2;                    // slots of tiles as they come
     static constexpr int KP = BN * TD * 2;          // bytes of one piece of a tile
-    static constexpr int RAW = BN * TD * 4;
     static constexpr int QL = kWide ? 128 * TD * 2 : 0;
-    static constexpr int CHUNKS = BN * TD / 4 / kConvert;  // 16-byte chunks a converting thread has of a tile
-    // registers a thread: the launch gives 512 threads 128 each
-    static constexpr int kRowRegs = kWide ? 200 : 184, kConvertRegs = kWide ? 72 : 104, kIssueRegs = 40;
-    static_assert(256 * kRowRegs + 128 * (kConvertRegs + kIssueRegs) <= kThreads * 128, "the groups share what the launch has");
+    // What is copied, waited for and converted at a time is 16 keys of a tile: `part`.  A thread has CHUNKS 16-byte chunks of it,
+    // and a group of converting warps NP parts under way.
+    static constexpr int PARTS = BN / 16, PART = 16 * TD * 4, CHUNKS = PART / 16 / kConvert;
+    static constexpr int GROUPS = kWide ? 1 : 2;
+    static constexpr int NP = TD == 64 ? 8 : (TD == 128 ? 5 : 4);
+    static constexpr int kThreads = 256 + GROUPS * kConvert + 128;
+    // registers a thread: the launch gives 640 threads 96 each, 512 threads 128
+    static constexpr int kLaunchRegs = kWide ? 128 : 96, kRowRegs = kWide ? 200 : 160, kConvertRegs = kWide ? 72 : 64, kIssueRegs = kWide ? 40 : 32;
+    static constexpr int kShare = 256 * kRowRegs + GROUPS * kConvert * kConvertRegs + 128 * kIssueRegs;
+    static_assert(kShare <= kThreads * kLaunchRegs, "the groups share what the launch has");
     static constexpr int cQh = 0, cQl = TD / 2, cO = kWide ? 128 : TD, cS = kWide ? 384 : 3 * TD;
-    static constexpr int kData = KS * 2 * KP + VS * 2 * KP + SU * RAW + QL;
+    static constexpr int kData = KS * 2 * KP + VS * 2 * KP + GROUPS * NP * PART + QL;
     static_assert(128 * (TD * 4 + 16) <= kData, "the finished rows are staged where the tiles were");
+    static_assert(NP <= 2 * PARTS, "rows are looked up two tiles ahead");
 };
 
 struct Shared {
@@ -69,11 +77,15 @@ struct Shared {
     volatile int abort;
     int found;
     float mk[4], mv[4];         // the scales of tiles j & 3
-    uint32_t odd[8][2];         // which values' rows of tile j & 7 hold something that is not finite
-    uint32_t top[2][4];         // per converting warp: max |x| of the unit
+    uint32_t odd[16][2];        // which values' rows of tile j & 15 hold something that is not finite
+    uint32_t top[2][2][4];      // [group][unit & 1][warp]: the largest hi piece; or max |x|
+    uint32_t seed[2][4];
     float m_ref[4][128];        // the rows' reference maxima of tile j & 3
     float fin_m[2][128], fin_l[2][128], q_top[2][128];
-    long long row[4][64];       // of tile j & 3: elements to every key's row; kNone: counts as zero; kNoPage: NaN
+    // elements to the rows of the next tiles' keys (kNone: counts as zero, kNoPage: NaN): of a group's tile j & 3 or, in tiles
+    // of 32 keys, of j & 7; and whether some key of the tile is on no page, by halves
+    long long row[512];
+    int holes[8][2];
 };
 constexpr long long kNone = -1, kNoPage = -2;
 
@@ -106,6 +118,16 @@ template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
+// -inf for those of 32 keys from key0 on that the query at `pos` does not see.
+__device__ __forceinline__ void mask_scores(uint32_t (&r)[32], const Seen &v, int key0, int pos) {
+    const auto below = [](int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); };  // the first n bits
+    uint32_t seen = below(pos - key0 + 1);
+    if (v.window > 0) seen &= ~below(pos - v.window - key0 + 1) | below(v.sinks - key0);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (!(seen >> i & 1u)) r[i] = 0xff800000u;
+}
+
 // The key tiles that the rows at positions [first, last] visit, numbered through: those with sinks, then the window's.
 struct Tiles {
     int n, sink_tiles, skip;
@@ -127,11 +149,11 @@ struct RowTile {
 };
 
 template <int TD, bool PAGED>
-__global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
+__global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Params p) {
     using C = Cfg<TD>;
-    constexpr int BN = C::BN, KP = C::KP, KS = C::KS, VS = C::VS, OB = C::OB, SU = C::SU;
+    constexpr int BN = C::BN, KP = C::KP, KS = C::KS, VS = C::VS, OB = C::OB, kThreads = C::kThreads, kIssuer = kThreads / 32 - 4;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t *sK = smem, *sV = sK + KS * 2 * KP, *sRaw = sV + VS * 2 * KP, *sQl = sRaw + SU * C::RAW;
+    uint8_t *sK = smem, *sV = sK + KS * 2 * KP, *sRaw = sV + VS * 2 * KP, *sQl = sRaw + C::GROUPS * C::NP * C::PART;
     Shared *sh = reinterpret_cast<Shared *>(sQl + C::QL);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = p.n_heads / p.n_kv_heads;
@@ -141,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
     pdl_wait();
     RowTile t{};
     if (PAGED) {
-        if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && warp == 15) {
+        if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && warp == kIssuer + 3) {
             int bad = 0;
             for (int i = lane; i < p.batch; i += 32) bad += new_rows(p.cu_rows, p.n_keys, i, p.rows, p.pg, true).bad;
             bad = __reduce_add_sync(0xffffffffu, bad);
@@ -197,8 +219,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh->k_full[i], kConvert / 32), mbar_init(&sh->k_free[i], 1);
-            mbar_init(&sh->v_full[i], kConvert / 32), mbar_init(&sh->v_free[i], 1);
+            mbar_init(&sh->k_full[i], 1), mbar_init(&sh->k_free[i], 1);
+            mbar_init(&sh->v_full[i], 1), mbar_init(&sh->v_free[i], 1);
             mbar_init(&sh->s_full[i], 1), mbar_init(&sh->p_full[i], 4), mbar_init(&sh->pv_done[i], 1);
             mbar_init(&sh->o_full[i], 1), mbar_init(&sh->o_free[i], 8);
         }
@@ -207,16 +229,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
         if (sh->abort) atomicMax(&g_tc_status, 100);
         mbar_fence_init();
     }
-    if (warp == 12) tmem_alloc(&sh->tmem_base, 512);
+    if (warp == kIssuer) tmem_alloc(&sh->tmem_base, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh->tmem_base;
     const int steps = head_steps(p.dim);
 
-    if (warp >= 12) {
+    if (warp >= kIssuer) {
         fewer_registers<C::kIssueRegs>();
-        if (warp == 12) {
+        if (warp == kIssuer) {
             // -------------------------------------------------------------- S(j) = Q K^T into buffer j & 1
             if (elect_one()) {
                 constexpr uint32_t id_s = idesc_f16(128, BN, false, false);
@@ -247,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
                 }
             }
             __syncwarp();
-        } else if (warp == 13) {
+        } else if (warp == kIssuer + 1) {
             // -------------------------------------------------------------- O(j) = P(j) V
             if (elect_one()) {
                 const uint32_t id_o = idesc_f16(128, 16 * steps, false, true);
@@ -276,19 +298,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
             __syncwarp();
         }
     } else if (warp >= 8) {
-        // ------------------------------------------------------------------ keys and values: copied, scaled, split.  The units
-        // go in the order in which the MMAs ask for them: K0, K1, V0, K2, V1, ...
+        // ------------------------------------------------------------------ keys and values: copied, scaled, split.  A group's
+        // units are tiles of K, or of V, or of both in the order in which the MMAs ask for them: K0, K1, V0, K2, V1, ...
         fewer_registers<C::kConvertRegs>();
-        const int ct = threadIdx.x - 256, cw = warp - 8;
-        constexpr int CPR = TD / 4;  // chunks of a row
-        const int n_units = 2 * n;
+        const int ct = threadIdx.x & (kConvert - 1), cw = warp & 3, gi = (warp - 8) >> 2;
+        constexpr int CPR = TD / 4, CH = C::CHUNKS, NP = C::NP, PARTS = C::PARTS;  // (CPR: chunks of a row)
+        constexpr float kAim = 0.25f;  // of block_mult's: the largest magnitude in [2^12, 2^13), with room for eight times as much
+        const bool both = C::GROUPS == 1;
+        const int n_units = both ? 2 * n : n;
         const long long width = PAGED ? p.pg.width : (long long)p.n_kv_heads * p.dim;
-        const auto tile_of = [&](int u, bool &is_k) {
-            is_k = u == 0 || ((u & 1) && u != n_units - 1);
-            return u == 0 ? 0 : (is_k ? (u + 1) >> 1 : (u == n_units - 1 ? n - 1 : (u >> 1) - 1));
+        uint8_t *ring = sRaw + gi * (NP * C::PART);
+        const auto unit = [&](int u, bool &is_k) {
+            is_k = both ? u == 0 || ((u & 1) && u != n_units - 1) : gi == 0;
+            return !both ? u : u == 0 ? 0 : (is_k ? (u + 1) >> 1 : (u == n_units - 1 ? n - 1 : (u >> 1) - 1));
         };
+        const auto sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(2 + gi) : "memory"); };
         // where the keys of tile j lie; one that no row of this CTA sees counts as zero
+        const auto place = [&](int j) { return both ? j & 7 : gi * 4 + (j & 3); };
+        const auto rows_of = [&](int j) { return sh->row + place(j) * BN; };
         const auto look_up = [&](int j) {
+            if (ct < 2 && (both || gi == 1)) sh->odd[j & 15][ct] = 0;
             if (ct >= BN || j >= n) return;
             const int key = key0(j) + ct;
             long long at = kNone;
@@ -296,88 +325,144 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
                 at = PAGED ? p.pg.row(t.b, key) : ((long long)t.b * p.T + key) * width;
                 if (at < 0) at = kNoPage;
             }
-            sh->row[j & 3][ct] = at;
+            rows_of(j)[ct] = at;
+            const bool hole = PAGED && __any_sync(0xffffffffu, at == kNoPage);
+            if (lane == 0) sh->holes[place(j)][cw] = hole;
         };
-        const auto copy_unit = [&](int u) {
+        const auto copy_part = [&](int P) {
+            const int u = P / PARTS, q = P % PARTS;
             if (u < n_units) {
                 bool is_k;
-                const int j = tile_of(u, is_k);
+                const int j = unit(u, is_k);
                 const float *base = is_k ? p.k : p.v;
-                const uint32_t dst = smem_u32(sRaw + (u % SU) * C::RAW) + (uint32_t)ct * 16;
+                const uint32_t dst = smem_u32(ring + (P % NP) * C::PART) + (uint32_t)ct * 16;
+                const long long *rows = rows_of(j) + q * 16;
+                long long at[CH];
 #pragma unroll
-                for (int i = 0; i < C::CHUNKS; ++i) {
-                    const int f = i * kConvert + ct, r = f / CPR, c = f - r * CPR;
-                    const long long at = sh->row[j & 3][r];
-                    const bool in = at >= 0 && c * 4 < p.dim;
-                    copy16_async(dst + i * (kConvert * 16), in ? base + at + (long long)g * p.dim + c * 4 : base, in);
+                for (int i = 0; i < CH; ++i) at[i] = rows[(i * kConvert + ct) / CPR];
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    const int c = (i * kConvert + ct) % CPR;
+                    const bool in = at[i] >= 0 && c * 4 < p.dim;
+                    copy16_async(dst + i * (kConvert * 16), in ? base + at[i] + (long long)g * p.dim + c * 4 : base, in);
                 }
             }
             copy_async_commit();
         };
-        look_up(0), look_up(1);
-        asm volatile("bar.sync 2, 128;" ::: "memory");
-        for (int u = 0; u < SU; ++u) copy_unit(u);
-        bool ok = true;
-        for (int u = 0; u < n_units; ++u) {
-            bool is_k;
-            const int j = tile_of(u, is_k);
-            copy_async_wait<SU - 1>();
-            const float4 *raw = reinterpret_cast<const float4 *>(sRaw + (u % SU) * C::RAW) + ct;
-            if (ct < 2 && is_k) sh->odd[j & 7][ct] = 0;  // (of V, whose unit comes later)
-            uint32_t top = 0, seen_bits = 0;
-#pragma unroll
-            for (int i = 0; i < C::CHUNKS; ++i) {
-                const float4 x = raw[i * kConvert];
-                top = max(max(top, __float_as_uint(x.x) & 0x7fffffffu), __float_as_uint(x.y) & 0x7fffffffu);
-                top = max(max(top, __float_as_uint(x.z) & 0x7fffffffu), __float_as_uint(x.w) & 0x7fffffffu);
-            }
-            seen_bits = top;
-            if (seen_bits >= 0x7f800000u) {  // something is not finite: the largest of what is; rows of V are noted
-                top = 0;
+        // a chunk's pieces into the operand tile: 64-column block, row, 16-byte chunk of eight halves with the 128-byte swizzle, its
+        // first or second half
+        const auto store_pieces = [&](uint8_t *dst, int f, uint2 h, uint2 l) {
+            const int r = f / CPR, c = f % CPR;
+            uint8_t *at = dst + (c >> 4) * (BN * 128) + r * 128 + ((((c & 15) >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
+            *reinterpret_cast<uint2 *>(at) = h;
+            *reinterpret_cast<uint2 *>(at + KP) = l;
+        };
+        // A tile once more, from memory: the scale is its own, keys on no page are NaN, values that are not finite are noted and
+        // left to the row threads.  Returns the scale.
+        const auto with_care = [&](uint8_t *dst, bool is_k, int j, int u) -> float {
+            const auto chunk = [&](int f) {
+                const long long at = rows_of(j)[f / CPR];
+                const int col = f % CPR * 4;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (at >= 0 && col < p.dim) x = *reinterpret_cast<const float4 *>((is_k ? p.k : p.v) + at + (long long)g * p.dim + col);
+                if (is_k && at == kNoPage) x.x = __int_as_float(0x7fc00000);
+                return x;
+            };
+            uint32_t top = 0;
 #pragma unroll 1
-                for (int i = 0; i < C::CHUNKS; ++i) {
-                    const float4 x = raw[i * kConvert];
-                    const int r = (i * kConvert + ct) / CPR;
-                    for (const float e : {x.x, x.y, x.z, x.w}) {
-                        if (finite(e)) top = max(top, __float_as_uint(e) & 0x7fffffffu);
-                        else if (!is_k) atomicOr(&sh->odd[j & 7][r >> 5], 1u << (r & 31));
-                    }
+            for (int f = ct; f < BN * CPR; f += kConvert) {
+                const float4 x = chunk(f);
+                const int r = f / CPR;
+                for (const float e : {x.x, x.y, x.z, x.w}) {
+                    if (finite(e)) top = max(top, __float_as_uint(e) & 0x7fffffffu);
+                    else if (!is_k) atomicOr(&sh->odd[j & 15][r >> 5], 1u << (r & 31));
                 }
             }
             top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) sh->top[u & 1][cw] = top;
-            if (u & 1) look_up(((u + 1) >> 1) + (SU + 1) / 2);
-            asm volatile("bar.sync 2, 128;" ::: "memory");
-            const float m = block_mult(max(max(sh->top[u & 1][0], sh->top[u & 1][1]), max(sh->top[u & 1][2], sh->top[u & 1][3])));
-            const int s = is_k ? j % KS : j % VS, S = is_k ? KS : VS;
-            if (ok && j >= S && !__all_sync(0xffffffffu, rwait(is_k ? &sh->k_free[s] : &sh->v_free[s], (uint32_t)((j / S - 1) & 1), sh))) {
-                rgive_up(sh, 104);
-                ok = false;
-            }
-            if (!ok) continue;  // (on to the barriers that the other warps wait at)
-            uint8_t *dst = (is_k ? sK : sV) + s * 2 * KP;
-            if (ct == 0) (is_k ? sh->mk : sh->mv)[j & 3] = m;
-#pragma unroll
-            for (int i = 0; i < C::CHUNKS; ++i) {
-                const int f = i * kConvert + ct, r = f / CPR, c = f - r * CPR;
-                float4 x = raw[i * kConvert];
-                if (is_k) {
-                    if (sh->row[j & 3][r] == kNoPage) x.x = __int_as_float(0x7fc00000);
-                } else if (seen_bits >= 0x7f800000u) {
-                    x.x = finite(x.x) ? x.x : 0.f, x.y = finite(x.y) ? x.y : 0.f, x.z = finite(x.z) ? x.z : 0.f, x.w = finite(x.w) ? x.w : 0.f;
-                }
-                const float2 mm = make_float2(m, m);
+            sync();  // (everyone has read what `top` held)
+            if (lane == 0) sh->top[gi][u & 1][cw] = top;
+            sync();
+            const uint32_t *tops = sh->top[gi][u & 1];
+            const float m = block_mult(max(max(tops[0], tops[1]), max(tops[2], tops[3]))) * kAim;
+#pragma unroll 1
+            for (int f = ct; f < BN * CPR; f += kConvert) {
+                float4 x = chunk(f);
+                if (!is_k) x.x = finite(x.x) ? x.x : 0.f, x.y = finite(x.y) ? x.y : 0.f, x.z = finite(x.z) ? x.z : 0.f, x.w = finite(x.w) ? x.w : 0.f;
                 uint2 h, l;
-                split_pack(mul2(make_float2(x.x, x.y), mm), h.x, l.x);
-                split_pack(mul2(make_float2(x.z, x.w), mm), h.y, l.y);
-                // 64-column block, row, 16-byte chunk of eight halves with the 128-byte swizzle, its first or second half
-                uint8_t *at = dst + (c >> 4) * (BN * 128) + r * 128 + ((((c & 15) >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
-                *reinterpret_cast<uint2 *>(at) = h;
-                *reinterpret_cast<uint2 *>(at + KP) = l;
+                split_pack(x.x * m, x.y * m, h.x, l.x);
+                split_pack(x.z * m, x.w * m, h.y, l.y);
+                store_pieces(dst, f, h, l);
             }
             fence_async_smem();
-            mbar_arrive_warp(is_k ? &sh->k_full[s] : &sh->v_full[s]);
-            copy_unit(u + SU);  // (into the slot that this thread has just read its own chunks out of)
+            sync();
+            return m;
+        };
+        if (ct < 8) sh->holes[ct][1] = 0;  // (tiles of 32 keys have one half)
+        for (int j = 0; j < 4; ++j) look_up(j);
+        sync();
+#pragma unroll 1
+        for (int P = 0; P < NP; ++P) copy_part(P);
+        bool ok = true;
+        float m_k = 0.f, m_v = 0.f;  // the next tile's scales; 0: none yet
+#pragma unroll 1
+        for (int u = 0, P = 0; u < n_units; ++u) {
+            bool is_k;
+            const int j = unit(u, is_k), s = is_k ? j % KS : j % VS, S = is_k ? KS : VS;
+            uint8_t *dst = (is_k ? sK : sV) + s * 2 * KP;
+            if (ok && j >= S && !__all_sync(0xffffffffu, rwait(is_k ? &sh->k_free[s] : &sh->v_free[s], (uint32_t)((j / S - 1) & 1), sh))) {
+                rgive_up(sh, 104);
+                ok = false;  // (on to the barriers that the other warps wait at)
+            }
+            float m = is_k ? m_k : m_v;
+            uint32_t top = 0;
+#pragma unroll 1
+            for (int q = 0; q < PARTS; ++q, ++P) {
+                copy_async_wait<NP - 1>();
+                const float4 *raw = reinterpret_cast<const float4 *>(ring + (P % NP) * C::PART) + ct;
+                float4 x[CH];
+#pragma unroll
+                for (int i = 0; i < CH; ++i) x[i] = raw[i * kConvert];
+                if (m == 0.f) {  // the first tile: by its first keys
+                    float most = 0.f;
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) most = fmaxf(most, max_abs4(x[i]));
+                    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+                    if (lane == 0) sh->seed[gi][cw] = bits;
+                    sync();
+                    const uint32_t *tops = sh->seed[gi];
+                    m = block_mult(max(max(tops[0], tops[1]), max(tops[2], tops[3]))) * kAim;
+                }
+                if (!ok) continue;
+                const float2 mm = make_float2(m, m);
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    uint2 h, l;
+                    split_pack(mul2(make_float2(x[i].x, x[i].y), mm), h.x, l.x);
+                    split_pack(mul2(make_float2(x[i].z, x[i].w), mm), h.y, l.y);
+                    top = __vmaxu2(top, __vmaxu2(h.x & 0x7fff7fffu, h.y & 0x7fff7fffu));
+                    store_pieces(dst, q * 16 * CPR + i * kConvert + ct, h, l);
+                }
+                copy_part(P + NP);  // (into the place of the chunks that this thread has just converted)
+            }
+            fence_async_smem();
+            top = max(top & 0xffffu, top >> 16);
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) sh->top[gi][u & 1][cw] = top;
+            const int hole = sh->holes[place(j)][0] | sh->holes[place(j)][1];
+            sync();
+            const uint32_t *tops = sh->top[gi][u & 1];
+            top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+            // The largest hi piece below 2^-3 (its lo piece would lose bits), or none, or not finite: with care.
+            const bool care = top < 0x3000u || top >= 0x7c00u || (is_k && hole);
+            if (care) m = with_care(dst, is_k, j, u);
+            if (ct == 0) {
+                (is_k ? sh->mk : sh->mv)[j & 3] = m;
+                if (ok) mbar_arrive(is_k ? &sh->k_full[s] : &sh->v_full[s]);
+            }
+            // the next tile's: with which this one's largest would have been in [2^12, 2^13)
+            if (!care) m *= __uint_as_float((uint32_t)(127 + 27 - (int)(top >> 10)) << 23);
+            (is_k ? m_k : m_v) = fminf(fmaxf(m, 0x1p-120f), 0x1p120f);
+            if (!both || is_k) look_up(j + 4);
         }
         copy_async_wait<0>();
     } else {
@@ -451,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) o[(c + i) >> 1] = fma2(floats2(r[i], r[i + 1]), make_float2(w, w), o[(c + i) >> 1]);
             }
-            const uint32_t odd[2] = {sh->odd[j & 7][0], sh->odd[j & 7][1]};
+            const uint32_t odd[2] = {sh->odd[j & 15][0], sh->odd[j & 15][1]};
             if (odd[0] | odd[1]) {  // values that are not finite, added to the rows that see them
                 for (int i = 0; i < BN; ++i) {
                     const int key = key0(j) + i;
@@ -484,18 +569,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
             const int s0 = key0(j);
             const float cs = fmaxf(cs0 / sh->mk[j & 3], 1.17549435e-38f);
             const uint32_t cS = tmem + lane_base + C::cS + set * BN;
-            uint32_t r[BN];
-            tmem_ld32(cS, reinterpret_cast<uint32_t(&)[32]>(r[0]));
-            if (BN > 32) tmem_ld32(cS + 32, reinterpret_cast<uint32_t(&)[32]>(r[BN - 32]));
-            tmem_wait_ld();
             const Seen &v = p.seen;
-            if (s0 + BN - 1 > warp_first || (v.window > 0 && s0 <= warp_last - v.window && s0 + BN > v.sinks)) {
+            const bool masked = s0 + BN - 1 > warp_first || (v.window > 0 && s0 <= warp_last - v.window && s0 + BN > v.sinks);
+            // 32 columns of S at a time: they come out of TMEM a second time for their exponentials, so that a thread's registers
+            // hold its half of O beside them
+            uint32_t r[32];
+            const auto scores = [&](int c) {
+                tmem_ld32(cS + c, r);
+                tmem_wait_ld();
+                if (masked) mask_scores(r, v, s0 + c, pos);
+            };
+            float mt = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < BN; ++i)
-                    if (!v(s0 + i, pos)) r[i] = 0xff800000u;
+            for (int c = 0; c < BN; c += 32) {
+                scores(c);
+                mt = row_max32(r, mt);
             }
-            float mt = row_max32(reinterpret_cast<uint32_t(&)[32]>(r[0]), -INFINITY);
-            if (BN > 32) mt = row_max32(reinterpret_cast<uint32_t(&)[32]>(r[BN - 32]), mt);
             mt *= cs;  // cs > 0
             if ((mt > m_ref + tcf16::kRescaleThreshold || m_ref == -INFINITY) && mt != -INFINITY) {
                 l *= m_ref == -INFINITY ? 0.f : ex2(m_ref - mt);
@@ -506,7 +595,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
                 uint32_t ph[16], pl[16];
-                l += row_exp32(reinterpret_cast<uint32_t(&)[32]>(r[c]), cs, off, ph, pl);
+                if (BN > 32) scores(c);
+                l += row_exp32(r, cs, off, ph, pl);
                 tmem_st16(cS + c, ph);
                 tmem_st16(cS + c + 16, pl);
             }
@@ -537,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_rows_tc(const Params p) {
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == kIssuer) tmem_dealloc(tmem, 512);
 }
 
 // out, lse <- the parts'.  A warp per (row, head); a row that belongs to no sequence is left as it is.
@@ -580,7 +670,7 @@ inline bool registers_suffice() {
         cudaGetLastError();
         return false;
     }
-    return a.numRegs * kThreads >= 256 * Cfg<TD>::kRowRegs + 128 * (Cfg<TD>::kConvertRegs + Cfg<TD>::kIssueRegs);
+    return a.numRegs * Cfg<TD>::kThreads >= Cfg<TD>::kShare;
 }
 template <int TD>
 inline int launch_td(const Params &p, long long slots, cudaStream_t stream) {
@@ -590,7 +680,7 @@ inline int launch_td(const Params &p, long long slots, cudaStream_t stream) {
     const auto kernel = p.pg.table ? attn_rows_tc<TD, true> : attn_rows_tc<TD, false>;
     if (optin_smem((const void *)kernel, smem)) return 1;
     const dim3 grid((unsigned)slots, (unsigned)p.n_kv_heads, (unsigned)p.parts);
-    return launch_after("attn_rows_tc", kernel, grid, dim3(kThreads), smem, stream, 1, p);
+    return launch_after("attn_rows_tc", kernel, grid, dim3(Cfg<TD>::kThreads), smem, stream, 1, p);
 }
 inline int launch(const Params &p, long long slots, cudaStream_t stream) {
     g_last_path = "tcgen05";
