@@ -329,34 +329,32 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
             const bool hole = PAGED && __any_sync(0xffffffffu, at == kNoPage);
             if (lane == 0) sh->holes[place(j)][cw] = hole;
         };
-        const auto copy_part = [&](int P) {
-            const int u = P / PARTS, q = P % PARTS;
-            if (u < n_units) {
+        // A part's sixteen rows by eight threads each, a thread the chunks (ct & 7) + 8 i of its row: one look-up and one address a
+        // part, whole 128-byte lines a row, and sixteen threads write eight bytes each of two rows whose chunks lie in
+        // different banks (rows four apart, see the swizzle).
+        const int pr = (ct >> 3 & 1) << 2 | (ct >> 4 & 3) | (ct >> 6) << 3, pc = ct & 7;
+        const int my_chunks = (p.dim / 4 - pc + 7) / 8;  // of the head's columns; the rest of the tile's are zeros
+        const float *k_col = p.k + (long long)g * p.dim + pc * 4, *v_col = p.v + (long long)g * p.dim + pc * 4;
+        int cu = 0, cq = 0, cs = 0;  // the part that is copied next: unit, part, place in the ring
+        const auto copy_part = [&]() {
+            if (cu < n_units) {
                 bool is_k;
-                const int j = unit(u, is_k);
-                const float *base = is_k ? p.k : p.v;
-                const uint32_t dst = smem_u32(ring + (P % NP) * C::PART) + (uint32_t)ct * 16;
-                const long long *rows = rows_of(j) + q * 16;
-                long long at[CH];
+                const int j = unit(cu, is_k);
+                const long long at = rows_of(j)[cq * 16 + pr];
+                const float *src = (is_k ? k_col : v_col) + (at >= 0 ? at : 0);
+                const int have = at >= 0 ? my_chunks : 0;
+                const uint32_t dst = smem_u32(ring) + (uint32_t)(cs * C::PART + ct * 16);
 #pragma unroll
-                for (int i = 0; i < CH; ++i) at[i] = rows[(i * kConvert + ct) / CPR];
-#pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    const int c = (i * kConvert + ct) % CPR;
-                    const bool in = at[i] >= 0 && c * 4 < p.dim;
-                    copy16_async(dst + i * (kConvert * 16), in ? base + at[i] + (long long)g * p.dim + c * 4 : base, in);
-                }
+                for (int i = 0; i < CH; ++i) copy16_async(dst + i * (kConvert * 16), i < have ? src + i * 32 : p.k, i < have);
+                cs = cs + 1 == NP ? 0 : cs + 1;
+                if (++cq == PARTS) cq = 0, ++cu;
             }
             copy_async_commit();
         };
-        // a chunk's pieces into the operand tile: 64-column block, row, 16-byte chunk of eight halves with the 128-byte swizzle, its
-        // first or second half
-        const auto store_pieces = [&](uint8_t *dst, int f, uint2 h, uint2 l) {
-            const int r = f / CPR, c = f % CPR;
-            uint8_t *at = dst + (c >> 4) * (BN * 128) + r * 128 + ((((c & 15) >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
-            *reinterpret_cast<uint2 *>(at) = h;
-            *reinterpret_cast<uint2 *>(at + KP) = l;
-        };
+        // Where chunk (r, c) has its pieces in the operand tile: 64-column block, row, 16-byte chunk of eight halves with the
+        // 128-byte swizzle, its first or second half.
+        const auto piece_at = [](int r, int c) { return (c >> 4) * (BN * 128) + r * 128 + ((((c & 15) >> 1) ^ (r & 7)) << 4) + (c & 1) * 8; };
+        const uint32_t piece0 = (uint32_t)piece_at(pr, pc);  // (the thread's other chunks: bit 6 for the odd ones, then the next block)
         // A tile once more, from memory: the scale is its own, keys on no page are NaN, values that are not finite are noted and
         // left to the row threads.  Returns the scale.
         const auto with_care = [&](uint8_t *dst, bool is_k, int j, int u) -> float {
@@ -391,7 +389,9 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
                 uint2 h, l;
                 split_pack(x.x * m, x.y * m, h.x, l.x);
                 split_pack(x.z * m, x.w * m, h.y, l.y);
-                store_pieces(dst, f, h, l);
+                uint8_t *at = dst + piece_at(f / CPR, f % CPR);
+                *reinterpret_cast<uint2 *>(at) = h;
+                *reinterpret_cast<uint2 *>(at + KP) = l;
             }
             fence_async_smem();
             sync();
@@ -401,11 +401,12 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
         for (int j = 0; j < 4; ++j) look_up(j);
         sync();
 #pragma unroll 1
-        for (int P = 0; P < NP; ++P) copy_part(P);
+        for (int i = 0; i < NP; ++i) copy_part();
         bool ok = true;
         float m_k = 0.f, m_v = 0.f;  // the next tile's scales; 0: none yet
+        int place_now = 0;           // in the ring, of the part that is converted next
 #pragma unroll 1
-        for (int u = 0, P = 0; u < n_units; ++u) {
+        for (int u = 0; u < n_units; ++u) {
             bool is_k;
             const int j = unit(u, is_k), s = is_k ? j % KS : j % VS, S = is_k ? KS : VS;
             uint8_t *dst = (is_k ? sK : sV) + s * 2 * KP;
@@ -416,9 +417,10 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
             float m = is_k ? m_k : m_v;
             uint32_t top = 0;
 #pragma unroll 1
-            for (int q = 0; q < PARTS; ++q, ++P) {
+            for (int q = 0; q < PARTS; ++q) {
                 copy_async_wait<NP - 1>();
-                const float4 *raw = reinterpret_cast<const float4 *>(ring + (P % NP) * C::PART) + ct;
+                const float4 *raw = reinterpret_cast<const float4 *>(ring + place_now * C::PART) + ct;
+                place_now = place_now + 1 == NP ? 0 : place_now + 1;
                 float4 x[CH];
 #pragma unroll
                 for (int i = 0; i < CH; ++i) x[i] = raw[i * kConvert];
@@ -434,15 +436,18 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
                 }
                 if (!ok) continue;
                 const float2 mm = make_float2(m, m);
+                uint8_t *even = dst + q * (16 * 128) + piece0, *odd = dst + q * (16 * 128) + (piece0 ^ 64);
 #pragma unroll
                 for (int i = 0; i < CH; ++i) {
                     uint2 h, l;
                     split_pack(mul2(make_float2(x[i].x, x[i].y), mm), h.x, l.x);
                     split_pack(mul2(make_float2(x[i].z, x[i].w), mm), h.y, l.y);
                     top = __vmaxu2(top, __vmaxu2(h.x & 0x7fff7fffu, h.y & 0x7fff7fffu));
-                    store_pieces(dst, q * 16 * CPR + i * kConvert + ct, h, l);
+                    uint8_t *at = (i & 1 ? odd : even) + (i >> 1) * (BN * 128);
+                    *reinterpret_cast<uint2 *>(at) = h;
+                    *reinterpret_cast<uint2 *>(at + KP) = l;
                 }
-                copy_part(P + NP);  // (into the place of the chunks that this thread has just converted)
+                copy_part();  // (into the place of the chunks that this thread has just converted)
             }
             fence_async_smem();
             top = max(top & 0xffffu, top >> 16);
