@@ -23,8 +23,8 @@
 // four warps that convert K and four that convert V (above 128 columns the same four), a warp that issues S and one that
 // issues P V (a thread issues an MMA of N <= 64 every 50 clocks, the pipe takes one every 32), two idle ones that make the
 // four a group for setmaxnreg.
-// TMEM: up to 128 columns Q hi, Q lo, two O and two S/P buffers; above, Q hi, one O and two S/P buffers of 32 keys, Q lo in
-// shared memory.
+// TMEM: Q hi, Q lo (above 128 columns in shared memory), one O buffer (up to 64 columns two), four S/P buffers: S runs ahead of
+// the rows, so that a set finds the next tile's when it has made P of one and summed those before.
 #pragma once
 
 #include "paged_kernels.cuh"
@@ -47,40 +47,43 @@ using tcf16::store_q_piece;
 
 constexpr int kConvert = 128;  // threads that convert a tile
 
-template <int TD>
+template <int TD, bool PLANES>
 struct Cfg {
     static constexpr bool kWide = TD > 128;
     static constexpr int BN = kWide ? 32 : 64;      // keys of a tile
-    static constexpr int OB = kWide ? 1 : 2;        // O buffers
-    static constexpr int KS = TD == 256 ? 1 : 2, VS = KS;  // slots of converted K and V tiles
+    static constexpr int OB = TD == 64 ? 2 : 1;     // O buffers
+    static constexpr int SB = 4;                    // S/P buffers
+    static constexpr int KS = (TD == 256 ? 1 : 2) + (PLANES ? 1 : 0), VS = KS;  // slots of K and V tiles
     static constexpr int KP = BN * TD * 2;          // bytes of one piece of a tile
     static constexpr int QL = kWide ? 128 * TD * 2 : 0;
     // What is copied, waited for and converted at a time is 16 keys of a tile: `part`.  A thread has CHUNKS 16-byte chunks of it,
     // and a group of converting warps NP parts under way.
     static constexpr int PARTS = BN / 16, PART = 16 * TD * 4, CHUNKS = PART / 16 / kConvert;
-    static constexpr int GROUPS = kWide ? 1 : 2;
+    static constexpr int GROUPS = PLANES ? 0 : (kWide ? 1 : 2);
     static constexpr int NP = TD == 64 ? 8 : (TD == 128 ? 5 : 4);
     static constexpr int kThreads = 256 + GROUPS * kConvert + 128;
-    // registers a thread: the launch gives 640 threads 96 each, 512 threads 128
-    static constexpr int kLaunchRegs = kWide ? 128 : 96, kRowRegs = kWide ? 200 : 160, kConvertRegs = kWide ? 72 : 64, kIssueRegs = kWide ? 40 : 32;
+    // registers a thread: the launch gives 640 threads 96 each, 512 threads 128, 384 threads 168
+    static constexpr int kLaunchRegs = PLANES ? 168 : (kWide ? 128 : 96), kRowRegs = PLANES ? 216 : (kWide ? 200 : 160);
+    static constexpr int kConvertRegs = kWide ? 72 : 64, kIssueRegs = PLANES ? 72 : (kWide ? 40 : 32);
     static constexpr int kShare = 256 * kRowRegs + GROUPS * kConvert * kConvertRegs + 128 * kIssueRegs;
     static_assert(kShare <= kThreads * kLaunchRegs, "the groups share what the launch has");
-    static constexpr int cQh = 0, cQl = TD / 2, cO = kWide ? 128 : TD, cS = kWide ? 384 : 3 * TD;
+    static constexpr int cQh = 0, cQl = TD / 2, cO = kWide ? 128 : TD, cS = kWide ? 384 : (OB + 1) * TD;
+    static_assert(cO + OB * TD <= cS && cS + SB * BN <= 512, "tensor memory");
     static constexpr int kData = KS * 2 * KP + VS * 2 * KP + GROUPS * NP * PART + QL;
     static_assert(128 * (TD * 4 + 16) <= kData, "the finished rows are staged where the tiles were");
     static_assert(NP <= 2 * PARTS, "rows are looked up two tiles ahead");
 };
 
 struct Shared {
-    uint64_t k_full[2], k_free[2], v_full[2], v_free[2], a_ready, s_full[2], p_full[2], pv_done[2], o_full[2], o_free[2];
+    uint64_t k_full[3], k_free[3], v_full[3], v_free[3], a_ready, s_full[4], p_full[4], pv_done[4], o_full[2], o_free[2];
     uint32_t tmem_base;
     volatile int abort;
     int found;
-    float mk[4], mv[4];         // the scales of tiles j & 3
+    float mk[16], mv[16];       // the scales of tiles j & 15
     uint32_t odd[16][2];        // which values' rows of tile j & 15 hold something that is not finite
     uint32_t top[2][2][4];      // [group][unit & 1][warp]: the largest hi piece; or max |x|
     uint32_t seed[2][4];
-    float m_ref[4][128];        // the rows' reference maxima of tile j & 3
+    float m_ref[8][128];        // the rows' reference maxima of tile j & 7
     float fin_m[2][128], fin_l[2][128], q_top[2][128];
     // elements to the rows of the next tiles' keys (kNone: counts as zero, kNoPage: NaN): of a group's tile j & 3 or, in tiles
     // of 32 keys, of j & 7; and whether some key of the tile is on no page, by halves
@@ -99,6 +102,11 @@ struct Params {
     int batch, rows, T, n_heads, n_kv_heads, dim, parts;
     Seen seen;
     float scale_log2;
+    // Converted beforehand (rows_planes_kernel): every key tile's K hi, K lo, V hi, V lo as shared memory is to hold them, and what
+    // Shared holds of the tile; `tiles` of a sequence's KV head.
+    uint8_t *planes;
+    uint4 *heads;
+    int tiles;
 };
 
 __device__ __forceinline__ bool rwait(uint64_t *bar, uint32_t parity, Shared *sh) {
@@ -116,6 +124,10 @@ template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 // -inf for those of 32 keys from key0 on that the query at `pos` does not see.
@@ -148,10 +160,10 @@ struct RowTile {
     bool bad;
 };
 
-template <int TD, bool PAGED>
-__global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Params p) {
-    using C = Cfg<TD>;
-    constexpr int BN = C::BN, KP = C::KP, KS = C::KS, VS = C::VS, OB = C::OB, kThreads = C::kThreads, kIssuer = kThreads / 32 - 4;
+template <int TD, bool PAGED, bool PLANES>
+__global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(const Params p) {
+    using C = Cfg<TD, PLANES>;
+    constexpr int BN = C::BN, KP = C::KP, KS = C::KS, VS = C::VS, OB = C::OB, SB = C::SB, kThreads = C::kThreads, kIssuer = kThreads / 32 - 4;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *sK = smem, *sV = sK + KS * 2 * KP, *sRaw = sV + VS * 2 * KP, *sQl = sRaw + C::GROUPS * C::NP * C::PART;
     Shared *sh = reinterpret_cast<Shared *>(sQl + C::QL);
@@ -218,12 +230,12 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
     const auto key0 = [&](int j) { return tiles.at(jb + j) * BN; };
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 3; ++i) {
             mbar_init(&sh->k_full[i], 1), mbar_init(&sh->k_free[i], 1);
             mbar_init(&sh->v_full[i], 1), mbar_init(&sh->v_free[i], 1);
-            mbar_init(&sh->s_full[i], 1), mbar_init(&sh->p_full[i], 4), mbar_init(&sh->pv_done[i], 1);
-            mbar_init(&sh->o_full[i], 1), mbar_init(&sh->o_free[i], 8);
         }
+        for (int i = 0; i < SB; ++i) mbar_init(&sh->s_full[i], 1), mbar_init(&sh->p_full[i], 4), mbar_init(&sh->pv_done[i], 1);
+        for (int i = 0; i < OB; ++i) mbar_init(&sh->o_full[i], 1), mbar_init(&sh->o_free[i], 8);
         mbar_init(&sh->a_ready, 8);
         sh->abort = (smem_u32(smem) & 1023u) ? 100 : 0;
         if (sh->abort) atomicMax(&g_tc_status, 100);
@@ -239,7 +251,7 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
     if (warp >= kIssuer) {
         fewer_registers<C::kIssueRegs>();
         if (warp == kIssuer) {
-            // -------------------------------------------------------------- S(j) = Q K^T into buffer j & 1
+            // -------------------------------------------------------------- S(j) = Q K^T into buffer j % SB
             if (elect_one()) {
                 constexpr uint32_t id_s = idesc_f16(128, BN, false, false);
                 bool ok = rwait(&sh->a_ready, 0, sh);
@@ -247,11 +259,11 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
                 const uint32_t k_u32 = smem_u32(sK), ql_u32 = smem_u32(sQl);
                 for (int j = 0; ok && j < n; ++j) {
                     const int s = j % KS;
-                    // (over P(j - 2), which its product has read)
+                    // (over P(j - SB), which its product has read)
                     if (!rwait(&sh->k_full[s], (uint32_t)((j / KS) & 1), sh) ||
-                        (j >= 2 && !rwait(&sh->pv_done[j & 1], (uint32_t)(((j >> 1) - 1) & 1), sh))) { rgive_up(sh, 102); break; }
+                        (j >= SB && !rwait(&sh->pv_done[j % SB], (uint32_t)((j / SB - 1) & 1), sh))) { rgive_up(sh, 102); break; }
                     tc_fence_after();
-                    const uint32_t cS = C::cS + (j & 1) * BN;
+                    const uint32_t cS = C::cS + (j % SB) * BN;
                     const uint64_t bkh = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP)), bkl = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP + KP));
                     const uint64_t bql = desc_kmajor(ql_u32);
 #pragma unroll
@@ -265,7 +277,7 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
                         else mma_ts_f16(tmem + cS, tmem + C::cQl + kk * 8, dkh, id_s, 1);
                     }
                     mma_commit(&sh->k_free[s]);
-                    mma_commit(&sh->s_full[j & 1]);
+                    mma_commit(&sh->s_full[j % SB]);
                 }
             }
             __syncwarp();
@@ -276,12 +288,12 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
                 const uint32_t v_u32 = smem_u32(sV);
                 for (int j = 0; j < n; ++j) {
                     const int s = j % VS, ob = j % OB;
-                    if (!rwait(&sh->p_full[j & 1], (uint32_t)((j >> 1) & 1), sh) || !rwait(&sh->v_full[s], (uint32_t)((j / VS) & 1), sh) ||
+                    if (!rwait(&sh->p_full[j % SB], (uint32_t)((j / SB) & 1), sh) || !rwait(&sh->v_full[s], (uint32_t)((j / VS) & 1), sh) ||
                         (j >= OB && !rwait(&sh->o_free[ob], (uint32_t)((j / OB - 1) & 1), sh))) { rgive_up(sh, 103); break; }
                     tc_fence_after();
                     const uint32_t vh = v_u32 + (uint32_t)(s * 2 * KP);
                     const uint64_t mvh = desc_mnmajor_16b(vh, BN * 128), mvl = desc_mnmajor_16b(vh + KP, BN * 128);
-                    const uint32_t cS = C::cS + (j & 1) * BN, cO = C::cO + ob * TD;
+                    const uint32_t cS = C::cS + (j % SB) * BN, cO = C::cO + ob * TD;
 #pragma unroll
                     for (int kk = 0; kk < BN / 16; ++kk) {
                         const uint32_t ac = (uint32_t)(32 * (kk >> 1) + (kk & 1) * 8);
@@ -292,12 +304,47 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
                     }
                     mma_commit(&sh->v_free[s]);
                     mma_commit(&sh->o_full[ob]);
-                    mma_commit(&sh->pv_done[j & 1]);
+                    mma_commit(&sh->pv_done[j % SB]);
+                }
+            }
+            __syncwarp();
+        } else if (PLANES && warp == kIssuer + 2) {
+            // -------------------------------------------------------------- the converted tiles, in the order in which they are asked for
+            if (elect_one() && !sh->abort) {
+                const long long first = ((long long)t.b * p.n_kv_heads + g) * p.tiles;
+                const auto tile_at = [&](int j) { return first + tiles.at(jb + j); };
+                int n_k = 0, n_v = 0;  // copied
+                bool ok = true;
+                uint4 head = p.heads[tile_at(0)];
+                const auto copy_v = [&](int j) {
+                    const int s = j % VS;
+                    if (j >= VS && !rwait(&sh->v_free[s], (uint32_t)((j / VS - 1) & 1), sh)) { rgive_up(sh, 107), ok = false; return; }
+                    mbar_arrive_expect_tx(&sh->v_full[s], 2 * KP);
+                    bulk_load(sV + s * 2 * KP, p.planes + tile_at(j) * (4 * KP) + 2 * KP, 2 * KP, &sh->v_full[s]);
+                    ++n_v;
+                };
+                for (int j = 0; ok && j < n; ++j) {
+                    const int s = j % KS;
+                    const uint4 now = head;
+                    if (j + 1 < n) head = p.heads[tile_at(j + 1)];
+                    if (j >= KS && !rwait(&sh->k_free[s], (uint32_t)((j / KS - 1) & 1), sh)) { rgive_up(sh, 107), ok = false; break; }
+                    sh->mk[j & 15] = __uint_as_float(now.x), sh->mv[j & 15] = __uint_as_float(now.y);
+                    sh->odd[j & 15][0] = now.z, sh->odd[j & 15][1] = now.w;
+                    mbar_arrive_expect_tx(&sh->k_full[s], 2 * KP);
+                    bulk_load(sK + s * 2 * KP, p.planes + tile_at(j) * (4 * KP), 2 * KP, &sh->k_full[s]);
+                    ++n_k;
+                    if (j > 0) copy_v(j - 1);
+                }
+                if (ok) copy_v(n - 1);
+                if (sh->abort) {
+                    // let the copies in flight land before the CTA's shared memory goes away
+                    for (int j = (n_k > KS ? n_k - KS : 0); j < n_k; ++j) mbar_wait(&sh->k_full[j % KS], (uint32_t)((j / KS) & 1));
+                    for (int j = (n_v > VS ? n_v - VS : 0); j < n_v; ++j) mbar_wait(&sh->v_full[j % VS], (uint32_t)((j / VS) & 1));
                 }
             }
             __syncwarp();
         }
-    } else if (warp >= 8) {
+    } else if (!PLANES && warp >= 8) {
         // ------------------------------------------------------------------ keys and values: copied, scaled, split.  A group's
         // units are tiles of K, or of V, or of both in the order in which the MMAs ask for them: K0, K1, V0, K2, V1, ...
         fewer_registers<C::kConvertRegs>();
@@ -461,7 +508,7 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
             const bool care = top < 0x3000u || top >= 0x7c00u || (is_k && hole);
             if (care) m = with_care(dst, is_k, j, u);
             if (ct == 0) {
-                (is_k ? sh->mk : sh->mv)[j & 3] = m;
+                (is_k ? sh->mk : sh->mv)[j & 15] = m;
                 if (ok) mbar_arrive(is_k ? &sh->k_full[s] : &sh->v_full[s]);
             }
             // the next tile's: with which this one's largest would have been in [2^12, 2^13)
@@ -519,7 +566,7 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
                 return false;
             }
             tc_fence_after();
-            const float mj = sh->m_ref[j & 3][tid];
+            const float mj = sh->m_ref[j & 7][tid];
             if (__any_sync(0xffffffffu, mj > m_o)) {
                 const float f = mj > m_o ? ex2(m_o - mj) : 1.f;
                 m_o = fmaxf(m_o, mj);
@@ -527,7 +574,7 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
                 for (int c = 0; c < TD / 4; ++c) o[c] = mul2(o[c], make_float2(f, f));
             }
             // (no key of the tile or before it is seen: P is zero)
-            const float w = mj == -INFINITY ? 0.f : ex2(mj - m_o) / sh->mv[j & 3];
+            const float w = mj == -INFINITY ? 0.f : ex2(mj - m_o) / sh->mv[j & 15];
             const uint32_t from = tmem + lane_base + C::cO + ob * TD + set * (TD / 2);
 #pragma unroll
             for (int c = 0; c < TD / 2; c += 32) {
@@ -565,15 +612,15 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
         // positions of this warp's rows: which tiles need a mask
         const int warp_first = __shfl_sync(0xffffffffu, pos, 0), warp_last = __shfl_sync(0xffffffffu, pos, 31);
         for (int j = set; ok && j < n; j += 2) {
-            if (!__all_sync(0xffffffffu, rwait(&sh->s_full[set], (uint32_t)((j >> 1) & 1), sh))) {
+            if (!__all_sync(0xffffffffu, rwait(&sh->s_full[j % SB], (uint32_t)((j / SB) & 1), sh))) {
                 rgive_up(sh, 105);
                 ok = false;
                 break;
             }
             tc_fence_after();
             const int s0 = key0(j);
-            const float cs = fmaxf(cs0 / sh->mk[j & 3], 1.17549435e-38f);
-            const uint32_t cS = tmem + lane_base + C::cS + set * BN;
+            const float cs = fmaxf(cs0 / sh->mk[j & 15], 1.17549435e-38f);
+            const uint32_t cS = tmem + lane_base + C::cS + (j % SB) * BN;
             const Seen &v = p.seen;
             const bool masked = s0 + BN - 1 > warp_first || (v.window > 0 && s0 <= warp_last - v.window && s0 + BN > v.sinks);
             // 32 columns of S at a time: they come out of TMEM a second time for their exponentials, so that a thread's registers
@@ -595,7 +642,7 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
                 l *= m_ref == -INFINITY ? 0.f : ex2(m_ref - mt);
                 m_ref = mt;
             }
-            sh->m_ref[j & 3][tid] = m_ref;
+            sh->m_ref[j & 7][tid] = m_ref;
             const float off = ((m_ref == -INFINITY) ? 0.f : m_ref) - 7.0f;  // log2 kPScale: l and O are in P's units
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
@@ -607,8 +654,8 @@ __global__ void __launch_bounds__(Cfg<TD>::kThreads, 1) attn_rows_tc(const Param
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive_warp(&sh->p_full[set]);
-            for (; ok && added <= j; ++added) ok = add_tile(added);
+            mbar_arrive_warp(&sh->p_full[j % SB]);
+            for (; ok && added < j; ++added) ok = add_tile(added);
         }
         for (; ok && added < n; ++added) ok = add_tile(added);
         // ---- the two sets' sums of exponentials; every thread then has its half of the row
@@ -666,26 +713,125 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const Params p, float *o
     if (lse && lane == 0) lse[row] = top + log2f(sum) * kLn2;
 }
 
+// Key tiles for a launch that reads them converted: a block per (tile, KV head, sequence), half of its threads for K and half for
+// V.  Reads f32 rows that some row of the sequence sees, writes as much; bound by memory.
+template <int TD, bool PAGED>
+__global__ void __launch_bounds__(256) rows_planes_kernel(const Params p) {
+    using C = Cfg<TD, true>;
+    constexpr int BN = C::BN, KP = C::KP, N = BN / 16 * (TD / 32);  // (N: chunks of a thread)
+    __shared__ uint32_t tops[2][4], odd[2];
+    pdl_wait();
+    pdl_launch();
+    const int tile = blockIdx.x, g = blockIdx.y, b = blockIdx.z, key0 = tile * BN;
+    int first = 0, last = p.T - 1;  // positions of the sequence's rows
+    if (PAGED) {
+        const NewRows r = new_rows(p.cu_rows, p.n_keys, b, p.rows, p.pg, true);
+        if (r.bad || r.count == 0) return;
+        first = r.pos, last = r.pos + r.count - 1;
+    }
+    // (some row sees it: the first one's window is the lowest)
+    const auto seen = [&](int key) { return key <= last && (p.seen.window == 0 || key > first - p.seen.window || key < p.seen.sinks); };
+    if (key0 > last || (p.seen.window > 0 && key0 + BN - 1 <= first - p.seen.window && key0 >= p.seen.sinks)) return;  // none of the tile's
+    const int ct = threadIdx.x & 127, lane = threadIdx.x & 31;
+    const bool is_k = threadIdx.x < 128;
+    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+    const int pr = (ct >> 3 & 1) << 2 | (ct >> 4 & 3) | (ct >> 6) << 3, pc = ct & 7;  // (see the converting warps)
+    const float *col = (is_k ? p.k : p.v) + (long long)g * p.dim + pc * 4;
+    const long long width = PAGED ? p.pg.width : (long long)p.n_kv_heads * p.dim;
+    float4 x[N];
+    bool hole[BN / 16];
+#pragma unroll
+    for (int q = 0; q < BN / 16; ++q) {
+        const int key = key0 + q * 16 + pr;
+        const long long at = !seen(key) ? kNone : PAGED ? p.pg.row(b, key) : ((long long)b * p.T + key) * width;
+        hole[q] = PAGED && seen(key) && at < 0;
+#pragma unroll
+        for (int i = 0; i < TD / 32; ++i)
+            x[q * (TD / 32) + i] = at >= 0 && (pc + 8 * i) * 4 < p.dim ? *reinterpret_cast<const float4 *>(col + at + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __syncthreads();
+    uint32_t top = 0;
+#pragma unroll
+    for (int q = 0; q < BN / 16; ++q)
+#pragma unroll
+        for (int i = 0; i < TD / 32; ++i) {
+            float4 &y = x[q * (TD / 32) + i];
+            for (float *e : {&y.x, &y.y, &y.z, &y.w}) {
+                const bool fine = finite(*e);
+                top = max(top, fine ? __float_as_uint(*e) & 0x7fffffffu : 0u);
+                if (!fine && !is_k) {
+                    *e = 0.f;
+                    const int r = q * 16 + pr;
+                    atomicOr(&odd[r >> 5], 1u << (r & 31));
+                }
+            }
+            if (is_k && hole[q]) y.x = __int_as_float(0x7fc00000);
+        }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[is_k ? 0 : 1][(threadIdx.x >> 5) & 3] = top;
+    __syncthreads();
+    float m[2];
+    for (int i = 0; i < 2; ++i) m[i] = block_mult(max(max(tops[i][0], tops[i][1]), max(tops[i][2], tops[i][3]))) * 0.25f;
+    const long long at = ((long long)b * p.n_kv_heads + g) * p.tiles + tile;
+    if (threadIdx.x == 0) p.heads[at] = make_uint4(__float_as_uint(m[0]), __float_as_uint(m[1]), odd[0], odd[1]);
+    uint8_t *dst = p.planes + at * (4 * KP) + (is_k ? 0 : 2 * KP);
+    const float2 mm = is_k ? make_float2(m[0], m[0]) : make_float2(m[1], m[1]);
+#pragma unroll
+    for (int q = 0; q < BN / 16; ++q)
+#pragma unroll
+        for (int i = 0; i < TD / 32; ++i) {
+            const float4 y = x[q * (TD / 32) + i];
+            const int r = q * 16 + pr, c = pc + 8 * i;
+            uint2 h, l;
+            split_pack(mul2(make_float2(y.x, y.y), mm), h.x, l.x);
+            split_pack(mul2(make_float2(y.z, y.w), mm), h.y, l.y);
+            uint8_t *to = dst + (c >> 4) * (BN * 128) + r * 128 + ((((c & 15) >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
+            *reinterpret_cast<uint2 *>(to) = h;
+            *reinterpret_cast<uint2 *>(to + KP) = l;
+        }
+}
+
+// Keys of a tile, and bytes of the converted tiles of `keys` keys of `batch` sequences with their heads.
+inline int tile_keys(int dim) { return tc_tile_dim(dim) > 128 ? 32 : 64; }
+inline long long key_tiles(int keys, int dim) { return ((long long)keys + tile_keys(dim) - 1) / tile_keys(dim); }
+inline size_t planes_bytes(int batch, int keys, int n_kv_heads, int dim) {
+    return (size_t)batch * n_kv_heads * (size_t)key_tiles(keys, dim) * ((size_t)4 * tile_keys(dim) * tc_tile_dim(dim) * 2 + sizeof(uint4)) + 512;
+}
+inline void place_planes(Params &p, void *scratch, int keys) {
+    p.tiles = (int)key_tiles(keys, p.dim);
+    uint8_t *c = static_cast<uint8_t *>(scratch);
+    c += (256 - (reinterpret_cast<uintptr_t>(c) & 255u)) & 255u;
+    p.planes = c;
+    p.heads = reinterpret_cast<uint4 *>(c + (size_t)p.batch * p.n_kv_heads * p.tiles * ((size_t)4 * tile_keys(p.dim) * tc_tile_dim(p.dim) * 2));
+}
+
 // The register shares are taken from what the kernel was compiled to be launched with: less than their sum, and a group that asks
 // for its share would wait for good.
-template <int TD, bool PAGED>
+template <int TD, bool PAGED, bool PLANES>
 inline bool registers_suffice() {
     cudaFuncAttributes a{};
-    if (cudaFuncGetAttributes(&a, attn_rows_tc<TD, PAGED>) != cudaSuccess) {
+    if (cudaFuncGetAttributes(&a, attn_rows_tc<TD, PAGED, PLANES>) != cudaSuccess) {
         cudaGetLastError();
         return false;
     }
-    return a.numRegs * Cfg<TD>::kThreads >= Cfg<TD>::kShare;
+    return a.numRegs * Cfg<TD, PLANES>::kThreads >= Cfg<TD, PLANES>::kShare;
+}
+template <int TD, bool PAGED, bool PLANES>
+inline int launch_as(const Params &p, long long slots, cudaStream_t stream) {
+    static const bool suffice = registers_suffice<TD, PAGED, PLANES>();
+    if (!suffice) return refuse("attn_rows_tc was not compiled for the registers that its warps share out.");
+    const size_t smem = (size_t)Cfg<TD, PLANES>::kData + sizeof(Shared);
+    if (optin_smem((const void *)attn_rows_tc<TD, PAGED, PLANES>, smem)) return 1;
+    if (PLANES && launch_pdl("rows_planes_kernel", rows_planes_kernel<TD, PAGED>, dim3((unsigned)p.tiles, (unsigned)p.n_kv_heads, (unsigned)p.batch),
+                             dim3(256), 0, stream, p))
+        return 1;
+    const dim3 grid((unsigned)slots, (unsigned)p.n_kv_heads, (unsigned)p.parts);
+    return launch_after("attn_rows_tc", attn_rows_tc<TD, PAGED, PLANES>, grid, dim3(Cfg<TD, PLANES>::kThreads), smem, stream, 1, p);
 }
 template <int TD>
 inline int launch_td(const Params &p, long long slots, cudaStream_t stream) {
-    static const bool suffice = registers_suffice<TD, true>() && registers_suffice<TD, false>();
-    if (!suffice) return refuse("attn_rows_tc was not compiled for the registers that its warps share out.");
-    const size_t smem = (size_t)Cfg<TD>::kData + sizeof(Shared);
-    const auto kernel = p.pg.table ? attn_rows_tc<TD, true> : attn_rows_tc<TD, false>;
-    if (optin_smem((const void *)kernel, smem)) return 1;
-    const dim3 grid((unsigned)slots, (unsigned)p.n_kv_heads, (unsigned)p.parts);
-    return launch_after("attn_rows_tc", kernel, grid, dim3(Cfg<TD>::kThreads), smem, stream, 1, p);
+    if (p.planes) return p.pg.table ? launch_as<TD, true, true>(p, slots, stream) : launch_as<TD, false, true>(p, slots, stream);
+    return p.pg.table ? launch_as<TD, true, false>(p, slots, stream) : launch_as<TD, false, false>(p, slots, stream);
 }
 inline int launch(const Params &p, long long slots, cudaStream_t stream) {
     g_last_path = "tcgen05";

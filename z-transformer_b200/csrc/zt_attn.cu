@@ -1178,6 +1178,9 @@ int zt_attn_forward_window_batched(const float *q, const float *k, const float *
         p.batch = batch, p.T = T, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.dim = dim, p.parts = 1;
         p.seen = Seen{window, sinks};
         p.scale_log2 = kLog2e / sqrtf((float)dim);
+        const bool planes = getenv("ZT_PLANES") ? atoi(getenv("ZT_PLANES")) : 0;
+        const StreamScratch scratch(planes ? tcr::planes_bytes(batch, T, n_kv_heads, dim) : 0, (cudaStream_t)stream);
+        if (scratch.get()) tcr::place_planes(p, scratch.get(), T);
         return tcr::launch(p, (long long)batch * (((long long)T * (n_heads / n_kv_heads) + 127) / 128), (cudaStream_t)stream);
     }
     SimtFwdParams p{};
