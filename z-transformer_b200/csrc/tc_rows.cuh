@@ -23,6 +23,8 @@
 // four warps that convert K and four that convert V (above 128 columns the same four), a warp that issues S and one that
 // issues P V (a thread issues an MMA of N <= 64 every 50 clocks, the pipe takes one every 32), two idle ones that make the
 // four a group for setmaxnreg.
+// Many rows of a sequence see the same keys: where a launch before this one (rows_planes_kernel) has converted them, whole tiles
+// come by bulk copies, and the converting warps' place is taken by row warps, of which some make P and others sum.
 // TMEM: Q hi, Q lo (above 128 columns in shared memory), one O buffer (up to 64 columns two), four S/P buffers: S runs ahead of
 // the rows, so that a set finds the next tile's when it has made P of one and summed those before.
 #pragma once
@@ -61,11 +63,13 @@ struct Cfg {
     static constexpr int PARTS = BN / 16, PART = 16 * TD * 4, CHUNKS = PART / 16 / kConvert;
     static constexpr int GROUPS = PLANES ? 0 : (kWide ? 1 : 2);
     static constexpr int NP = TD == 64 ? 8 : (TD == 128 ? 5 : 4);
-    static constexpr int kThreads = 256 + GROUPS * kConvert + 128;
-    // registers a thread: the launch gives 640 threads 96 each, 512 threads 128, 384 threads 168
-    static constexpr int kLaunchRegs = PLANES ? 168 : (kWide ? 128 : 96), kRowRegs = PLANES ? 216 : (kWide ? 200 : 160);
-    static constexpr int kConvertRegs = kWide ? 72 : 64, kIssueRegs = PLANES ? 72 : (kWide ? 40 : 32);
-    static constexpr int kShare = 256 * kRowRegs + GROUPS * kConvert * kConvertRegs + 128 * kIssueRegs;
+    static constexpr int SETS = PLANES && kWide ? 1 : 2;  // of warps that make P: with tiles of 32 keys of wide heads one keeps up
+    static constexpr int kThreads = (PLANES ? 128 * SETS : GROUPS * kConvert) + 256 + 128;
+    // registers a thread, of what the launch gives: 640 threads 96 each, 512 threads 128
+    static constexpr int kLaunchRegs = kWide ? 128 : 96;
+    static constexpr int kRowRegs = kWide ? (PLANES ? 184 : 200) : (PLANES ? 120 : 160);
+    static constexpr int kSoftRegs = 104, kConvertRegs = kWide ? 72 : 64, kIssueRegs = kWide ? 40 : 32;
+    static constexpr int kShare = 256 * kRowRegs + (PLANES ? 128 * SETS * kSoftRegs : GROUPS * kConvert * kConvertRegs) + 128 * kIssueRegs;
     static_assert(kShare <= kThreads * kLaunchRegs, "the groups share what the launch has");
     static constexpr int cQh = 0, cQl = TD / 2, cO = kWide ? 128 : TD, cS = kWide ? 384 : (OB + 1) * TD;
     static_assert(cO + OB * TD <= cS && cS + SB * BN <= 512, "tensor memory");
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             is_k = both ? u == 0 || ((u & 1) && u != n_units - 1) : gi == 0;
             return !both ? u : u == 0 ? 0 : (is_k ? (u + 1) >> 1 : (u == n_units - 1 ? n - 1 : (u >> 1) - 1));
         };
-        const auto sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(2 + gi) : "memory"); };
+        const auto sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(3 + gi) : "memory"); };
         // where the keys of tile j lie; one that no row of this CTA sees counts as zero
         const auto place = [&](int j) { return both ? j & 7 : gi * 4 + (j & 3); };
         const auto rows_of = [&](int j) { return sh->row + place(j) * BN; };
@@ -518,48 +522,94 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
         }
         copy_async_wait<0>();
     } else {
-        // ------------------------------------------------------------------ rows
-        more_registers<C::kRowRegs>();
-        const int tid = threadIdx.x & 127, set = threadIdx.x >> 7;
+        // ------------------------------------------------------------------ rows.  A thread of a set of four warps has a row; of the
+        // two sets that sum, half of its columns.
+        const int tid = threadIdx.x & 127;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const bool mine = tid < n_rows;
         const int pos = t.pos + (t.f0 + (mine ? tid : n_rows - 1)) / group;  // (rows past the last repeat it, with q zero)
         const long long rh = mine ? row_head(tid) : 0;
         bool ok = true;
-        float cs0;  // scale_log2 over the row's scale
-        {
+        // The row's pieces of q, a half of its columns by each of 256 threads.  (Shared::q_top has the halves' maxima.)
+        const auto place_q = [&](int half) {
             float4 x[TD / 8];
             float top = 0.f;
 #pragma unroll
             for (int c = 0; c < TD / 8; ++c) {
-                const int col = set * (TD / 2) + c * 4;
+                const int col = half * (TD / 2) + c * 4;
                 x[c] = mine && col < p.dim ? *reinterpret_cast<const float4 *>(p.q + rh * p.dim + col) : make_float4(0.f, 0.f, 0.f, 0.f);
                 top = fmaxf(top, max_abs4(x[c]));
             }
-            sh->q_top[set][tid] = top;
+            sh->q_top[half][tid] = top;
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            top = fmaxf(top, sh->q_top[set ^ 1][tid]);
-            const float m = block_mult(__float_as_uint(top));
-            cs0 = p.scale_log2 / m;
+            const float m = block_mult(__float_as_uint(fmaxf(top, sh->q_top[half ^ 1][tid])));
 #pragma unroll
             for (int cb = 0; cb < TD / 64; ++cb) {
                 uint32_t qh[16], ql[16];
                 split_q32([&](int c) { return x[cb * 8 + c]; }, m, qh, ql);
-                tmem_st16(tmem + lane_base + C::cQh + set * (TD / 4) + cb * 16, qh);
-                if (C::kWide) store_q_piece(sQl, tid, set * (TD / 64) + cb, ql);
-                else tmem_st16(tmem + lane_base + C::cQl + set * (TD / 4) + cb * 16, ql);
+                tmem_st16(tmem + lane_base + C::cQh + half * (TD / 4) + cb * 16, qh);
+                if (C::kWide) store_q_piece(sQl, tid, half * (TD / 64) + cb, ql);
+                else tmem_st16(tmem + lane_base + C::cQl + half * (TD / 4) + cb * 16, ql);
             }
             tmem_wait_st();
             if (C::kWide) fence_async_smem();
             tc_fence_before();
             mbar_arrive_warp(&sh->a_ready);
-        }
-        float2 o[TD / 4];  // this set's half of the row's columns, relative to m_o
+        };
+        // positions of this warp's rows: which tiles need a mask
+        const int warp_first = __shfl_sync(0xffffffffu, pos, 0), warp_last = __shfl_sync(0xffffffffu, pos, 31);
+        float cs0 = 0.f, m_ref = -INFINITY, l = 0.f;
+        // P of tile j over S
+        const auto make_p = [&](int j) -> bool {
+            if (!__all_sync(0xffffffffu, rwait(&sh->s_full[j % SB], (uint32_t)((j / SB) & 1), sh))) {
+                rgive_up(sh, 105);
+                return false;
+            }
+            tc_fence_after();
+            if (cs0 == 0.f) cs0 = fmaxf(p.scale_log2 / block_mult(__float_as_uint(fmaxf(sh->q_top[0][tid], sh->q_top[1][tid]))), 1.17549435e-38f);
+            const int s0 = key0(j);
+            const float cs = fmaxf(cs0 / sh->mk[j & 15], 1.17549435e-38f);
+            const uint32_t cS = tmem + lane_base + C::cS + (j % SB) * BN;
+            const Seen &v = p.seen;
+            const bool masked = s0 + BN - 1 > warp_first || (v.window > 0 && s0 <= warp_last - v.window && s0 + BN > v.sinks);
+            // Where a thread also holds its half of O, 32 columns of S at a time: they come out of TMEM a second time for their
+            // exponentials.
+            constexpr bool kTwice = !PLANES && BN > 32;
+            constexpr int R = BN > 32 && !kTwice ? 2 : 1;
+            uint32_t r[R][32];
+            const auto scores = [&](uint32_t(&x)[32], int c) {
+                tmem_ld32(cS + c, x);
+                tmem_wait_ld();
+                if (masked) mask_scores(x, v, s0 + c, pos);
+            };
+            float mt = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < TD / 4; ++c) o[c] = make_float2(0.f, 0.f);
-        float m_o = -INFINITY, m_ref = -INFINITY, l = 0.f;
-        // adds tile j's P V to the row
-        const auto add_tile = [&](int j) -> bool {
+            for (int c = 0; c < BN; c += 32) {
+                scores(r[c / 32 % R], c);
+                mt = row_max32(r[c / 32 % R], mt);
+            }
+            mt *= cs;  // cs > 0
+            if ((mt > m_ref + tcf16::kRescaleThreshold || m_ref == -INFINITY) && mt != -INFINITY) {
+                l *= m_ref == -INFINITY ? 0.f : ex2(m_ref - mt);
+                m_ref = mt;
+            }
+            sh->m_ref[j & 7][tid] = m_ref;
+            const float off = ((m_ref == -INFINITY) ? 0.f : m_ref) - 7.0f;  // log2 kPScale: l and O are in P's units
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) {
+                uint32_t ph[16], pl[16];
+                if (kTwice) scores(r[0], c);
+                l += row_exp32(r[c / 32 % R], cs, off, ph, pl);
+                tmem_st16(cS + c, ph);
+                tmem_st16(cS + c + 16, pl);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive_warp(&sh->p_full[j % SB]);
+            return true;
+        };
+        // Adds tile j's P V to the thread's half of the row, which is relative to m_o.
+        const auto add_tile = [&](int j, int half, float2(&o)[TD / 4], float &m_o) -> bool {
             const int ob = j % OB;
             if (!__all_sync(0xffffffffu, rwait(&sh->o_full[ob], (uint32_t)((j / OB) & 1), sh))) {
                 rgive_up(sh, 106);
@@ -575,7 +625,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             }
             // (no key of the tile or before it is seen: P is zero)
             const float w = mj == -INFINITY ? 0.f : ex2(mj - m_o) / sh->mv[j & 15];
-            const uint32_t from = tmem + lane_base + C::cO + ob * TD + set * (TD / 2);
+            const uint32_t from = tmem + lane_base + C::cO + ob * TD + half * (TD / 2);
 #pragma unroll
             for (int c = 0; c < TD / 2; c += 32) {
                 uint32_t r[32];
@@ -590,6 +640,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             }
             const uint32_t odd[2] = {sh->odd[j & 15][0], sh->odd[j & 15][1]};
             if (odd[0] | odd[1]) {  // values that are not finite, added to the rows that see them
+#pragma unroll 1
                 for (int i = 0; i < BN; ++i) {
                     const int key = key0(j) + i;
                     if (!(odd[i >> 5] >> (i & 31) & 1u) || !p.seen(key, pos)) continue;
@@ -597,7 +648,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                     if (at < 0) continue;
 #pragma unroll
                     for (int c = 0; c < TD / 4; ++c) {
-                        const int col = set * (TD / 2) + 2 * c;
+                        const int col = half * (TD / 2) + 2 * c;
                         if (col >= p.dim) continue;
                         const float2 x = *reinterpret_cast<const float2 *>(p.v + at + (long long)g * p.dim + col);
                         if (!finite(x.x)) o[c].x += x.x;
@@ -608,73 +659,48 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             }
             return true;
         };
-        int added = 0;
-        // positions of this warp's rows: which tiles need a mask
-        const int warp_first = __shfl_sync(0xffffffffu, pos, 0), warp_last = __shfl_sync(0xffffffffu, pos, 31);
-        for (int j = set; ok && j < n; j += 2) {
-            if (!__all_sync(0xffffffffu, rwait(&sh->s_full[j % SB], (uint32_t)((j / SB) & 1), sh))) {
-                rgive_up(sh, 105);
-                ok = false;
-                break;
-            }
-            tc_fence_after();
-            const int s0 = key0(j);
-            const float cs = fmaxf(cs0 / sh->mk[j & 15], 1.17549435e-38f);
-            const uint32_t cS = tmem + lane_base + C::cS + (j % SB) * BN;
-            const Seen &v = p.seen;
-            const bool masked = s0 + BN - 1 > warp_first || (v.window > 0 && s0 <= warp_last - v.window && s0 + BN > v.sinks);
-            // 32 columns of S at a time: they come out of TMEM a second time for their exponentials, so that a thread's registers
-            // hold its half of O beside them
-            uint32_t r[32];
-            const auto scores = [&](int c) {
-                tmem_ld32(cS + c, r);
-                tmem_wait_ld();
-                if (masked) mask_scores(r, v, s0 + c, pos);
-            };
-            float mt = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < BN; c += 32) {
-                scores(c);
-                mt = row_max32(r, mt);
-            }
-            mt *= cs;  // cs > 0
-            if ((mt > m_ref + tcf16::kRescaleThreshold || m_ref == -INFINITY) && mt != -INFINITY) {
-                l *= m_ref == -INFINITY ? 0.f : ex2(m_ref - mt);
-                m_ref = mt;
-            }
-            sh->m_ref[j & 7][tid] = m_ref;
-            const float off = ((m_ref == -INFINITY) ? 0.f : m_ref) - 7.0f;  // log2 kPScale: l and O are in P's units
-#pragma unroll
-            for (int c = 0; c < BN; c += 32) {
-                uint32_t ph[16], pl[16];
-                if (BN > 32) scores(c);
-                l += row_exp32(r, cs, off, ph, pl);
-                tmem_st16(cS + c, ph);
-                tmem_st16(cS + c + 16, pl);
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive_warp(&sh->p_full[j % SB]);
-            for (; ok && added < j; ++added) ok = add_tile(added);
-        }
-        for (; ok && added < n; ++added) ok = add_tile(added);
-        // ---- the two sets' sums of exponentials; every thread then has its half of the row
-        sh->fin_m[set][tid] = m_ref, sh->fin_l[set][tid] = l;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (ok) {
-            const float m0 = sh->fin_m[0][tid], m1 = sh->fin_m[1][tid], mm = fmaxf(m0, m1);
+        // The row leaves: the sets' sums of exponentials together, then every half as one bulk copy.
+        const auto publish_sums = [&](int set) { sh->fin_m[set][tid] = m_ref, sh->fin_l[set][tid] = l; };
+        const auto send_rows = [&](int half, const float2(&o)[TD / 4], float m_o) {
+            const float m0 = sh->fin_m[0][tid], m1 = C::SETS > 1 ? sh->fin_m[1][tid] : -INFINITY, mm = fmaxf(m0, m1);
             // (a part may hold no key that the row sees)
             const float w0 = m0 == -INFINITY ? 0.f : ex2(m0 - mm), w1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
-            const float sum = w0 * sh->fin_l[0][tid] + w1 * sh->fin_l[1][tid];
+            const float sum = w0 * sh->fin_l[0][tid] + (C::SETS > 1 ? w1 * sh->fin_l[1][tid] : 0.f);
             const float f = m_o == -INFINITY ? sum : ex2(m_o - mm) / sum;  // (sum: zero, or NaN)
             constexpr int RS = TD * 4 + 16;
-            const int c0 = set * (TD / 2), cols = p.dim - c0 < TD / 2 ? p.dim - c0 : TD / 2;
+            const int c0 = half * (TD / 2), cols = p.dim - c0 < TD / 2 ? p.dim - c0 : TD / 2;
             uint8_t *srow = smem + tid * RS + c0 * 4;
 #pragma unroll
             for (int c = 0; c < TD / 4; c += 2)
                 *reinterpret_cast<float4 *>(srow + c * 8) = make_float4(o[c].x * f, o[c].y * f, o[c + 1].x * f, o[c + 1].y * f);
             tcf16::send_row<false>(p.out + part * p.out_part + rh * p.dim + c0, srow, cols, mine);
-            if (set == 0 && p.lse && mine) p.lse[part * p.lse_part + rh] = (mm + log2f(sum) - 7.0f) * kLn2;
+            if (half == 0 && p.lse && mine) p.lse[part * p.lse_part + rh] = (mm + log2f(sum) - 7.0f) * kLn2;
+        };
+        const auto sync_rows = [&]() { asm volatile("bar.sync 2, %0;" ::"n"(PLANES ? 128 * C::SETS + 256 : 256) : "memory"); };
+        if (PLANES && warp < 4 * C::SETS) {
+            (C::kSoftRegs > C::kLaunchRegs ? more_registers<C::kSoftRegs> : fewer_registers<C::kSoftRegs>)();
+            const int set = warp >> 2;
+            for (int j = set; ok && j < n; j += C::SETS) ok = make_p(j);
+            publish_sums(set);
+            sync_rows();
+        } else {
+            more_registers<C::kRowRegs>();
+            const int half = (PLANES ? warp - 4 * C::SETS : warp) >> 2;
+            place_q(half);
+            float2 o[TD / 4];
+#pragma unroll
+            for (int c = 0; c < TD / 4; ++c) o[c] = make_float2(0.f, 0.f);
+            float m_o = -INFINITY;
+            int added = 0;
+            if (!PLANES)
+                for (int j = half; ok && j < n; j += 2) {
+                    ok = make_p(j);
+                    for (; ok && added < j; ++added) ok = add_tile(added, half, o, m_o);
+                }
+            for (; ok && added < n; ++added) ok = add_tile(added, half, o, m_o);
+            if (!PLANES) publish_sums(half);
+            sync_rows();
+            if (ok) send_rows(half, o, m_o);
         }
     }
     tc_fence_before();
