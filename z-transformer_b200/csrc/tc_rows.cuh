@@ -67,8 +67,8 @@ struct Cfg {
     static constexpr int kThreads = (PLANES ? 128 * SETS : GROUPS * kConvert) + 256 + 128;
     // registers a thread, of what the launch gives: 640 threads 96 each, 512 threads 128
     static constexpr int kLaunchRegs = kWide ? 128 : 96;
-    static constexpr int kRowRegs = kWide ? (PLANES ? 184 : 200) : (PLANES ? 120 : 160);
-    static constexpr int kSoftRegs = 104, kConvertRegs = kWide ? 72 : 64, kIssueRegs = kWide ? 40 : 32;
+    static constexpr int kRowRegs = kWide ? (PLANES ? 184 : 200) : (PLANES ? 144 : 160);
+    static constexpr int kSoftRegs = kWide ? 104 : 80, kConvertRegs = kWide ? 72 : 64, kIssueRegs = kWide ? 40 : 32;
     static constexpr int kShare = 256 * kRowRegs + (PLANES ? 128 * SETS * kSoftRegs : GROUPS * kConvert * kConvertRegs) + 128 * kIssueRegs;
     static_assert(kShare <= kThreads * kLaunchRegs, "the groups share what the launch has");
     static constexpr int cQh = 0, cQl = TD / 2, cO = kWide ? 128 : TD, cS = kWide ? 384 : (OB + 1) * TD;
@@ -83,7 +83,7 @@ struct Shared {
     uint32_t tmem_base;
     volatile int abort;
     int found;
-    float mk[16], mv[16];       // the scales of tiles j & 15
+    float mk[16], mv[16];       // one over the scales of tiles j & 15 (powers of two)
     uint32_t odd[16][2];        // which values' rows of tile j & 15 hold something that is not finite
     uint32_t top[2][2][4];      // [group][unit & 1][warp]: the largest hi piece; or max |x|
     uint32_t seed[2][4];
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             const bool care = top < 0x3000u || top >= 0x7c00u || (is_k && hole);
             if (care) m = with_care(dst, is_k, j, u);
             if (ct == 0) {
-                (is_k ? sh->mk : sh->mv)[j & 15] = m;
+                (is_k ? sh->mk : sh->mv)[j & 15] = 1.f / m;
                 if (ok) mbar_arrive(is_k ? &sh->k_full[s] : &sh->v_full[s]);
             }
             // the next tile's: with which this one's largest would have been in [2^12, 2^13)
@@ -568,25 +568,24 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             tc_fence_after();
             if (cs0 == 0.f) cs0 = fmaxf(p.scale_log2 / block_mult(__float_as_uint(fmaxf(sh->q_top[0][tid], sh->q_top[1][tid]))), 1.17549435e-38f);
             const int s0 = key0(j);
-            const float cs = fmaxf(cs0 / sh->mk[j & 15], 1.17549435e-38f);
+            const float cs = fmaxf(cs0 * sh->mk[j & 15], 1.17549435e-38f);
             const uint32_t cS = tmem + lane_base + C::cS + (j % SB) * BN;
             const Seen &v = p.seen;
             const bool masked = s0 + BN - 1 > warp_first || (v.window > 0 && s0 <= warp_last - v.window && s0 + BN > v.sinks);
-            // Where a thread also holds its half of O, 32 columns of S at a time: they come out of TMEM a second time for their
-            // exponentials.
-            constexpr bool kTwice = !PLANES && BN > 32;
-            constexpr int R = BN > 32 && !kTwice ? 2 : 1;
-            uint32_t r[R][32];
-            const auto scores = [&](uint32_t(&x)[32], int c) {
-                tmem_ld32(cS + c, x);
+            // 32 columns of S at a time: of a tile of 64 they come out of TMEM a second time for their exponentials, which costs less
+            // than the registers to hold them (that sum the rows, or hold half of O beside them)
+            constexpr bool kTwice = BN > 32;
+            uint32_t r[32];
+            const auto scores = [&](int c) {
+                tmem_ld32(cS + c, r);
                 tmem_wait_ld();
-                if (masked) mask_scores(x, v, s0 + c, pos);
+                if (masked) mask_scores(r, v, s0 + c, pos);
             };
             float mt = -INFINITY;
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
-                scores(r[c / 32 % R], c);
-                mt = row_max32(r[c / 32 % R], mt);
+                scores(c);
+                mt = row_max32(r, mt);
             }
             mt *= cs;  // cs > 0
             if ((mt > m_ref + tcf16::kRescaleThreshold || m_ref == -INFINITY) && mt != -INFINITY) {
@@ -598,8 +597,8 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
                 uint32_t ph[16], pl[16];
-                if (kTwice) scores(r[0], c);
-                l += row_exp32(r[c / 32 % R], cs, off, ph, pl);
+                if (kTwice) scores(c);
+                l += row_exp32(r, cs, off, ph, pl);
                 tmem_st16(cS + c, ph);
                 tmem_st16(cS + c + 16, pl);
             }
@@ -616,27 +615,34 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 return false;
             }
             tc_fence_after();
-            const float mj = sh->m_ref[j & 7][tid];
-            if (__any_sync(0xffffffffu, mj > m_o)) {
-                const float f = mj > m_o ? ex2(m_o - mj) : 1.f;
-                m_o = fmaxf(m_o, mj);
-#pragma unroll
-                for (int c = 0; c < TD / 4; ++c) o[c] = mul2(o[c], make_float2(f, f));
-            }
-            // (no key of the tile or before it is seen: P is zero)
-            const float w = mj == -INFINITY ? 0.f : ex2(mj - m_o) / sh->mv[j & 15];
+            // The next product may go over O once it is in registers: its columns are asked for first, the factors formed meanwhile.
+            constexpr int COLS = TD / 2 < 64 || !PLANES || C::kWide ? 32 : 64;
             const uint32_t from = tmem + lane_base + C::cO + ob * TD + half * (TD / 2);
+            uint32_t r[COLS / 32][32];
+            float w = 0.f;
 #pragma unroll
-            for (int c = 0; c < TD / 2; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(from + c, r);
+            for (int c = 0; c < TD / 2; c += COLS) {
+#pragma unroll
+                for (int i = 0; i < COLS; i += 32) tmem_ld32(from + c + i, r[i / 32]);
+                if (c == 0) {
+                    const float mj = sh->m_ref[j & 7][tid];
+                    if (__any_sync(0xffffffffu, mj > m_o)) {
+                        const float f = mj > m_o ? ex2(m_o - mj) : 1.f;
+                        m_o = fmaxf(m_o, mj);
+#pragma unroll
+                        for (int i = 0; i < TD / 4; ++i) o[i] = mul2(o[i], make_float2(f, f));
+                    }
+                    // (no key of the tile or before it is seen: P is zero)
+                    w = mj == -INFINITY ? 0.f : ex2(mj - m_o) * sh->mv[j & 15];
+                }
                 tmem_wait_ld();
-                if (c + 32 >= TD / 2) {
+                if (c + COLS >= TD / 2) {
                     tc_fence_before();
                     mbar_arrive_warp_relaxed(&sh->o_free[ob]);
                 }
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) o[(c + i) >> 1] = fma2(floats2(r[i], r[i + 1]), make_float2(w, w), o[(c + i) >> 1]);
+                for (int i = 0; i < COLS; i += 2)
+                    o[(c + i) >> 1] = fma2(floats2(r[i / 32][i % 32], r[i / 32][i % 32 + 1]), make_float2(w, w), o[(c + i) >> 1]);
             }
             const uint32_t odd[2] = {sh->odd[j & 15][0], sh->odd[j & 15][1]};
             if (odd[0] | odd[1]) {  // values that are not finite, added to the rows that see them
@@ -799,7 +805,7 @@ __global__ void __launch_bounds__(256) rows_planes_kernel(const Params p) {
     float m[2];
     for (int i = 0; i < 2; ++i) m[i] = block_mult(max(max(tops[i][0], tops[i][1]), max(tops[i][2], tops[i][3]))) * 0.25f;
     const long long at = ((long long)b * p.n_kv_heads + g) * p.tiles + tile;
-    if (threadIdx.x == 0) p.heads[at] = make_uint4(__float_as_uint(m[0]), __float_as_uint(m[1]), odd[0], odd[1]);
+    if (threadIdx.x == 0) p.heads[at] = make_uint4(__float_as_uint(1.f / m[0]), __float_as_uint(1.f / m[1]), odd[0], odd[1]);
     uint8_t *dst = p.planes + at * (4 * KP) + (is_k ? 0 : 2 * KP);
     const float2 mm = is_k ? make_float2(m[0], m[0]) : make_float2(m[1], m[1]);
 #pragma unroll
