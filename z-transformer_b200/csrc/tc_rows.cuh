@@ -74,7 +74,14 @@ struct Cfg {
     static constexpr int cQh = 0, cQl = TD / 2, cO = kWide ? 128 : TD, cS = kWide ? 384 : (OB + 1) * TD;
     static_assert(cO + OB * TD <= cS && cS + SB * BN <= 512, "tensor memory");
     static constexpr int kData = KS * 2 * KP + VS * 2 * KP + GROUPS * NP * PART + QL;
-    static_assert(128 * (TD * 4 + 16) <= kData, "the finished rows are staged where the tiles were");
+    // The query rows go through shared memory on their way in (kStaged), the finished ones on their way out, where the tiles are, 16
+    // bytes apart from a multiple of 128: eight threads' chunks lie in different banks.
+    static constexpr int RS = TD * 4 + 16;
+    static constexpr bool kStaged = PLANES || !kWide;
+    static constexpr int kQ = (PLANES ? kData : (KS + VS) * 2 * KP) - 128 * RS;
+    static constexpr int kEarly = kQ / (2 * KP) < KS ? kQ / (2 * KP) : KS;  // K slots in front of the query rows
+    static_assert(!kStaged || kEarly >= 1, "the query rows are staged where tiles come later");
+    static_assert(128 * RS <= kData, "the finished rows are staged where the tiles were");
     static_assert(NP <= 2 * PARTS, "rows are looked up two tiles ahead");
 };
 
@@ -111,6 +118,7 @@ struct Params {
     uint8_t *planes;
     uint4 *heads;
     int tiles;
+    int ahead;  // the query rows of the block this many places on in launch order are fetched into L2 (whole sequences)
 };
 
 __device__ __forceinline__ bool rwait(uint64_t *bar, uint32_t parity, Shared *sh) {
@@ -329,6 +337,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 };
                 for (int j = 0; ok && j < n; ++j) {
                     const int s = j % KS;
+                    if (j == C::kEarly && !rwait(&sh->a_ready, 0, sh)) { rgive_up(sh, 107), ok = false; break; }  // (the query rows lie there until then)
                     const uint4 now = head;
                     if (j + 1 < n) head = p.heads[tile_at(j + 1)];
                     if (j >= KS && !rwait(&sh->k_free[s], (uint32_t)((j / KS - 1) & 1), sh)) { rgive_up(sh, 107), ok = false; break; }
@@ -337,9 +346,10 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                     mbar_arrive_expect_tx(&sh->k_full[s], 2 * KP);
                     bulk_load(sK + s * 2 * KP, p.planes + tile_at(j) * (4 * KP), 2 * KP, &sh->k_full[s]);
                     ++n_k;
-                    if (j > 0) copy_v(j - 1);
+                    while (ok && j >= C::kEarly && n_v < j) copy_v(n_v);
                 }
-                if (ok) copy_v(n - 1);
+                if (ok && n <= C::kEarly && !rwait(&sh->a_ready, 0, sh)) rgive_up(sh, 107), ok = false;
+                while (ok && n_v < n) copy_v(n_v);
                 if (sh->abort) {
                     // let the copies in flight land before the CTA's shared memory goes away
                     for (int j = (n_k > KS ? n_k - KS : 0); j < n_k; ++j) mbar_wait(&sh->k_full[j % KS], (uint32_t)((j / KS) & 1));
@@ -347,6 +357,20 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 }
             }
             __syncwarp();
+        } else if (PLANES && !PAGED && p.ahead > 0) {
+            // The query rows of the block that will start when one of the running ones ends, into L2: from DRAM, under load, they
+            // would be waited for.
+            const long long next = blockIdx.x + (long long)gridDim.x * blockIdx.y + p.ahead;
+            const int ny = (int)(next / gridDim.x), nslot = (int)(gridDim.x - 1 - next % gridDim.x);
+            if (ny < (int)gridDim.y) {
+                const int per = (int)(((long long)p.T * group + 127) / 128), nb = nslot / per, nf = (nslot - nb * per) * 128;
+                const int bytes = p.dim * 4;
+                for (int r = lane; r < 128 && nf + r < (long long)p.T * group; r += 32) {
+                    const int f = nf + r, i = f / group;
+                    const char *row = reinterpret_cast<const char *>(p.q + (((long long)nb * p.T + i) * p.n_heads + ny * group + (f - i * group)) * p.dim);
+                    for (int c = 0; c < bytes; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
+                }
+            }
         }
     } else if (!PLANES && warp >= 8) {
         // ------------------------------------------------------------------ keys and values: copied, scaled, split.  A group's
@@ -461,6 +485,10 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             bool is_k;
             const int j = unit(u, is_k), s = is_k ? j % KS : j % VS, S = is_k ? KS : VS;
             uint8_t *dst = (is_k ? sK : sV) + s * 2 * KP;
+            if (C::kStaged && ok && j == (is_k ? C::kEarly : 0) && !__all_sync(0xffffffffu, rwait(&sh->a_ready, 0, sh))) {
+                rgive_up(sh, 104);  // (the query rows lie there until then)
+                ok = false;
+            }
             if (ok && j >= S && !__all_sync(0xffffffffu, rwait(is_k ? &sh->k_free[s] : &sh->v_free[s], (uint32_t)((j / S - 1) & 1), sh))) {
                 rgive_up(sh, 104);
                 ok = false;  // (on to the barriers that the other warps wait at)
@@ -534,12 +562,33 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
         const auto place_q = [&](int half) {
             float4 x[TD / 8];
             float top = 0.f;
+            if (C::kStaged) {
+                // a warp fetches its 32 half rows whole lines at a time (each thread its own half row took 10000 clocks)
+                constexpr int N = TD / 8;  // chunks of a half row
+                uint8_t *staged = smem + C::kQ + half * (TD * 2);
 #pragma unroll
-            for (int c = 0; c < TD / 8; ++c) {
-                const int col = half * (TD / 2) + c * 4;
-                x[c] = mine && col < p.dim ? *reinterpret_cast<const float4 *>(p.q + rh * p.dim + col) : make_float4(0.f, 0.f, 0.f, 0.f);
-                top = fmaxf(top, max_abs4(x[c]));
+                for (int i = 0; i < N; ++i) {
+                    // (the row's place is known to its own thread; a division each cost 4000 clocks)
+                    const int r = (i * 32 + lane) / N, col = half * (TD / 2) + (i * 32 + lane) % N * 4;
+                    const long long row = __shfl_sync(0xffffffffu, rh, r);
+                    const bool in = (warp & 3) * 32 + r < n_rows && col < p.dim;
+                    x[i] = in ? *reinterpret_cast<const float4 *>(p.q + row * p.dim + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    *reinterpret_cast<float4 *>(staged + ((warp & 3) * 32 + (i * 32 + lane) / N) * C::RS + (i * 32 + lane) % N * 16) = x[i];
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < TD / 8; ++c) x[c] = *reinterpret_cast<const float4 *>(staged + tid * C::RS + c * 16);
+            } else {
+#pragma unroll
+                for (int c = 0; c < TD / 8; ++c) {
+                    const int col = half * (TD / 2) + c * 4;
+                    x[c] = mine && col < p.dim ? *reinterpret_cast<const float4 *>(p.q + rh * p.dim + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
             }
+#pragma unroll
+            for (int c = 0; c < TD / 8; ++c) top = fmaxf(top, max_abs4(x[c]));
             sh->q_top[half][tid] = top;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const float m = block_mult(__float_as_uint(fmaxf(top, sh->q_top[half ^ 1][tid])));
@@ -552,7 +601,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 else tmem_st16(tmem + lane_base + C::cQl + half * (TD / 4) + cb * 16, ql);
             }
             tmem_wait_st();
-            if (C::kWide) fence_async_smem();
+            if (C::kWide || C::kStaged) fence_async_smem();  // (Q lo, and before the bulk copies that land where the rows were)
             tc_fence_before();
             mbar_arrive_warp(&sh->a_ready);
         };
@@ -673,9 +722,8 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             const float w0 = m0 == -INFINITY ? 0.f : ex2(m0 - mm), w1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
             const float sum = w0 * sh->fin_l[0][tid] + (C::SETS > 1 ? w1 * sh->fin_l[1][tid] : 0.f);
             const float f = m_o == -INFINITY ? sum : ex2(m_o - mm) / sum;  // (sum: zero, or NaN)
-            constexpr int RS = TD * 4 + 16;
             const int c0 = half * (TD / 2), cols = p.dim - c0 < TD / 2 ? p.dim - c0 : TD / 2;
-            uint8_t *srow = smem + tid * RS + c0 * 4;
+            uint8_t *srow = smem + tid * C::RS + c0 * 4;
 #pragma unroll
             for (int c = 0; c < TD / 4; c += 2)
                 *reinterpret_cast<float4 *>(srow + c * 8) = make_float4(o[c].x * f, o[c].y * f, o[c + 1].x * f, o[c + 1].y * f);
@@ -828,6 +876,22 @@ inline int tile_keys(int dim) { return tc_tile_dim(dim) > 128 ? 32 : 64; }
 inline long long key_tiles(int keys, int dim) { return ((long long)keys + tile_keys(dim) - 1) / tile_keys(dim); }
 inline size_t planes_bytes(int batch, int keys, int n_kv_heads, int dim) {
     return (size_t)batch * n_kv_heads * (size_t)key_tiles(keys, dim) * ((size_t)4 * tile_keys(dim) * tc_tile_dim(dim) * 2 + sizeof(uint4)) + 512;
+}
+// Whether a launch of its own converts the key tiles: where that many row tiles visit each of them.
+inline bool converts_beforehand(long long visits) { return visits >= 4; }
+// The same for new rows over pages, as far as the host knows them -- the sequences have rows / batch each on average --, with the
+// bytes that it takes (0: none), and their bound over smaller calls.  Beyond kPlanesMost the rows convert for themselves.
+constexpr size_t kPlanesMost = (size_t)2 << 30;
+inline size_t paged_planes_bytes(int batch, int rows, int keys, int n_heads, int n_kv_heads, int dim) {
+    const size_t bytes = planes_bytes(batch, keys, n_kv_heads, dim);
+    return converts_beforehand((long long)rows * (n_heads / n_kv_heads) / 128 / batch) && bytes <= kPlanesMost ? bytes : 0;
+}
+inline size_t paged_planes_bound(int batch, int rows, int keys, int n_heads, int n_kv_heads, int dim) {
+    const int group = n_heads / n_kv_heads;
+    const long long most = (long long)rows * group / 128 / 4;  // sequences of a call that converts beforehand, at most
+    if (most < 1) return 0;
+    const size_t bytes = planes_bytes(batch < most ? batch : (int)most, keys, n_kv_heads, dim);
+    return bytes < kPlanesMost ? bytes : kPlanesMost;
 }
 inline void place_planes(Params &p, void *scratch, int keys) {
     p.tiles = (int)key_tiles(keys, p.dim);

@@ -1178,9 +1178,11 @@ int zt_attn_forward_window_batched(const float *q, const float *k, const float *
         p.batch = batch, p.T = T, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.dim = dim, p.parts = 1;
         p.seen = Seen{window, sinks};
         p.scale_log2 = kLog2e / sqrtf((float)dim);
-        const bool planes = getenv("ZT_PLANES") ? atoi(getenv("ZT_PLANES")) : 0;
-        const StreamScratch scratch(planes ? tcr::planes_bytes(batch, T, n_kv_heads, dim) : 0, (cudaStream_t)stream);
+        // (a key tile is visited by the row tiles of the tokens that see one of its keys)
+        const long long visits = ((long long)(window > 0 ? window : T) + 64) * (n_heads / n_kv_heads) / 128;
+        const StreamScratch scratch(tcr::converts_beforehand(visits) ? tcr::planes_bytes(batch, T, n_kv_heads, dim) : 0, (cudaStream_t)stream);
         if (scratch.get()) tcr::place_planes(p, scratch.get(), T);
+        p.ahead = split_sm_count();
         return tcr::launch(p, (long long)batch * (((long long)T * (n_heads / n_kv_heads) + 127) / 128), (cudaStream_t)stream);
     }
     SimtFwdParams p{};
@@ -1235,7 +1237,8 @@ int zt_kv_append_paged(float *k_pages, float *v_pages, const int *table, int *n_
 size_t zt_attn_paged_workspace_bytes(int batch, int rows, int max_keys, int n_heads, int n_kv_heads, int dim) {
     if (batch < 1 || rows < 0 || max_keys < 1 || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || !zt_attn_dim_ok(dim) || dim % 4 != 0)
         return 0;
-    return most(decode_bytes_bound(batch, max_keys, n_heads, n_kv_heads, dim), kDecodeHeaderBytes + tcr::row_parts_bound(rows, n_heads, dim) * sizeof(float));
+    const size_t parts = tcr::row_parts_bound(rows, n_heads, dim) * sizeof(float), planes = tcr::paged_planes_bound(batch, rows, max_keys, n_heads, n_kv_heads, dim);
+    return most(decode_bytes_bound(batch, max_keys, n_heads, n_kv_heads, dim), kDecodeHeaderBytes + most(parts, planes));
 }
 
 int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, const int *n_keys,
@@ -1279,6 +1282,8 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     const long long keys = window > 0 ? (long long)window + sinks + rows : capacity;
     p.parts = tcr::row_parts(batch, rows, (int)(keys < capacity ? keys : capacity), n_heads, n_kv_heads);
     const long long slots = tcr::row_slots(batch, rows, n_heads / n_kv_heads);
+    const size_t planes = tcr::paged_planes_bytes(batch, rows, capacity, n_heads, n_kv_heads, dim);
+    if (planes > 0) p.parts = 1, tcr::place_planes(p, static_cast<char *>(workspace) + kDecodeHeaderBytes, capacity);
     if (p.parts == 1) return tcr::launch(p, slots, (cudaStream_t)stream);
     p.lse_part = (long long)rows * n_heads, p.out_part = p.lse_part * dim;
     p.out = reinterpret_cast<float *>(static_cast<char *>(workspace) + kDecodeHeaderBytes), p.lse = p.out + p.parts * p.out_part;
