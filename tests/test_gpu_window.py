@@ -63,6 +63,8 @@ SHAPES = [
     # other widths and groups
     (1, 260, 4, 2, 128, 100, 4), (2, 200, 6, 2, 96, 77, 3), (1, 190, 16, 4, 80, 50, 17), (1, 300, 5, 1, 100, 129, 5), (1, 140, 12, 4, 112, 31, 2),
     (1, 260, 4, 2, 256, 64, 4), (1, 200, 2, 2, 192, 90, 0), (2, 150, 4, 1, 160, 40, 33), (1, 330, 4, 2, 132, 131, 1), (1, 70, 32, 8, 128, 16, 2),
+    # walks of many tiles: sinks' keys in several blocks, contractions in several pieces
+    (1, 3000, 2, 1, 64, 100, 4), (2, 1400, 2, 1, 128, 60, 129), (1, 1500, 2, 1, 192, 300, 5), (1, 2300, 2, 1, 256, 100, 140),
     # widths that no tensor-core tile takes
     (1, 70, 4, 2, 34, 20, 3), (1, 50, 2, 1, 62, 33, 0), (1, 100, 4, 2, 36, 64, 1),
 ]

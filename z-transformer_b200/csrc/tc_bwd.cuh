@@ -73,6 +73,7 @@ struct BwdParams {
     BwdParts parts;     // how the walk of a key tile is split; more than one part: dk, dv are the first part's,
     long long dkv_part; // and this many elements lie between two parts'
     float p_scale;  // P is multiplied by this power of two before its 16-bit split
+    BwdWindow win;  // (the fused kernels) window 0: none
 };
 
 // The scale of dS.  dS = P (dP - delta) leaves the row threads as a pair of f16 pieces, so it must sit inside the

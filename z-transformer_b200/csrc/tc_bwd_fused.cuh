@@ -60,7 +60,8 @@ constexpr size_t kFusedSmem = 3 * (size_t)(128 * 128 * 2) + 2 * (size_t)(128 * 1
 constexpr int kFusedThreads = (kKvRowWarps + 3) * 32;
 // PARTS: the walk is split, or the blocks go tile by tile (tc_split.cuh).  A variant of its own: large launches are 1-2 % slower
 // with the code in it.
-template <bool PARTS, bool PAD>
+// WIN: a window (BwdWindow); the blocks along y are window_block's.
+template <bool PARTS, bool PAD, bool WIN>
 __global__ void __launch_bounds__(kFusedThreads, 1)
     attn_bwd_fused_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                       const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
@@ -79,14 +80,15 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
 
     const int warp = threadIdx.x >> 5;
     // (the slowest index is the sequence, or the tile: see tile_by_tile)
-    const int g = blockIdx.x, kt = PARTS && p.by_tile ? (int)blockIdx.z : (int)blockIdx.y, bp = PARTS && p.by_tile ? (int)blockIdx.y : (int)blockIdx.z;
+    const WindowBlock mine_of = WIN ? window_block(p.win, p.T, (int)blockIdx.y, BQ) : WindowBlock{};
+    const int g = blockIdx.x, kt = WIN ? mine_of.kt : PARTS && p.by_tile ? (int)blockIdx.z : (int)blockIdx.y, bp = PARTS && p.by_tile ? (int)blockIdx.y : (int)blockIdx.z;
     const int b = PARTS ? bp / p.parts.n() : bp, part = PARTS ? bp - b * p.parts.n() : 0;
     const int group = p.n_heads / p.n_kv_heads;
     const int s0 = kt * 128;
     // this CTA's part of the walk: heads [head0, head0 + n_heads_mine) and query tiles [qi0, n_q)
     const int n_heads_mine = PARTS ? group / p.parts.heads : group;
     const int head0 = PARTS ? g * group + part / p.parts.ranges * n_heads_mine : g * group;
-    int n_q = (p.T + BQ - 1) / BQ, qi0 = s0 / BQ;
+    int n_q = WIN ? mine_of.n_q : (p.T + BQ - 1) / BQ, qi0 = WIN ? mine_of.qi0 : s0 / BQ;
     if (PARTS && p.parts.ranges > 1) {
         const int per = (n_q - qi0 + p.parts.ranges - 1) / p.parts.ranges;
         qi0 += part % p.parts.ranges * per;
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
                         float4 a;
                         a.x = __uint_as_float(r[4 * i]) * f, a.y = __uint_as_float(r[4 * i + 1]) * f;
                         a.z = __uint_as_float(r[4 * i + 2]) * f, a.w = __uint_as_float(r[4 * i + 3]) * f;
-                        if (n_flush == 0) *reinterpret_cast<float4 *>(dst + i * wo + c) = a;
+                        if (n_flush == 0 && !(WIN && mine_of.adds)) *reinterpret_cast<float4 *>(dst + i * wo + c) = a;
                         else red_add_v4(dst + i * wo + c, a);
                     }
                 }
@@ -514,7 +516,8 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
                 tmem_wait_ld();
                 uint32_t ph[8], pl[8];
                 const int q_first = walk.qi * BQ;
-                const bool plain = (q_first >= s0 + 127 || ZT_DEFECT(11)) && q_first + BQ <= p.T && s0 + 128 <= p.T;
+                const bool plain = (q_first >= s0 + 127 || ZT_DEFECT(11)) && q_first + BQ <= p.T && s0 + 128 <= p.T &&
+                                   (!WIN || s0 > q_first + BQ - 1 - p.win.window || s0 + 128 <= p.win.sinks);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float2 x = fma2(floats2(rs[2 * i], rs[2 * i + 1]), csc[i], nlse[i]);
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
                 if (!plain) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const auto vis = [&](int t) { return (key <= t || ZT_DEFECT(11)) && t < p.T && key < p.T; };
+                        const auto vis = [&](int t) { return (key <= t || ZT_DEFECT(11)) && t < p.T && key < p.T && (!WIN || window_sees(p.win, key, t)); };
                         pr[i].x = vis(t0 + 2 * i) ? pr[i].x : 0.f, pr[i].y = vis(t0 + 2 * i + 1) ? pr[i].y : 0.f;
                     }
                 }
@@ -622,9 +625,11 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
 
 inline int launch_bwd_fused(const CUtensorMap &k128, const CUtensorMap &v128, const CUtensorMap &qs64, const CUtensorMap &g64,
                             const BwdParams &p, cudaStream_t stream) {
-    const auto kernel = with_flags([](auto parts, auto pad) { return attn_bwd_fused_tc<parts.value, pad.value>; }, p.parts.n() > 1 || p.by_tile, head_steps(p.dim_out) < 8);
+    const bool win = p.win.window > 0;
+    const auto kernel = win ? (head_steps(p.dim_out) < 8 ? attn_bwd_fused_tc<false, true, true> : attn_bwd_fused_tc<false, false, true>)
+                            : with_flags([](auto parts, auto pad) { return attn_bwd_fused_tc<parts.value, pad.value, false>; }, p.parts.n() > 1 || p.by_tile, head_steps(p.dim_out) < 8);
     if (optin_smem((const void *)kernel, kFusedSmem)) return 1;
-    const unsigned tiles = (unsigned)((p.T + 127) / 128), seqs = (unsigned)(p.batch * p.parts.n()), kv = (unsigned)p.n_kv_heads;
+    const unsigned tiles = (unsigned)(win ? window_blocks(p.win, p.T, 64) : (p.T + 127) / 128), seqs = (unsigned)(p.batch * p.parts.n()), kv = (unsigned)p.n_kv_heads;
     const dim3 grid = p.by_tile ? dim3(kv, seqs, tiles) : dim3(kv, tiles, seqs);
     return launch_after("attn_bwd_fused_tc", kernel, grid, dim3(kFusedThreads), kFusedSmem, stream, 1, k128, v128, qs64, g64, p);
 }
@@ -639,6 +644,21 @@ inline bool tc_bwd_takes_fused(int dim, bool two_kernels, const PeerList *dq_pee
     return (td == 64 || td == 128) && !two_kernels && !(dq_peers && dq_peers->n > 0);
 }
 
+// The rows of dk and dv that several blocks add to (of key tiles with sinks whose walks go on beyond their window) begin as zeros.
+inline int zero_added_rows(const BwdWindow &w, float *dk, float *dv, int batch, int T, int width, int rows, cudaStream_t stream) {
+    long long n = 0;
+    for (int kt = 0; kt * 128 < T && kt * 128 < w.sinks; ++kt)
+        if (near_tiles(w, T, kt, rows) < (T + rows - 1) / rows) n = (kt + 1) * 128;
+    if (n == 0) return 0;
+    const size_t pitch = (size_t)T * width * sizeof(float), bytes = (size_t)(n < T ? n : T) * width * sizeof(float);
+    for (float *x : {dk, dv})
+        if (cudaMemset2DAsync(x, pitch, 0, bytes, batch, stream) != cudaSuccess) {
+            cudaGetLastError();
+            return refuse("could not clear the gradients of the sinks");
+        }
+    return 0;
+}
+
 // delta (= sum_j dout out, per row) is formed here; dq, dk, dv are assigned.  `out` may alias dq: it has been read when
 // dq is first written.
 // rope_t: only with the two-kernel form (the fused kernel's dq takes its rotation in a pass of its own, by the caller).
@@ -646,11 +666,12 @@ inline int launch_bwd_tc(const float *q, const float *k, const float *v, const f
                          const float *lse, float *delta, float *dq, float *dk, float *dv, void *workspace, size_t workspace_bytes, int batch, int T,
                          int n_heads, int n_kv_heads, int dim, cudaStream_t stream, const float2 *rope = nullptr,
                          const float2 *rope_t = nullptr, bool qkv_planes_kept = false, const PeerList *dq_peers = nullptr,
-                         bool two_kernels = false) {
+                         bool two_kernels = false, int window = 0, int sinks = 0) {
     using namespace tcb;
     const int td = tc_tile_dim(dim), pd = tc::plane_dim(dim);  // the kernels' D; the planes' head width
     const bool fused = tc_bwd_takes_fused(dim, two_kernels, dq_peers);
     if (fused && rope_t) return refuse("internal: the fused backward does not rotate dq.");
+    if (!fused && window > 0) return refuse("internal: only the fused backward takes a window.");
     const BwdWorkspace w = bwd_workspace(workspace, batch, T, n_heads, n_kv_heads, pd);
     const int group = n_heads / n_kv_heads;
     const int blocks = td / 64;
@@ -674,8 +695,10 @@ inline int launch_bwd_tc(const float *q, const float *k, const float *v, const f
         pass_add(pa, v, batch, T, n_kv_heads, 1, w.part[2], w.amax_v, w.vnmax, w.v_planes);
     }
     if (fused) pass_fill(pa, dq, (long long)batch * T * n_heads * dim);
-    if (launch_pass_backward(pa, w, fused, !fused, qkv_planes_kept, stream)) return 1;
     const int rows = fused && td == 64 ? tcf::fused64_rows(T) : 64;  // of a query tile
+    const BwdWindow win{window, sinks, (window + 127) / rows + 2};
+    if (window > 0 && zero_added_rows(win, dk, dv, batch, T, n_kv_heads * dim, rows, stream)) return 1;
+    if (launch_pass_backward(pa, w, fused, !fused, qkv_planes_kept, stream)) return 1;
     BwdMaps m;
     bool maps = make_head_map(&m.k128, w.k_planes, 2 * batch, T, n_kv_heads, dim, blocks, 128) &&
                 make_head_map(&m.v128, w.v_planes, 2 * batch, T, n_kv_heads, dim, blocks, 128) &&
@@ -702,6 +725,11 @@ inline int launch_bwd_tc(const float *q, const float *k, const float *v, const f
     // dS is scaled inside the kernels (see "The scale of dS" in tc_bwd.cuh and the head of this file).
     p.p_scale = ldexpf(1.0f, 10);
     g_last_path = "tcgen05";
+    p.win = win;
+    if (fused && window > 0) {
+        p.parts = BwdParts{1, 1};
+        return td == 64 ? tcf::launch_bwd_fused64(m.k128, m.v128, m.q64, m.g64, p, stream) : tcf::launch_bwd_fused(m.k128, m.v128, m.q64, m.g64, p, stream);
+    }
     if (fused) {
         p.parts = bwd_parts(batch, T, n_heads, n_kv_heads, dim);
         if (p.parts.n() > 1 && w.base_bytes + bwd_parts_floats(batch, T, n_heads, n_kv_heads, pd) * sizeof(float) > workspace_bytes) p.parts = BwdParts{1, 1};

@@ -65,8 +65,8 @@ constexpr int kFused64Threads = (kKvRowWarps + 8) * 32, kReadWarps = 4;
 constexpr size_t kFused64Smem = 3 * (size_t)(128 * 64 * 2) + 2 * (size_t)(128 * 128 * 2) + 6 * (size_t)(128 * 64 * 2) +
                                 kReadWarps * 4096 + sizeof(Fused64Shared);
 
-// PARTS, PAD: as in attn_bwd_fused_tc.  ROWS: query rows of a step, 128, or 64 for sequences that have no more.
-template <bool PARTS, bool PAD, int ROWS>
+// PARTS, PAD, WIN: as in attn_bwd_fused_tc.  ROWS: query rows of a step, 128, or 64 for sequences that have no more.
+template <bool PARTS, bool PAD, int ROWS, bool WIN>
 __global__ void __launch_bounds__(kFused64Threads, 1)
     attn_bwd_fused64_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
@@ -86,14 +86,15 @@ __global__ void __launch_bounds__(kFused64Threads, 1)
 
     const int warp = threadIdx.x >> 5;
     // (the slowest index is the sequence, or the tile: see tile_by_tile)
-    const int g = blockIdx.x, kt = PARTS && p.by_tile ? (int)blockIdx.z : (int)blockIdx.y, bp = PARTS && p.by_tile ? (int)blockIdx.y : (int)blockIdx.z;
+    const WindowBlock mine_of = WIN ? window_block(p.win, p.T, (int)blockIdx.y, BQ) : WindowBlock{};
+    const int g = blockIdx.x, kt = WIN ? mine_of.kt : PARTS && p.by_tile ? (int)blockIdx.z : (int)blockIdx.y, bp = PARTS && p.by_tile ? (int)blockIdx.y : (int)blockIdx.z;
     const int b = PARTS ? bp / p.parts.n() : bp, part = PARTS ? bp - b * p.parts.n() : 0;
     const int group = p.n_heads / p.n_kv_heads;
     const int s0 = kt * 128;
     // this CTA's part of the walk: heads [head0, head0 + n_heads_mine) and query tiles [qi0, n_q)
     const int n_heads_mine = PARTS ? group / p.parts.heads : group;
     const int head0 = PARTS ? g * group + part / p.parts.ranges * n_heads_mine : g * group;
-    int n_q = (p.T + BQ - 1) / BQ, qi0 = kt * (128 / BQ);
+    int n_q = WIN ? mine_of.n_q : (p.T + BQ - 1) / BQ, qi0 = WIN ? mine_of.qi0 : kt * (128 / BQ);
     if (PARTS && p.parts.ranges > 1) {
         const int per = (n_q - qi0 + p.parts.ranges - 1) / p.parts.ranges;
         qi0 += part % p.parts.ranges * per;
@@ -445,7 +446,7 @@ __global__ void __launch_bounds__(kFused64Threads, 1)
                     take((is_dv ? cDV : cDK) + c0, is_dv ? 1.0f / (p.p_scale * mdo) : p.scale / (mq * cmin), i == 1 ? &sh->dv_free : i == 3 ? &sh->dk_free : nullptr);
                     if (lane == 0 && s0 + q32 < p.T && c0 < p.dim_out) {
                         const CUtensorMap *map = is_dv ? &dvmap : &dkmap;
-                        if (n_flush == 0) tma_store_4d(map, out, c0, g, s0 + q32, bz);
+                        if (n_flush == 0 && !(WIN && mine_of.adds)) tma_store_4d(map, out, c0, g, s0 + q32, bz);
                         else tma_add_4d(map, out, c0, g, s0 + q32, bz);
                         tma_commit();
                     }
@@ -505,7 +506,8 @@ __global__ void __launch_bounds__(kFused64Threads, 1)
                 const float4 *csc = reinterpret_cast<const float4 *>(sh->csc + set * CW);
                 const float4 *nlse = reinterpret_cast<const float4 *>(sh->nlse + set * CW);
                 const int q_first = walk.qi * BQ, t0 = q_first + set * CW;
-                const bool plain = (q_first >= s0 + 127 || ZT_DEFECT(11)) && q_first + BQ <= p.T && s0 + 128 <= p.T;
+                const bool plain = (q_first >= s0 + 127 || ZT_DEFECT(11)) && q_first + BQ <= p.T && s0 + 128 <= p.T &&
+                                   (!WIN || s0 > q_first + BQ - 1 - p.win.window || s0 + 128 <= p.win.sinks);
 #pragma unroll
                 for (int w = 0; w < CW / 16; ++w) {
                     uint32_t rs[16], ph[8], pl[8];
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(kFused64Threads, 1)
                         float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
                         if (!plain) {
                             const int t = t0 + 16 * w + i;
-                            const auto vis = [&](int at) { return (key <= at || ZT_DEFECT(11)) && at < p.T && key < p.T; };
+                            const auto vis = [&](int at) { return (key <= at || ZT_DEFECT(11)) && at < p.T && key < p.T && (!WIN || window_sees(p.win, key, at)); };
                             p0.x = vis(t) ? p0.x : 0.f, p0.y = vis(t + 1) ? p0.y : 0.f;
                             p1.x = vis(t + 2) ? p1.x : 0.f, p1.y = vis(t + 3) ? p1.y : 0.f;
                         }
@@ -603,10 +605,12 @@ inline int launch_bwd_fused64(const CUtensorMap &k128, const CUtensorMap &v128, 
         !make_row_map(&dkmap, p.dk, kv_batch, p.T, p.n_kv_heads, p.dim_out, 32) ||
         !make_row_map(&dvmap, p.dv, kv_batch, p.T, p.n_kv_heads, p.dim_out, 32))
         return refuse("the TMA tensor maps for the backward's gradients could not be encoded.");
-    const auto kernel = fused64_rows(p.T) == 64 ? attn_bwd_fused64_tc<true, true, 64>
-                                  : with_flags([](auto parts, auto pad) { return attn_bwd_fused64_tc<parts.value, pad.value, 128>; }, p.parts.n() > 1 || p.by_tile, head_steps(p.dim_out) < 4);
+    const bool win = p.win.window > 0, pad = head_steps(p.dim_out) < 4;
+    const auto kernel = fused64_rows(p.T) == 64 ? (win ? attn_bwd_fused64_tc<false, true, 64, true> : attn_bwd_fused64_tc<true, true, 64, false>)
+                        : win ? (pad ? attn_bwd_fused64_tc<false, true, 128, true> : attn_bwd_fused64_tc<false, false, 128, true>)
+                              : with_flags([](auto parts, auto pad) { return attn_bwd_fused64_tc<parts.value, pad.value, 128, false>; }, p.parts.n() > 1 || p.by_tile, pad);
     if (optin_smem((const void *)kernel, kFused64Smem)) return 1;
-    const unsigned tiles = (unsigned)((p.T + 127) / 128), seqs = (unsigned)(p.batch * p.parts.n()), kv = (unsigned)p.n_kv_heads;
+    const unsigned tiles = (unsigned)(win ? window_blocks(p.win, p.T, fused64_rows(p.T)) : (p.T + 127) / 128), seqs = (unsigned)(p.batch * p.parts.n()), kv = (unsigned)p.n_kv_heads;
     const dim3 grid = p.by_tile ? dim3(kv, seqs, tiles) : dim3(kv, tiles, seqs);
     return launch_after("attn_bwd_fused64_tc", kernel, grid, dim3(kFused64Threads), kFused64Smem, stream, 1, k128, v128, qs128, g128, dqmap, dkmap, dvmap, p);
 }

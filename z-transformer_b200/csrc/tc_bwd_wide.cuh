@@ -53,6 +53,23 @@ constexpr int kResThreads = 18 * 32;    // TMA producer, MMA issuer, sixteen row
 constexpr int kTriThreads = 6 * 32;     // TMA producer, MMA issuer, four epilogue warps
 constexpr int kPiece = 1024;            // contraction depth of one unit of wide_products
 
+// Of a window, tiles of 128 on both sides: query tile m visits the key tiles that hold sinks and those from `low` on, numbered
+// through; key tile n is visited by the query tiles from n on up to `last`.
+struct WideTiles {
+    int sink_tiles, skip, n;
+    __host__ __device__ __forceinline__ WideTiles(const BwdWindow &w, int m) {
+        const int low = w.window > 0 && m * 128 >= w.window ? (m * 128 - w.window + 1) / 128 : 0;
+        sink_tiles = w.window > 0 ? (w.sinks + 127) / 128 : 0;
+        sink_tiles = sink_tiles < low ? sink_tiles : low;
+        skip = low - sink_tiles, n = m + 1 - skip;
+    }
+    __host__ __device__ __forceinline__ int at(int i) const { return i < sink_tiles ? i : i + skip; }
+};
+__host__ __device__ inline int wide_last(const BwdWindow &w, int n, int nt) {
+    const int last = w.window > 0 && n * 128 >= w.sinks ? ((n + 1) * 128 + w.window + 126) / 128 - 1 : nt - 1;
+    return last < nt - 1 ? last : nt - 1;
+}
+
 struct WideShared {
     uint64_t full[kStages], freed[kStages], all_done, staged;
     uint32_t tmem_base;
@@ -81,6 +98,7 @@ struct WideParams {
     int unit0, unit_cap;               // the chunk: units (b * n_heads + h) from unit0; planes allocated for unit_cap
     int units, pieces;                 // wide_products: units of the chunk, pieces of kPiece along one head's contraction
     bool in_turn;                      // and the order of its units (products_in_turn)
+    BwdWindow win;                     // window 0: none
     float scale, scale_log2, p_scale;
 };
 
@@ -329,7 +347,7 @@ __device__ __forceinline__ void store_rows_quad(__half *dst, long long ld, const
 template <int D>
 __host__ __device__ constexpr int res_slots() { return D == 256 ? 3 : 4; }
 
-template <int D>
+template <int D, bool WIN>
 __global__ void __launch_bounds__(kResThreads, 1)
     bwd_wide_scores_res(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap gmap, const __grid_constant__ CUtensorMap vmap, const WideParams p) {
@@ -349,7 +367,9 @@ __global__ void __launch_bounds__(kResThreads, 1)
     const int b = ug / p.n_heads, h = ug % p.n_heads;
     const int group = p.n_heads / p.n_kv_heads, g = h / group;
     const int B = p.batch;
-    const int n_tiles = m + 1;
+    const WideTiles tiles(p.win, WIN ? m : 0);
+    const int n_tiles = WIN ? tiles.n : m + 1;
+    const auto key_tile = [&](int i) { return WIN ? tiles.at(i) : i; };
     const int n_blocks = 2 * NB * n_tiles;  // per tile: K's blocks, then V's
 
     if (threadIdx.x == 0) {
@@ -391,8 +411,8 @@ __global__ void __launch_bounds__(kResThreads, 1)
                 const CUtensorMap *mp = is_v ? &vmap : &kmap;
                 uint8_t *base = ring + st * 2 * BT;
                 mbar_arrive_expect_tx(&sh->full[st], 2 * BT);
-                tma_load_4d(base, mp, &sh->full[st], 0, n * 128, g * NB + blk, b);
-                tma_load_4d(base + BT, mp, &sh->full[st], 0, n * 128, g * NB + blk, B + b);
+                tma_load_4d(base, mp, &sh->full[st], 0, key_tile(n) * 128, g * NB + blk, b);
+                tma_load_4d(base + BT, mp, &sh->full[st], 0, key_tile(n) * 128, g * NB + blk, B + b);
                 ++issued;
             };
             for (int j = 0; j < NR && j < n_blocks; ++j) load_block(j);
@@ -497,8 +517,8 @@ __global__ void __launch_bounds__(kResThreads, 1)
         __half *d_hi = p.ds_planes + (long long)u * plane + (long long)(m0 + (row & ~3)) * p.Tp + quarter * 32;
         const long long lo_off = (long long)p.unit_cap * plane;
         for (int n = 0; ok && n < n_tiles; ++n) {
-            const int n0 = n * 128;
-            const bool diag = (n == m) || (m0 + 128 > p.T);
+            const int n0 = key_tile(n) * 128;
+            const bool diag = (n0 == m0) || (m0 + 128 > p.T) || (WIN && n0 <= m0 + 127 - p.win.window && n0 + 128 > p.win.sinks);
             float2 pr[16];
             if (!__all_sync(0xffffffffu, rwait(&sh->s_full, (uint32_t)(n & 1), sh))) { rgive_up(sh, 96); ok = false; break; }
             tc_fence_after();
@@ -519,7 +539,7 @@ __global__ void __launch_bounds__(kResThreads, 1)
                 if (diag) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const auto vis = [&](int key) { return (key <= t || ZT_DEFECT(11)) && key < p.T && t < p.T; };
+                        const auto vis = [&](int key) { return (key <= t || ZT_DEFECT(11)) && key < p.T && t < p.T && (!WIN || window_sees(p.win, key, t)); };
                         pr[i].x = vis(key0 + 2 * i) ? pr[i].x : 0.f, pr[i].y = vis(key0 + 2 * i + 1) ? pr[i].y : 0.f;
                     }
                 }
@@ -610,6 +630,11 @@ __host__ __device__ inline bool products_in_turn(int pieces, int nt, int heads, 
 
 struct TriUnit {
     int which, u, m0, b, h, k_begin, n_steps;  // which: 0 dQ, 1 dK, 2 dV; n_steps <= 0: nothing to do
+    int sinks_end, skip;                       // (a window's dQ) from contraction index sinks_end on, `skip` keys are left out
+    __host__ __device__ __forceinline__ int contraction(int step) const {
+        const int k = k_begin + step * 64;
+        return k < sinks_end ? k : k + skip;
+    }
     __host__ __device__ __forceinline__ TriUnit(const WideParams &p, int i) {
         const int nt = p.Tp / 128;
         int m, piece = 0;
@@ -628,6 +653,19 @@ struct TriUnit {
         m0 = m * 128;
         k_begin = piece * kPiece;
         int k_end = k_begin + kPiece;
+        sinks_end = 0, skip = 0;
+        if (p.win.window > 0) {  // pieces of what is visited
+            if (which == 0) {
+                const WideTiles t(p.win, m);
+                sinks_end = t.sink_tiles * 128, skip = t.skip * 128;
+                k_end = k_end < t.n * 128 ? k_end : t.n * 128;
+            } else {
+                const int n = (wide_last(p.win, m, nt) + 1) * 128 - m0;
+                k_end = (k_end < n ? k_end : n) + m0, k_begin += m0;
+            }
+            n_steps = (k_end - k_begin) / 64;
+            return;
+        }
         if (which == 0) k_end = k_end < m0 + 128 ? k_end : m0 + 128;
         else k_begin = k_begin > m0 ? k_begin : m0;
         k_end = k_end < p.Tp ? k_end : p.Tp;
@@ -679,7 +717,7 @@ __global__ void __launch_bounds__(kTriThreads, 1)
                 // B's column blocks: the head's (dQ: the KV head's) columns
                 const int bblk = (w.which == 0 ? w.h / group : w.h) * (D / 64);
                 for (int s = 0; s < w.n_steps; ++s, ++it) {
-                    const int st = it & 1, k0 = w.k_begin + s * 64;
+                    const int st = it & 1, k0 = w.contraction(s);
                     if (it >= 2 && !twait(&sh->freed[st], (uint32_t)(((it >> 1) & 1) ^ 1), sh)) { tgive_up(sh, 85); break; }
                     uint8_t *base = smem_raw + st * kStage;
                     mbar_arrive_expect_tx(&sh->full[st], kStage);
@@ -881,7 +919,7 @@ inline WorkspaceNeed tc_bwd_wide_workspace_need(int batch, int T, int n_heads, i
 inline int launch_bwd_wide(const float *q, const float *k, const float *v, const float *out, const float *dout,
                            const float *lse, float *delta, float *dq, float *dk, float *dv, void *workspace, size_t workspace_bytes, int batch, int T,
                            int n_heads, int n_kv_heads, int dim, cudaStream_t stream, bool qkv_planes_kept = false,
-                           bool tile_scores = false) {
+                           bool tile_scores = false, int window = 0, int sinks = 0) {
     using namespace tcb;
     using namespace tcw;
     const int td = tc_tile_dim(dim);
@@ -924,7 +962,8 @@ inline int launch_bwd_wide(const float *q, const float *k, const float *v, const
     const size_t smem = wide_smem_bytes();
     const size_t smem_t = td == 192 ? tri_smem_bytes<192>() : tri_smem_bytes<256>();
     const size_t smem_r = td == 192 ? res_smem_bytes<192>() : res_smem_bytes<256>();
-    const auto scores = td == 192 ? bwd_wide_scores_res<192> : bwd_wide_scores_res<256>;
+    const auto scores = window > 0 ? (td == 192 ? bwd_wide_scores_res<192, true> : bwd_wide_scores_res<256, true>)
+                                   : (td == 192 ? bwd_wide_scores_res<192, false> : bwd_wide_scores_res<256, false>);
     const auto products = td == 192 ? wide_products<192> : wide_products<256>;
     if (optin_smem((const void *)bwd_wide_scores, smem) || optin_smem((const void *)scores, smem_r) ||
         optin_smem((const void *)products, smem_t))
@@ -939,6 +978,7 @@ inline int launch_bwd_wide(const float *q, const float *k, const float *v, const
     p.unit_cap = cap;
     p.dq = dq, p.dk = dk, p.dv = dv;
     p.pieces = pieces;
+    p.win = BwdWindow{window, sinks, 0};
     p.scale = 1.0f / sqrtf((float)dim), p.scale_log2 = kLog2e / sqrtf((float)dim);
     p.p_scale = ldexpf(1.0f, 10);
     g_last_path = "tcgen05";

@@ -102,6 +102,43 @@ inline size_t bwd_parts_floats(int batch, int T, int n_heads, int n_kv_heads, in
     return n < 2 ? 0 : (size_t)n * 2 * batch * T * n_kv_heads * dim;
 }
 
+// The backward of a sliding window with sinks (window > 0).  A key tile's walk ends with the last query whose window reaches
+// it; only the tiles with sinks go on to the last query of all, and what lies beyond their window is given to further blocks,
+// `far` query tiles each -- about as long as the others' walks -- that come first in launch order.  Such a tile's dk and dv are sums
+// of several blocks, added in memory.
+struct BwdWindow {
+    int window, sinks, far;
+};
+struct WindowBlock {
+    int kt, qi0, n_q;  // key tile; query tiles [qi0, n_q) of `rows`
+    bool adds;
+};
+__host__ __device__ inline int near_tiles(const BwdWindow &w, int T, int kt, int rows) {
+    const int all = (T + rows - 1) / rows, near = (kt * 128 + 126 + w.window) / rows + 1;
+    return near < all ? near : all;
+}
+__host__ __device__ inline WindowBlock window_block(const BwdWindow &w, int T, int i, int rows) {
+    const int all = (T + rows - 1) / rows;
+    for (int kt = 0; kt * 128 < T && kt * 128 < w.sinks; ++kt) {
+        const int near = near_tiles(w, T, kt, rows), blocks = (all - near + w.far - 1) / w.far;
+        if (i < blocks) {
+            const int qi0 = near + i * w.far;
+            return WindowBlock{kt, qi0, qi0 + w.far < all ? qi0 + w.far : all, true};
+        }
+        i -= blocks;
+    }
+    const int near = near_tiles(w, T, i, rows);
+    return WindowBlock{i, i * (128 / rows), near, i * 128 < w.sinks && near < all};
+}
+inline int window_blocks(const BwdWindow &w, int T, int rows) {
+    const int all = (T + rows - 1) / rows;
+    int n = (T + 127) / 128;
+    for (int kt = 0; kt * 128 < T && kt * 128 < w.sinks; ++kt) n += (all - near_tiles(w, T, kt, rows) + w.far - 1) / w.far;
+    return n;
+}
+// Whether query t sees key j, of those at or before it.
+__host__ __device__ inline bool window_sees(const BwdWindow &w, int j, int t) { return j > t - w.window || j < w.sinks; }
+
 // Neither number grows with the shape -- a shorter sequence may be split where a longer one is not -- so a scratch that is to
 // serve every smaller shape too takes these, which do: the blocks that a split ends at, times what one of them writes.
 inline size_t fwd_parts_floats_bound(int dim) { return (size_t)split_sm_count() * 128 * (2 * (size_t)dim + 1); }

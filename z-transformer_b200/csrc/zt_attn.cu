@@ -306,18 +306,20 @@ static int backward_impl(const float *q, const float *k, const float *v, const f
                          const PeerList *dq_peers = nullptr, int window = 0, int sinks = 0) {
 #ifndef ZT_NO_TC
     const size_t least = backward_need(batch, T, n_heads, n_kv_heads, dim).least;
-    if (g_path.load() != 1 && window == 0 && workspace && workspace_bytes >= least &&
+    // (a window has fused kernels only: the caller that wants dq the same bit for bit, path 8, gets the CUDA cores' for it)
+    const bool path_takes = g_path.load() != 1 && !(g_path.load() == 8 && window > 0);
+    if (path_takes && workspace && workspace_bytes >= least &&
         (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
         n_kv_heads <= tcb::kPrepassMaxGroups && tcb::tc_bwd_supported(batch, T, dim, q, k, v, dout, dq, dk, dv)) {
         return launch_bwd_tc(q, k, v, out, dout, lse, delta, dq, dk, dv, workspace, workspace_bytes, batch, T, n_heads, n_kv_heads,
-                             dim, stream, nullptr, nullptr, kept, dq_peers, g_path.load() == 8);
+                             dim, stream, nullptr, nullptr, kept, dq_peers, g_path.load() == 8, window, sinks);
     }
-    if (g_path.load() != 1 && window == 0 && workspace && least > 0 && workspace_bytes >= least &&
+    if (path_takes && workspace && least > 0 && workspace_bytes >= least &&
         (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 && n_kv_heads <= tcb::kPrepassMaxGroups &&
         !(dq_peers && dq_peers->n > 0) &&
         tcw::tc_bwd_wide_supported(batch, T, n_heads, n_kv_heads, dim, q, k, v, dout, dq, dk, dv)) {
         return launch_bwd_wide(q, k, v, out, dout, lse, delta, dq, dk, dv, workspace, workspace_bytes, batch, T, n_heads, n_kv_heads, dim,
-                               stream, kept, g_path.load() == 8);
+                               stream, kept, g_path.load() == 8, window, sinks);
     }
 #endif
     if (dq_peers && dq_peers->n > 0)
