@@ -22,8 +22,11 @@ struct Pages {
     int shift;
     // Elements from the pool's begin to the row of slot j of sequence b; negative where the table names no page for it.
     __device__ __forceinline__ long long row(int b, int j) const {
-        const int slot = page_of(j), id = table[(long long)b * max_pages + slot];
-        return id < 0 || id >= n_pages ? -1 : ((long long)id * page_size + (j - slot * page_size)) * width;
+        return row_on(table[(long long)b * max_pages + page_of(j)], j);
+    }
+    // The same where the slot's page is known.
+    __device__ __forceinline__ long long row_on(int id, int j) const {
+        return id < 0 || id >= n_pages ? -1 : ((long long)id * page_size + (j - page_of(j) * page_size)) * width;
     }
     __device__ __forceinline__ int page_of(int j) const { return (int)(((uint64_t)(uint32_t)j * per) >> shift); }
     __device__ __forceinline__ long long capacity() const { return (long long)max_pages * page_size; }

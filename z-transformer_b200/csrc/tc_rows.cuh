@@ -37,12 +37,10 @@ namespace tcr {
 
 using namespace tc;
 using tcb::block_mult;
-using tcb::split_pack;
 using tcb::floats2;
 using tcb::fma2;
 using tcb::mul2;
 using tcf16::max_abs4;
-using tcf16::row_exp32;
 using tcf16::row_max32;
 using tcf16::split_q32;
 using tcf16::store_q_piece;
@@ -58,11 +56,11 @@ struct Cfg {
     static constexpr int KS = (TD == 256 ? 1 : 2) + (PLANES ? 1 : 0), VS = KS;  // slots of K and V tiles
     static constexpr int KP = BN * TD * 2;          // bytes of one piece of a tile
     static constexpr int QL = kWide ? 128 * TD * 2 : 0;
-    // What is copied, waited for and converted at a time is 16 keys of a tile: `part`.  A thread has CHUNKS 16-byte chunks of it,
-    // and a group of converting warps NP parts under way.
-    static constexpr int PARTS = BN / 16, PART = 16 * TD * 4, CHUNKS = PART / 16 / kConvert;
+    // What is copied, waited for and converted at a time is 16 keys of a tile (32 of 64 columns): a part.  A thread has CHUNKS 16-byte
+    // chunks of it, and a group of converting warps NP parts under way.
+    static constexpr int KEYS = TD == 64 ? 32 : 16, PARTS = BN / KEYS, PART = KEYS * TD * 4, CHUNKS = PART / 16 / kConvert;
     static constexpr int GROUPS = PLANES ? 0 : (kWide ? 1 : 2);
-    static constexpr int NP = TD == 64 ? 8 : (TD == 128 ? 5 : 4);
+    static constexpr int NP = TD == 128 ? 5 : 4;
     static constexpr int SETS = PLANES && kWide ? 1 : 2;  // of warps that make P: with tiles of 32 keys of wide heads one keeps up
     static constexpr int kThreads = (PLANES ? 128 * SETS : GROUPS * kConvert) + 256 + 128;
     // registers a thread, of what the launch gives: 640 threads 96 each, 512 threads 128
@@ -92,7 +90,7 @@ struct Shared {
     int found;
     float mk[16], mv[16];       // one over the scales of tiles j & 15 (powers of two)
     uint32_t odd[16][2];        // which values' rows of tile j & 15 hold something that is not finite
-    uint32_t top[2][2][4];      // [group][unit & 1][warp]: the largest hi piece; or max |x|
+    alignas(16) uint32_t top[2][2][4];  // [group][unit & 1][warp]: the largest hi piece; or max |x|
     uint32_t seed[2][4];
     float m_ref[8][128];        // the rows' reference maxima of tile j & 7
     float fin_m[2][128], fin_l[2][128], q_top[2][128];
@@ -140,7 +138,35 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
                  "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+// One over a power of two between 2^-126 and 2^126.
+__device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// v -> packed hi pieces and packed lo pieces.  What the hi ones leave of v comes of one instruction each, which takes a half and
+// two floats: with the halves turned into floats first a tile of 64 keys took 3 % longer.
+__device__ __forceinline__ void split(float2 v, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    float2 rest;
+    asm("{\n\t.reg .b16 a, b, m;\n\tmov.b32 {a, b}, %2;\n\tmov.b16 m, 0xBC00;\n\t"  // -1
+        "fma.rn.f32.f16 %0, a, m, %3;\n\tfma.rn.f32.f16 %1, b, m, %4;\n\t}"
+        : "=f"(rest.x), "=f"(rest.y) : "r"(hi), "f"(v.x), "f"(v.y));
+    const __half2 l = __floats2half2_rn(rest.x, rest.y);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+// P of 32 columns, times kPScale (which rides in the exponent, see tcf16::row_exp32); returns its sum.
+__device__ __forceinline__ float row_exp32(const uint32_t (&r)[32], float cs, float off, uint32_t (&ph)[16], uint32_t (&pl)[16]) {
+    const float2 cs2 = make_float2(cs, cs), off2 = make_float2(-off, -off);
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float2 x = fma2(floats2(r[i], r[i + 1]), cs2, off2);
+        const float2 pe = make_float2(ex2(x.x), ex2(x.y));
+        sum = tcb::add2(sum, pe);
+        split(pe, ph[i >> 1], pl[i >> 1]);
+    }
+    return sum.x + sum.y;
+}
 
 // -inf for those of 32 keys from key0 on that the query at `pos` does not see.
 __device__ __forceinline__ void mask_scores(uint32_t (&r)[32], const Seen &v, int key0, int pos) {
@@ -391,36 +417,54 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
         // where the keys of tile j lie; one that no row of this CTA sees counts as zero
         const auto place = [&](int j) { return both ? j & 7 : gi * 4 + (j & 3); };
         const auto rows_of = [&](int j) { return sh->row + place(j) * BN; };
+        // (in two steps: the table is asked a tile's conversion before its answer is used)
+        int key = 0, page = 0;
+        bool wanted = false;
+        const auto ask = [&](int j) {
+            wanted = false;
+            if (ct >= BN || j >= n) return;
+            key = key0(j) + ct;
+            wanted = key <= pos_last && (p.seen.window == 0 || key > pos_first - p.seen.window || key < p.seen.sinks);
+            if (PAGED && wanted) page = p.pg.table[(long long)t.b * p.pg.max_pages + p.pg.page_of(key)];
+        };
         const auto look_up = [&](int j) {
             if (ct < 2 && (both || gi == 1)) sh->odd[j & 15][ct] = 0;
             if (ct >= BN || j >= n) return;
-            const int key = key0(j) + ct;
             long long at = kNone;
-            if (key <= pos_last && (p.seen.window == 0 || key > pos_first - p.seen.window || key < p.seen.sinks)) {
-                at = PAGED ? p.pg.row(t.b, key) : ((long long)t.b * p.T + key) * width;
-                if (at < 0) at = kNoPage;
-            }
+            if (wanted) at = PAGED ? p.pg.row_on(page, key) : ((long long)t.b * p.T + key) * width;
+            if (PAGED && wanted && at < 0) at = kNoPage;
             rows_of(j)[ct] = at;
             const bool hole = PAGED && __any_sync(0xffffffffu, at == kNoPage);
             if (lane == 0) sh->holes[place(j)][cw] = hole;
         };
-        // A part's sixteen rows by eight threads each, a thread the chunks (ct & 7) + 8 i of its row: one look-up and one address a
-        // part, whole 128-byte lines a row, and sixteen threads write eight bytes each of two rows whose chunks lie in
+        // Sixteen rows by eight threads each, a thread the chunks (ct & 7) + 8 i of its row: one look-up and one address a row, whole 128-byte lines a row, and sixteen threads write eight bytes each of two rows whose chunks lie in
         // different banks (rows four apart, see the swizzle).
         const int pr = (ct >> 3 & 1) << 2 | (ct >> 4 & 3) | (ct >> 6) << 3, pc = ct & 7;
+        constexpr int CPT = TD / 32;                     // chunks that a thread has of a row
         const int my_chunks = (p.dim / 4 - pc + 7) / 8;  // of the head's columns; the rest of the tile's are zeros
+        const bool whole = p.dim == TD;
         const float *k_col = p.k + (long long)g * p.dim + pc * 4, *v_col = p.v + (long long)g * p.dim + pc * 4;
         int cu = 0, cq = 0, cs = 0;  // the part that is copied next: unit, part, place in the ring
         const auto copy_part = [&]() {
             if (cu < n_units) {
                 bool is_k;
                 const int j = unit(cu, is_k);
-                const long long at = rows_of(j)[cq * 16 + pr];
-                const float *src = (is_k ? k_col : v_col) + (at >= 0 ? at : 0);
-                const int have = at >= 0 ? my_chunks : 0;
                 const uint32_t dst = smem_u32(ring) + (uint32_t)(cs * C::PART + ct * 16);
+                const float *col = is_k ? k_col : v_col;
 #pragma unroll
-                for (int i = 0; i < CH; ++i) copy16_async(dst + i * (kConvert * 16), i < have ? src + i * 32 : p.k, i < have);
+                for (int r = 0; r < C::KEYS; r += 16) {
+                    const long long at = rows_of(j)[cq * C::KEYS + r + pr];
+                    const float *src = col + (at >= 0 ? at : 0);
+                    const uint32_t to = dst + (r / 16) * CPT * (kConvert * 16);
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < CPT; ++i) copy16_async(to + i * (kConvert * 16), src + i * 32, at >= 0);
+                    } else {
+                        const int have = at >= 0 ? my_chunks : 0;
+#pragma unroll
+                        for (int i = 0; i < CPT; ++i) copy16_async(to + i * (kConvert * 16), i < have ? src + i * 32 : p.k, i < have);
+                    }
+                }
                 cs = cs + 1 == NP ? 0 : cs + 1;
                 if (++cq == PARTS) cq = 0, ++cu;
             }
@@ -462,8 +506,8 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 float4 x = chunk(f);
                 if (!is_k) x.x = finite(x.x) ? x.x : 0.f, x.y = finite(x.y) ? x.y : 0.f, x.z = finite(x.z) ? x.z : 0.f, x.w = finite(x.w) ? x.w : 0.f;
                 uint2 h, l;
-                split_pack(x.x * m, x.y * m, h.x, l.x);
-                split_pack(x.z * m, x.w * m, h.y, l.y);
+                split(make_float2(x.x * m, x.y * m), h.x, l.x);
+                split(make_float2(x.z * m, x.w * m), h.y, l.y);
                 uint8_t *at = dst + piece_at(f / CPR, f % CPR);
                 *reinterpret_cast<uint2 *>(at) = h;
                 *reinterpret_cast<uint2 *>(at + KP) = l;
@@ -473,7 +517,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             return m;
         };
         if (ct < 8) sh->holes[ct][1] = 0;  // (tiles of 32 keys have one half)
-        for (int j = 0; j < 4; ++j) look_up(j);
+        for (int j = 0; j < 4; ++j) ask(j), look_up(j);
         sync();
 #pragma unroll 1
         for (int i = 0; i < NP; ++i) copy_part();
@@ -493,6 +537,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 rgive_up(sh, 104);
                 ok = false;  // (on to the barriers that the other warps wait at)
             }
+            if (!both || is_k) ask(j + 4);
             float m = is_k ? m_k : m_v;
             uint32_t top = 0;
 #pragma unroll 1
@@ -515,14 +560,14 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 }
                 if (!ok) continue;
                 const float2 mm = make_float2(m, m);
-                uint8_t *even = dst + q * (16 * 128) + piece0, *odd = dst + q * (16 * 128) + (piece0 ^ 64);
+                uint8_t *even = dst + q * (C::KEYS * 128) + piece0, *odd = dst + q * (C::KEYS * 128) + (piece0 ^ 64);
 #pragma unroll
                 for (int i = 0; i < CH; ++i) {
                     uint2 h, l;
-                    split_pack(mul2(make_float2(x[i].x, x[i].y), mm), h.x, l.x);
-                    split_pack(mul2(make_float2(x[i].z, x[i].w), mm), h.y, l.y);
+                    split(mul2(make_float2(x[i].x, x[i].y), mm), h.x, l.x);
+                    split(mul2(make_float2(x[i].z, x[i].w), mm), h.y, l.y);
                     top = __vmaxu2(top, __vmaxu2(h.x & 0x7fff7fffu, h.y & 0x7fff7fffu));
-                    uint8_t *at = (i & 1 ? odd : even) + (i >> 1) * (BN * 128);
+                    uint8_t *at = (i & 1 ? odd : even) + (i % CPT >> 1) * (BN * 128) + (i / CPT) * (16 * 128);
                     *reinterpret_cast<uint2 *>(at) = h;
                     *reinterpret_cast<uint2 *>(at + KP) = l;
                 }
@@ -532,15 +577,15 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             top = max(top & 0xffffu, top >> 16);
             top = __reduce_max_sync(0xffffffffu, top);
             if (lane == 0) sh->top[gi][u & 1][cw] = top;
-            const int hole = sh->holes[place(j)][0] | sh->holes[place(j)][1];
+            const int hole = PAGED ? sh->holes[place(j)][0] | sh->holes[place(j)][1] : 0;
             sync();
-            const uint32_t *tops = sh->top[gi][u & 1];
-            top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+            const uint4 tops = *reinterpret_cast<const uint4 *>(sh->top[gi][u & 1]);
+            top = max(max(tops.x, tops.y), max(tops.z, tops.w));
             // The largest hi piece below 2^-3 (its lo piece would lose bits), or none, or not finite: with care.
             const bool care = top < 0x3000u || top >= 0x7c00u || (is_k && hole);
             if (care) m = with_care(dst, is_k, j, u);
             if (ct == 0) {
-                (is_k ? sh->mk : sh->mv)[j & 15] = 1.f / m;
+                (is_k ? sh->mk : sh->mv)[j & 15] = pow2_inverse(m);
                 if (ok) mbar_arrive(is_k ? &sh->k_full[s] : &sh->v_full[s]);
             }
             // the next tile's: with which this one's largest would have been in [2^12, 2^13)
@@ -853,7 +898,7 @@ __global__ void __launch_bounds__(256) rows_planes_kernel(const Params p) {
     float m[2];
     for (int i = 0; i < 2; ++i) m[i] = block_mult(max(max(tops[i][0], tops[i][1]), max(tops[i][2], tops[i][3]))) * 0.25f;
     const long long at = ((long long)b * p.n_kv_heads + g) * p.tiles + tile;
-    if (threadIdx.x == 0) p.heads[at] = make_uint4(__float_as_uint(1.f / m[0]), __float_as_uint(1.f / m[1]), odd[0], odd[1]);
+    if (threadIdx.x == 0) p.heads[at] = make_uint4(__float_as_uint(pow2_inverse(m[0])), __float_as_uint(pow2_inverse(m[1])), odd[0], odd[1]);
     uint8_t *dst = p.planes + at * (4 * KP) + (is_k ? 0 : 2 * KP);
     const float2 mm = is_k ? make_float2(m[0], m[0]) : make_float2(m[1], m[1]);
 #pragma unroll
@@ -863,8 +908,8 @@ __global__ void __launch_bounds__(256) rows_planes_kernel(const Params p) {
             const float4 y = x[q * (TD / 32) + i];
             const int r = q * 16 + pr, c = pc + 8 * i;
             uint2 h, l;
-            split_pack(mul2(make_float2(y.x, y.y), mm), h.x, l.x);
-            split_pack(mul2(make_float2(y.z, y.w), mm), h.y, l.y);
+            split(mul2(make_float2(y.x, y.y), mm), h.x, l.x);
+            split(mul2(make_float2(y.z, y.w), mm), h.y, l.y);
             uint8_t *to = dst + (c >> 4) * (BN * 128) + r * 128 + ((((c & 15) >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
             *reinterpret_cast<uint2 *>(to) = h;
             *reinterpret_cast<uint2 *>(to + KP) = l;
