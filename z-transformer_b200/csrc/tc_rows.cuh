@@ -50,9 +50,12 @@ constexpr int kConvert = 128;  // threads that convert a tile
 template <int TD, bool PLANES>
 struct Cfg {
     static constexpr bool kWide = TD > 128;
-    static constexpr int BN = kWide ? 32 : 64;      // keys of a tile
+    // Keys of a tile.  (Narrow heads that convert their own: what a tile costs beside its conversion is shared by twice the keys.  Us,
+    // 64 / 128: 32 ragged sequences of 16 heads of 64 378 / 353; converted beforehand, where a tile waits for two S buffers then,
+    // batch 4, T 2048, 32/8 heads of 64 206 / 272.)
+    static constexpr int BN = kWide ? 32 : (TD == 64 && !PLANES ? 128 : 64);
     static constexpr int OB = TD == 64 ? 2 : 1;     // O buffers
-    static constexpr int SB = 4;                    // S/P buffers
+    static constexpr int SB = BN == 128 ? 2 : 4;    // S/P buffers
     static constexpr int KS = (TD == 256 ? 1 : 2) + (PLANES ? 1 : 0), VS = KS;  // slots of K and V tiles
     static constexpr int KP = BN * TD * 2;          // bytes of one piece of a tile
     static constexpr int QL = kWide ? 128 * TD * 2 : 0;
@@ -60,7 +63,7 @@ struct Cfg {
     // chunks of it, and a group of converting warps NP parts under way.
     static constexpr int KEYS = TD == 64 ? 32 : 16, PARTS = BN / KEYS, PART = KEYS * TD * 4, CHUNKS = PART / 16 / kConvert;
     static constexpr int GROUPS = PLANES ? 0 : (kWide ? 1 : 2);
-    static constexpr int NP = TD == 128 ? 5 : 4;
+    static constexpr int NP = kWide || PLANES ? 4 : 5;
     static constexpr int SETS = PLANES && kWide ? 1 : 2;  // of warps that make P: with tiles of 32 keys of wide heads one keeps up
     static constexpr int kThreads = (PLANES ? 128 * SETS : GROUPS * kConvert) + 256 + 128;
     // registers a thread, of what the launch gives: 640 threads 96 each, 512 threads 128
@@ -89,15 +92,15 @@ struct Shared {
     volatile int abort;
     int found;
     float mk[16], mv[16];       // one over the scales of tiles j & 15 (powers of two)
-    uint32_t odd[16][2];        // which values' rows of tile j & 15 hold something that is not finite
+    uint32_t odd[16][4];        // which values' rows of tile j & 15 hold something that is not finite
     alignas(16) uint32_t top[2][2][4];  // [group][unit & 1][warp]: the largest hi piece; or max |x|
     uint32_t seed[2][4];
     float m_ref[8][128];        // the rows' reference maxima of tile j & 7
     float fin_m[2][128], fin_l[2][128], q_top[2][128];
     // elements to the rows of the next tiles' keys (kNone: counts as zero, kNoPage: NaN): of a group's tile j & 3 or, in tiles
-    // of 32 keys, of j & 7; and whether some key of the tile is on no page, by halves
-    long long row[512];
-    int holes[8][2];
+    // of 32 keys, of j & 7; and whether some key of the tile is on no page, 32 keys a word
+    long long row[1024];
+    int holes[8][4];
 };
 constexpr long long kNone = -1, kNoPage = -2;
 
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             if (PAGED && wanted) page = p.pg.table[(long long)t.b * p.pg.max_pages + p.pg.page_of(key)];
         };
         const auto look_up = [&](int j) {
-            if (ct < 2 && (both || gi == 1)) sh->odd[j & 15][ct] = 0;
+            if (ct < BN / 32 && (both || gi == 1)) sh->odd[j & 15][ct] = 0;
             if (ct >= BN || j >= n) return;
             long long at = kNone;
             if (wanted) at = PAGED ? p.pg.row_on(page, key) : ((long long)t.b * p.T + key) * width;
@@ -516,7 +519,8 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             sync();
             return m;
         };
-        if (ct < 8) sh->holes[ct][1] = 0;  // (tiles of 32 keys have one half)
+        if (ct < 32) sh->holes[ct >> 2][ct & 3] = 0;  // (not every tile has four words)
+        sync();
         for (int j = 0; j < 4; ++j) ask(j), look_up(j);
         sync();
 #pragma unroll 1
@@ -577,7 +581,9 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             top = max(top & 0xffffu, top >> 16);
             top = __reduce_max_sync(0xffffffffu, top);
             if (lane == 0) sh->top[gi][u & 1][cw] = top;
-            const int hole = PAGED ? sh->holes[place(j)][0] | sh->holes[place(j)][1] : 0;
+            int hole = 0;
+            if (PAGED && is_k)
+                for (int i = 0; i < BN / 32; ++i) hole |= sh->holes[place(j)][i];
             sync();
             const uint4 tops = *reinterpret_cast<const uint4 *>(sh->top[gi][u & 1]);
             top = max(max(tops.x, tops.y), max(tops.z, tops.w));
@@ -738,12 +744,14 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 for (int i = 0; i < COLS; i += 2)
                     o[(c + i) >> 1] = fma2(floats2(r[i / 32][i % 32], r[i / 32][i % 32 + 1]), make_float2(w, w), o[(c + i) >> 1]);
             }
-            const uint32_t odd[2] = {sh->odd[j & 15][0], sh->odd[j & 15][1]};
-            if (odd[0] | odd[1]) {  // values that are not finite, added to the rows that see them
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) any |= sh->odd[j & 15][i];
+            if (any) {  // values that are not finite, added to the rows that see them
 #pragma unroll 1
                 for (int i = 0; i < BN; ++i) {
                     const int key = key0(j) + i;
-                    if (!(odd[i >> 5] >> (i & 31) & 1u) || !p.seen(key, pos)) continue;
+                    if (!(sh->odd[j & 15][i >> 5] >> (i & 31) & 1u) || !p.seen(key, pos)) continue;
                     const long long at = PAGED ? p.pg.row(t.b, key) : ((long long)t.b * p.T + key) * ((long long)p.n_kv_heads * p.dim);
                     if (at < 0) continue;
 #pragma unroll
