@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const Params p, float *o
 // Key tiles for a launch that reads them converted: a block per (tile, KV head, sequence), half of its threads for K and half for
 // V.  Reads f32 rows that some row of the sequence sees, writes as much; bound by memory.
 template <int TD, bool PAGED>
-__global__ void __launch_bounds__(256) rows_planes_kernel(const Params p) {
+__global__ void __launch_bounds__(256, 3) rows_planes_kernel(const Params p) {
     using C = Cfg<TD, true>;
     constexpr int BN = C::BN, KP = C::KP, N = BN / 16 * (TD / 32);  // (N: chunks of a thread)
     __shared__ uint32_t tops[2][4], odd[2];
@@ -872,12 +872,12 @@ __global__ void __launch_bounds__(256) rows_planes_kernel(const Params p) {
     const float *col = (is_k ? p.k : p.v) + (long long)g * p.dim + pc * 4;
     const long long width = PAGED ? p.pg.width : (long long)p.n_kv_heads * p.dim;
     float4 x[N];
-    bool hole[BN / 16];
+    uint32_t holes = 0;
 #pragma unroll
     for (int q = 0; q < BN / 16; ++q) {
         const int key = key0 + q * 16 + pr;
         const long long at = !seen(key) ? kNone : PAGED ? p.pg.row(b, key) : ((long long)b * p.T + key) * width;
-        hole[q] = PAGED && seen(key) && at < 0;
+        if (PAGED && seen(key) && at < 0) holes |= 1u << q;
 #pragma unroll
         for (int i = 0; i < TD / 32; ++i)
             x[q * (TD / 32) + i] = at >= 0 && (pc + 8 * i) * 4 < p.dim ? *reinterpret_cast<const float4 *>(col + at + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -898,7 +898,7 @@ __global__ void __launch_bounds__(256) rows_planes_kernel(const Params p) {
                     atomicOr(&odd[r >> 5], 1u << (r & 31));
                 }
             }
-            if (is_k && hole[q]) y.x = __int_as_float(0x7fc00000);
+            if (PAGED && is_k && (holes >> q & 1u)) y.x = __int_as_float(0x7fc00000);
         }
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) tops[is_k ? 0 : 1][(threadIdx.x >> 5) & 3] = top;
