@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
     const int per_head = n_q - qi0;
     const int n_it = n_heads_mine * per_head;
     const int B = p.batch;
+    using Walk = WalkOf<BQ, WIN ? kFlushRowsWin : kFlushRows>;
     Walk walk(n_heads_mine, per_head, qi0, n_q);
 
     if (threadIdx.x == 0) {
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
                 const uint32_t qh = q_u32 + (uint32_t)((j & 1) * 2 * QP);
                 const uint64_t bqh = desc_kmajor(qh), bql = desc_kmajor(qh + QP);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
+                for (int kk = 0; !WIN && kk < D / 16; ++kk) {
                     if (PAD && kk >= steps) break;
                     const uint32_t ao = (uint32_t)((kk >> 2) * (128 * 128) + (kk & 3) * 32);
                     const uint32_t bo = (uint32_t)((kk >> 2) * (BQ * 128) + (kk & 3) * 32);
@@ -218,6 +219,20 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
                     mma_ss_f16(tmem + cST, dkh, dqh, id_s, kk > 0);
                     mma_ss_f16(tmem + cST, dkh, dql, id_s, 1);
                     mma_ss_f16(tmem + cST, dkl, dqh, id_s, 1);
+                }
+                // (a window's in the order of its forward, attn_rows_tc)
+#pragma unroll
+                for (int i = 0; WIN && i < D / 8; ++i) {
+                    const int kk = (i >> 3) * 4 + (i & 3);
+                    if (PAD && kk >= steps) continue;
+                    const uint32_t ao = (uint32_t)((kk >> 2) * (128 * 128) + (kk & 3) * 32), bo = (uint32_t)((kk >> 2) * (BQ * 128) + (kk & 3) * 32);
+                    const uint64_t dkh = desc_advance(bkh, ao), dqh = desc_advance(bqh, bo);
+                    if (i & 4) {
+                        mma_ss_f16(tmem + cST, dkh, dqh, id_s, 1);
+                    } else {
+                        mma_ss_f16(tmem + cST, desc_advance(bkl, ao), dqh, id_s, kk > 0);
+                        mma_ss_f16(tmem + cST, dkh, desc_advance(bql, bo), id_s, 1);
+                    }
                 }
                 mma_commit(&sh->st_full);
             };
@@ -295,10 +310,18 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
                     const uint32_t bo = (uint32_t)((kk >> 2) * (BQ * 128) + (kk & 3) * 32);
                     const uint64_t dvl = desc_advance(bvl, ao);
                     const uint64_t dgh = desc_advance(bgh, bo), dgl = desc_advance(bgl, bo);
-                    mma_ts_f16(tmem + cDPT, tmem + cVh + kk * 8, dgh, id_s, kk > 0);
-                    mma_ts_f16(tmem + cDPT, tmem + cVh + kk * 8, dgl, id_s, 1);
+                    // (a window's: the two small terms of the whole contraction first, while there is little to truncate)
+                    if (!WIN) mma_ts_f16(tmem + cDPT, tmem + cVh + kk * 8, dgh, id_s, kk > 0);
+                    mma_ts_f16(tmem + cDPT, tmem + cVh + kk * 8, dgl, id_s, !WIN || kk > 0);
                     mma_ss_f16(tmem + cDPT, dvl, dgh, id_s, 1);
                 }
+                if (WIN)
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        if (PAD && kk >= steps) break;
+                        const uint32_t bo = (uint32_t)((kk >> 2) * (BQ * 128) + (kk & 3) * 32);
+                        mma_ts_f16(tmem + cDPT, tmem + cVh + kk * 8, desc_advance(bgh, bo), id_s, 1);
+                    }
                 mma_commit(&sh->free_g);  // (one of two arrivals: dV(j) reads the same tile)
                 mma_commit(&sh->dp_full);
                 return true;
@@ -308,10 +331,14 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
                 for (int kk = kk0; kk < kk0 + 4; ++kk) {
                     const uint64_t dkh = desc_advance(mkh, kk * 2048), dkl = desc_advance(mkl, kk * 2048);
                     const uint64_t ddh = desc_advance(mdh, kk * 2048), ddl = desc_advance(mdl, kk * 2048);
-                    mma_ss_f16(tmem + cDQT, dkh, ddh, id_q, kk > 0);
-                    mma_ss_f16(tmem + cDQT, dkh, ddl, id_q, 1);
+                    if (!WIN) mma_ss_f16(tmem + cDQT, dkh, ddh, id_q, kk > 0);
+                    mma_ss_f16(tmem + cDQT, dkh, ddl, id_q, !WIN || kk > 0);
                     mma_ss_f16(tmem + cDQT, dkl, ddh, id_q, 1);
                 }
+                if (WIN)
+#pragma unroll
+                    for (int kk = kk0; kk < kk0 + 4; ++kk)
+                        mma_ss_f16(tmem + cDQT, desc_advance(mkh, kk * 2048), desc_advance(mdh, kk * 2048), id_q, 1);
             };
             int n_flush = 0;
             if (ok && !issue_dp(0)) { fgive_up(sh, 63); ok = false; }

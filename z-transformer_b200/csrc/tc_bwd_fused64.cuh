@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kFused64Threads, 1)
     const int per_head = n_q - qi0;
     const int n_it = n_heads_mine * per_head;
     const int B = p.batch;
-    WalkOf<BQ> walk(n_heads_mine, per_head, qi0, n_q);
+    using Walk = WalkOf<BQ, WIN ? kFlushRowsWin : kFlushRows>;
+    Walk walk(n_heads_mine, per_head, qi0, n_q);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&sh->full_q[i], 1), mbar_init(&sh->free_q[i], 1);
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(kFused64Threads, 1)
             load_head<1>(sVl, &vmap, &sh->k_full, s0, g, B + b, BR, padded);
             int n_ql = 0, n_gl = 0;  // tiles issued
             bool live = true;
-            WalkOf<BQ> wq = walk, wg = walk;
+            Walk wq = walk, wg = walk;
             auto load_q = [&]() {  // Q tile of step n_ql
                 const int j = n_ql, s = j & 1;
                 // (its slot was last read by dK(j - 2))
@@ -214,12 +215,25 @@ __global__ void __launch_bounds__(kFused64Threads, 1)
                 const uint32_t qh = q_u32 + (uint32_t)((j & 1) * 2 * QP);
                 const uint64_t bqh = desc_kmajor(qh), bql = desc_kmajor(qh + QP);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
+                for (int kk = 0; !WIN && kk < D / 16; ++kk) {
                     if (PAD && kk >= steps) break;
                     const uint64_t dkh = desc_advance(bkh, kk * 32), dqh = desc_advance(bqh, kk * 32);
                     mma_ss_f16(tmem + cST, dkh, dqh, id_s, kk > 0);
                     mma_ss_f16(tmem + cST, desc_advance(bkl, kk * 32), dqh, id_s, 1);
                     mma_ss_f16(tmem + cST, dkh, desc_advance(bql, kk * 32), id_s, 1);
+                }
+                // (a window's in the order of its forward, attn_rows_tc, where the small terms go first)
+#pragma unroll
+                for (int i = 0; WIN && i < D / 8; ++i) {
+                    const int kk = i & 3;
+                    if (PAD && kk >= steps) continue;
+                    const uint64_t dkh = desc_advance(bkh, kk * 32), dqh = desc_advance(bqh, kk * 32);
+                    if (i & 4) {
+                        mma_ss_f16(tmem + cST, dkh, dqh, id_s, 1);
+                    } else {
+                        mma_ss_f16(tmem + cST, desc_advance(bkl, kk * 32), dqh, id_s, kk > 0);
+                        mma_ss_f16(tmem + cST, dkh, desc_advance(bql, kk * 32), id_s, 1);
+                    }
                 }
                 mma_commit(&sh->st_full);
             };

@@ -458,13 +458,26 @@ __global__ void __launch_bounds__(kResThreads, 1)
                         const uint64_t bh = desc_kmajor(base), bl = desc_kmajor(base + BT);
                         const uint64_t al = desc_kmajor(a_lo + (uint32_t)(blk * BT));
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
+                        for (int kk = 0; !WIN && kk < 4; ++kk) {
                             if (blk * 4 + kk >= steps) break;
                             const uint64_t dbh = desc_advance(bh, kk * 32), dbl = desc_advance(bl, kk * 32);
                             const uint32_t at = a_hi + (uint32_t)((blk * 4 + kk) * 8);
                             mma_ts_f16(acc, at, dbh, idesc, (blk > 0 || kk > 0) ? 1 : 0);
                             mma_ts_f16(acc, at, dbl, idesc, 1);
                             mma_ss_f16(acc, desc_advance(al, kk * 32), dbh, idesc, 1);
+                        }
+                        // (a window's in the order of its forward, attn_rows_tc, where the small terms go first)
+#pragma unroll
+                        for (int i = 0; WIN && i < 8; ++i) {
+                            const int kk = i & 3;
+                            if (blk * 4 + kk >= steps) continue;
+                            const uint32_t at = a_hi + (uint32_t)((blk * 4 + kk) * 8);
+                            if (i & 4) {
+                                mma_ts_f16(acc, at, desc_advance(bh, kk * 32), idesc, 1);
+                            } else {
+                                mma_ts_f16(acc, at, desc_advance(bl, kk * 32), idesc, (blk > 0 || kk > 0) ? 1 : 0);
+                                mma_ss_f16(acc, desc_advance(al, kk * 32), desc_advance(bh, kk * 32), idesc, 1);
+                            }
                         }
                         mma_commit(&sh->freed[st]);
                     }

@@ -307,15 +307,23 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                     const uint32_t cS = C::cS + (j % SB) * BN;
                     const uint64_t bkh = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP)), bkl = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP + KP));
                     const uint64_t bql = desc_kmajor(ql_u32);
+// (64 columns at a time the two small terms first, while there is little to truncate.  The backward forms S in the same
+                    // order: where a softmax is saturated, what its dP and delta leave of each other is as good as the two S agree.)
 #pragma unroll
-                    for (int kk = 0; kk < TD / 16; ++kk) {
-                        if (kk >= steps) break;
-                        const uint32_t bo = (uint32_t)((kk >> 2) * (BN * 128) + (kk & 3) * 32);
-                        const uint64_t dkh = desc_advance(bkh, bo), dkl = desc_advance(bkl, bo);
-                        mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, dkh, id_s, kk > 0);
-                        mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, dkl, id_s, 1);
-                        if (C::kWide) mma_ss_f16(tmem + cS, desc_advance(bql, (uint32_t)((kk >> 2) * (128 * 128) + (kk & 3) * 32)), dkh, id_s, 1);
-                        else mma_ts_f16(tmem + cS, tmem + C::cQl + kk * 8, dkh, id_s, 1);
+                    for (int c = 0; c < TD / 64; ++c) {
+#pragma unroll
+                        for (int kk = 4 * c; kk < 4 * c + 4; ++kk) {
+                            if (kk >= steps) break;
+                            const uint32_t bo = (uint32_t)(c * (BN * 128) + (kk & 3) * 32);
+                            mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, desc_advance(bkl, bo), id_s, kk > 0);
+                            if (C::kWide) mma_ss_f16(tmem + cS, desc_advance(bql, (uint32_t)(c * (128 * 128) + (kk & 3) * 32)), desc_advance(bkh, bo), id_s, 1);
+                            else mma_ts_f16(tmem + cS, tmem + C::cQl + kk * 8, desc_advance(bkh, bo), id_s, 1);
+                        }
+#pragma unroll
+                        for (int kk = 4 * c; kk < 4 * c + 4; ++kk) {
+                            if (kk >= steps) break;
+                            mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, desc_advance(bkh, (uint32_t)(c * (BN * 128) + (kk & 3) * 32)), id_s, 1);
+                        }
                     }
                     mma_commit(&sh->k_free[s]);
                     mma_commit(&sh->s_full[j % SB]);
@@ -339,10 +347,13 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                     for (int kk = 0; kk < BN / 16; ++kk) {
                         const uint32_t ac = (uint32_t)(32 * (kk >> 1) + (kk & 1) * 8);
                         const uint64_t dvh = desc_advance(mvh, kk * 2048), dvl = desc_advance(mvl, kk * 2048);
-                        mma_ts_f16(tmem + cO, tmem + cS + ac, dvh, id_o, kk > 0);
-                        mma_ts_f16(tmem + cO, tmem + cS + ac, dvl, id_o, 1);
+                        // (the two small terms of the whole contraction first, while there is little to truncate)
+                        mma_ts_f16(tmem + cO, tmem + cS + ac, dvl, id_o, kk > 0);
                         mma_ts_f16(tmem + cO, tmem + cS + ac + 16, dvh, id_o, 1);
                     }
+#pragma unroll
+                    for (int kk = 0; kk < BN / 16; ++kk)
+                        mma_ts_f16(tmem + cO, tmem + cS + (uint32_t)(32 * (kk >> 1) + (kk & 1) * 8), desc_advance(mvh, kk * 2048), id_o, 1);
                     mma_commit(&sh->v_free[s]);
                     mma_commit(&sh->o_full[ob]);
                     mma_commit(&sh->pv_done[j % SB]);

@@ -1204,6 +1204,8 @@ int zt_attn_backward_window_batched(const float *q, const float *k, const float 
     g_last_error[0] = 0;
     if (check_window(window, sinks)) return 1;
     normal_window(T, &window, &sinks);
+    // (no window: one as long as the sequence, so that S is formed as this entry's forward formed it)
+    if (window == 0 && T > 0) window = T;
     return backward_kept_impl(q, k, v, out, lse, dout, dq, dk, dv, delta, workspace, workspace_bytes, batch, T, n_heads,
                               n_kv_heads, dim, stream, 0ull, nullptr, window, sinks);
 }
