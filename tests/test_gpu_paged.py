@@ -402,6 +402,47 @@ def test_offsets_beyond_31_bits(zt):
     assert torch.equal(kp[n_pages - 1, page - 1], new[0]) and int(n) == page
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_table_too_long_to_convert_beforehand(zt, D):
+    """Many rows over a table of a million places, nearly all without a page: the rows convert their own keys, and find the same."""
+    c = Case([300, 500], [900, 40], 8, 2, D, 16, 100, 3, seed=23)
+    ref = c.call(zt)
+    room = zt.PagedWorkspace(2, c.N, c.table.shape[1] * 16, 8, 2, D).nbytes
+    c.check(*ref)
+    c.table = torch.nn.functional.pad(c.table, (0, 2**16 - c.table.shape[1]), value=-1)
+    ws = zt.PagedWorkspace(2, c.N, 2**20, 8, 2, D)
+    assert ws.nbytes > room
+    out, lse = c.call(zt, workspace=ws)
+    c.check(out, lse)
+    near(out, ref[0].double(), "the two forms")
+
+
+def test_numbers_at_the_edge_of_31_bits(zt):
+    """Windows and sinks of any size, and a table whose capacity nearly fills 31 bits."""
+    c = Case([40, 1], [100, 900], 8, 2, 64, 16, seed=24)
+    for window, sinks in ((2**31 - 1, 0), (2**30 - 1, 2**31 - 1), (2**40, 2**40), (5, 2**31 - 1), (2**30 - 5, 3)):
+        out, lse = zt.attention_paged(c.q, c.k, c.v, c.table, c.n_keys, 8, 2, 64, cu_rows=c.cu, window=window, sinks=sinks, want_lse=True)
+        c.check(out, lse)
+        s = Case([1, 1], [100, 900], 8, 2, 64, 16, seed=25)
+        out, lse = zt.attention_paged(s.q, s.k, s.v, s.table, s.n_keys, 8, 2, 64, window=window, sinks=sinks, want_lse=True)
+        s.check(out, lse)
+    page = 2**24
+    k = torch.zeros(1, 16, 128, device="cuda")  # (a pool of one page of 16 rows: no slot from 16 on is filled)
+    table = torch.zeros(1, 127, dtype=torch.int32, device="cuda")
+    n = torch.tensor([9], dtype=torch.int32, device="cuda")
+    L = zt.lib.load()
+    q, out = rand(9, 256, seed=1), torch.empty(9, 256, device="cuda")
+    cu = torch.tensor([0, 9], dtype=torch.int32, device="cuda")
+    ws = zt.PagedWorkspace(1, 9, 127 * page, 4, 2, 64)
+    k.copy_(rand(1, 16, 128, seed=2))
+    assert L.zt_attn_paged(q.data_ptr(), k.data_ptr(), k.data_ptr(), table.data_ptr(), n.data_ptr(), cu.data_ptr(), out.data_ptr(), None,
+                           ws.buf.data_ptr(), ws.nbytes, 1, 9, 1, page, 127, 4, 2, 64, 3, 1, torch.cuda.current_stream().cuda_stream) == 0
+    c = Case.__new__(Case)
+    c.rows, c.past, c.H, c.G, c.D, c.window, c.sinks = [9], [0], 4, 2, 64, 3, 1
+    c.q, c.cu, c.keys = q, torch.tensor([0, 9]), [[k[0, :9], k[0, :9]]]
+    near(out, c.reference(0)[0], "one long page")
+
+
 def test_on_another_stream_than_the_tensors_own(zt):
     c = Case([40, 3], [100, 900], 8, 2, 64, 16, seed=20)
     torch.cuda.synchronize()

@@ -80,8 +80,8 @@ struct Cfg {
     static constexpr int RS = TD * 4 + 16;
     static constexpr bool kStaged = PLANES || !kWide;
     static constexpr int kQ = (PLANES ? kData : (KS + VS) * 2 * KP) - 128 * RS;
-    static constexpr int kEarly = kQ / (2 * KP) < KS ? kQ / (2 * KP) : KS;  // K slots in front of the query rows
-    static_assert(!kStaged || kEarly >= 1, "the query rows are staged where tiles come later");
+    static constexpr int kEarly = 1;  // K tiles that come before the query rows are through
+    static_assert(!kStaged || kQ >= 2 * KP, "the query rows are staged where tiles come later");
     static_assert(128 * RS <= kData, "the finished rows are staged where the tiles were");
     static_assert(NP <= 2 * PARTS, "rows are looked up two tiles ahead");
 };
@@ -119,7 +119,6 @@ struct Params {
     uint8_t *planes;
     uint4 *heads;
     int tiles;
-    int ahead;  // the query rows of the block this many places on in launch order are fetched into L2 (whole sequences)
 };
 
 __device__ __forceinline__ bool rwait(uint64_t *bar, uint32_t parity, Shared *sh) {
@@ -157,13 +156,13 @@ __device__ __forceinline__ void split(float2 v, uint32_t &hi, uint32_t &lo) {
     const __half2 l = __floats2half2_rn(rest.x, rest.y);
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
-// P of 32 columns, times kPScale (which rides in the exponent, see tcf16::row_exp32); returns its sum.
-__device__ __forceinline__ float row_exp32(const uint32_t (&r)[32], float cs, float off, uint32_t (&ph)[16], uint32_t (&pl)[16]) {
+// P of sixteen of 32 columns, times kPScale (which rides in the exponent, see tcf16::row_exp32); returns its sum.
+__device__ __forceinline__ float row_exp16(const uint32_t (&r)[32], int first, float cs, float off, uint32_t (&ph)[8], uint32_t (&pl)[8]) {
     const float2 cs2 = make_float2(cs, cs), off2 = make_float2(-off, -off);
     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-        const float2 x = fma2(floats2(r[i], r[i + 1]), cs2, off2);
+    for (int i = 0; i < 16; i += 2) {
+        const float2 x = fma2(floats2(r[first + i], r[first + i + 1]), cs2, off2);
         const float2 pe = make_float2(ex2(x.x), ex2(x.y));
         sum = tcb::add2(sum, pe);
         split(pe, ph[i >> 1], pl[i >> 1]);
@@ -397,20 +396,6 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 }
             }
             __syncwarp();
-        } else if (PLANES && !PAGED && p.ahead > 0) {
-            // The query rows of the block that will start when one of the running ones ends, into L2: from DRAM, under load, they
-            // would be waited for.
-            const long long next = blockIdx.x + (long long)gridDim.x * blockIdx.y + p.ahead;
-            const int ny = (int)(next / gridDim.x), nslot = (int)(gridDim.x - 1 - next % gridDim.x);
-            if (ny < (int)gridDim.y) {
-                const int per = (int)(((long long)p.T * group + 127) / 128), nb = nslot / per, nf = (nslot - nb * per) * 128;
-                const int bytes = p.dim * 4;
-                for (int r = lane; r < 128 && nf + r < (long long)p.T * group; r += 32) {
-                    const int f = nf + r, i = f / group;
-                    const char *row = reinterpret_cast<const char *>(p.q + (((long long)nb * p.T + i) * p.n_heads + ny * group + (f - i * group)) * p.dim);
-                    for (int c = 0; c < bytes; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
-                }
-            }
         }
     } else if (!PLANES && warp >= 8) {
         // ------------------------------------------------------------------ keys and values: copied, scaled, split.  A group's
@@ -707,11 +692,14 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             const float off = ((m_ref == -INFINITY) ? 0.f : m_ref) - 7.0f;  // log2 kPScale: l and O are in P's units
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
-                uint32_t ph[16], pl[16];
                 if (kTwice) scores(c);
-                l += row_exp32(r, cs, off, ph, pl);
-                tmem_st16(cS + c, ph);
-                tmem_st16(cS + c + 16, pl);
+#pragma unroll
+                for (int i = 0; i < 32; i += 16) {
+                    uint32_t ph[8], pl[8];
+                    l += row_exp16(r, i, cs, off, ph, pl);
+                    tmem_st8(cS + c + i / 2, ph);
+                    tmem_st8(cS + c + 16 + i / 2, pl);
+                }
             }
             tmem_wait_st();
             tc_fence_before();
@@ -941,18 +929,22 @@ inline long long key_tiles(int keys, int dim) { return ((long long)keys + tile_k
 inline size_t planes_bytes(int batch, int keys, int n_kv_heads, int dim) {
     return (size_t)batch * n_kv_heads * (size_t)key_tiles(keys, dim) * ((size_t)4 * tile_keys(dim) * tc_tile_dim(dim) * 2 + sizeof(uint4)) + 512;
 }
-// Whether a launch of its own converts the key tiles: where that many row tiles visit each of them.
-inline bool converts_beforehand(long long visits) { return visits >= 4; }
+// Whether a launch of its own converts the key tiles, each of which so many row tiles visit.  Us, windows of whole sequences, converted
+// by the row tiles / beforehand: heads of 64, two visits 17.4 / 16.8, 55.2 / 48.0, three 34.0 / 32.2; of 128, two 24.9 / 27.4, 49.5 / 55.6, three
+// 44.3 / 41.0, 71.9 / 70.0; of 192, two 38.6 / 31.3; of 256, two 77 / 44, 40 / 22.  (Wide heads' row warps have no registers to spare
+// beside converting warps.)
+inline bool converts_beforehand(long long visits, int dim) { return visits >= (dim > 128 ? 1 : dim > 64 ? 3 : 2); }
 // The same for new rows over pages, as far as the host knows them -- the sequences have rows / batch each on average --, with the
 // bytes that it takes (0: none), and their bound over smaller calls.  Beyond kPlanesMost the rows convert for themselves.
 constexpr size_t kPlanesMost = (size_t)2 << 30;
 inline size_t paged_planes_bytes(int batch, int rows, int keys, int n_heads, int n_kv_heads, int dim) {
     const size_t bytes = planes_bytes(batch, keys, n_kv_heads, dim);
-    return converts_beforehand((long long)rows * (n_heads / n_kv_heads) / 128 / batch) && bytes <= kPlanesMost ? bytes : 0;
+    return converts_beforehand((long long)rows * (n_heads / n_kv_heads) / 128 / batch, dim) && bytes <= kPlanesMost ? bytes : 0;
 }
 inline size_t paged_planes_bound(int batch, int rows, int keys, int n_heads, int n_kv_heads, int dim) {
     const int group = n_heads / n_kv_heads;
-    const long long most = (long long)rows * group / 128 / 4;  // sequences of a call that converts beforehand, at most
+    long long most = (long long)rows * group / 128;  // sequences of a call that converts beforehand, at most
+    while (most > 0 && !converts_beforehand((long long)rows * group / 128 / most, dim)) --most;
     if (most < 1) return 0;
     const size_t bytes = planes_bytes(batch < most ? batch : (int)most, keys, n_kv_heads, dim);
     return bytes < kPlanesMost ? bytes : kPlanesMost;

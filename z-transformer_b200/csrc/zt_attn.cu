@@ -1155,8 +1155,10 @@ int zt_kv_append(float *k_cache, float *v_cache, int *n_keys, const float *k_new
 
 // ---- sliding windows over whole sequences ---------------------------------------------------------------------
 // A window, or sinks, as long as the sequence leave nothing out: the plain calls' case (window 0).
+// (nor do 2^30 keys, which no memory holds: positions, less a window and a tile, stay within 31 bits)
 static void normal_window(int T, int *window, int *sinks) {
-    if (*window == 0 || *window >= T || *sinks >= T) *window = 0, *sinks = 0;
+    constexpr int kAll = 1 << 30;
+    if (*window == 0 || *window >= T || *sinks >= T || *window >= kAll || *sinks >= kAll) *window = 0, *sinks = 0;
 }
 static int check_window(int window, int sinks) {
     if (window < 0) return refuse("a window of %d keys is refused (0: no window).", window);
@@ -1182,9 +1184,8 @@ int zt_attn_forward_window_batched(const float *q, const float *k, const float *
         p.scale_log2 = kLog2e / sqrtf((float)dim);
         // (a key tile is visited by the row tiles of the tokens that see one of its keys)
         const long long visits = ((long long)(window > 0 ? window : T) + 64) * (n_heads / n_kv_heads) / 128;
-        const StreamScratch scratch(tcr::converts_beforehand(visits) ? tcr::planes_bytes(batch, T, n_kv_heads, dim) : 0, (cudaStream_t)stream);
+        const StreamScratch scratch(tcr::converts_beforehand(visits, dim) ? tcr::planes_bytes(batch, T, n_kv_heads, dim) : 0, (cudaStream_t)stream);
         if (scratch.get()) tcr::place_planes(p, scratch.get(), T);
-        p.ahead = split_sm_count();
         return tcr::launch(p, (long long)batch * (((long long)T * (n_heads / n_kv_heads) + 127) / 128), (cudaStream_t)stream);
     }
     SimtFwdParams p{};
@@ -1264,7 +1265,7 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     if (d->cc_major != 10 || !tc_takes_dim(dim)) return refuse("paged attention needs an sm_100 device.");
     if (rows == 0) return 0;
     const int capacity = max_pages * page_size;
-    if (window == 0 || window >= capacity || sinks >= capacity) window = sinks = 0;
+    normal_window(capacity, &window, &sinks);
     if (!cu_rows) {
         // one row a sequence: split over the keys that it sees
         const int seen = window > 0 && sinks < capacity - window ? window + sinks : capacity;

@@ -267,6 +267,8 @@ def attention_forward_window(q, k, v, n_heads, n_kv_heads, head_dim, window, *, 
     B, T, (window, sinks) = _window_args(q, k, v, n_heads, n_kv_heads, head_dim, window, sinks)
     out = torch.empty_like(q)
     lse = torch.empty((B, T, n_heads), dtype=torch.float32, device=q.device) if want_lse else None
+    if T == 0:
+        return (out, lse) if want_lse else out
     with torch.cuda.device(q.device):
         rc = _lib.load().zt_attn_forward_window_batched(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None, B, T, n_heads,
