@@ -382,6 +382,25 @@ def test_captured_append_and_attention_replayed(zt, rows):
             near(lse[b * rows:(b + 1) * rows], ref_lse, i)
 
 
+def test_a_layer_decides_nothing_inside_a_capture(zt):
+    """Its counts and pages are the host's, which a replay does not pass."""
+    layer = zt.kv_cache.PagedLayer(8, 4, 64, 2, 4)
+    layer.append(*(rand(2, 64, seed=5) for _ in range(2)))
+    k, v, table, held = *(rand(2, 64, seed=6) for _ in range(2)), layer.table.clone(), (layer.free_pages(), list(layer._len))
+    x = torch.zeros(1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        for call in (lambda: layer.append(k, v), lambda: layer.append(k, v, [1, 1]), lambda: layer.reserve([5, 5]), lambda: layer.release(0),
+                     lambda: layer.trim(1)):
+            with pytest.raises(zt.device.ConfigRefused, match="captured"):
+                call()
+    graph.replay()
+    assert torch.equal(layer.table, table) and (layer.free_pages(), layer._len) == held and layer.len.tolist() == layer._len
+    layer.append(k, v)
+    assert layer.len.tolist() == [2, 2] == layer._len
+
+
 def test_offsets_beyond_31_bits(zt):
     """Pages whose elements lie past 2^31 from the pool's begin."""
     H, G, D, page = 4, 2, 128, 256

@@ -119,6 +119,10 @@ def test_pages_are_handed_out_once_and_all_or_nothing(zt):
         assert torch.equal(c.table, before) and c.free_pages() == 3
     c.reserve([3, 0])  # the second page has room
     assert c.free_pages() == 3
+    for counts in ([1], [1, 0, 1], [1, -1]):
+        with pytest.raises(zt.ops.DimensionMismatch):
+            c.reserve(counts)
+        assert c.free_pages() == 3
     c.reserve([11, 0])
     assert c.free_pages() == 1
     c._len = [16, 4]

@@ -139,7 +139,8 @@ def attn_step(q, layer: Layer, n_heads, n_kv_heads, head_dim, *, workspace: Deco
 class PagedLayer:
     """A layer's cache for `batch` sequences whose rows lie in pages of a common pool: k, v [n_pages, page_size, width], a table
     [batch, max_pages] of every sequence's pages (-1: none) and per-sequence len.  Which pages are whose is decided on the host, from
-    counts kept there; no step reads the device.  (kv_cache.Layer, src/kv_cache.zig:60-135, keeps n_ctx rows for each.)"""
+    counts kept there; no step reads the device.  So what changes them is refused inside a stream capture, whose replays would not: a graph
+    calls paged_append and attn_rows, over pages that reserve() has found beforehand.  (kv_cache.Layer, src/kv_cache.zig:60-135, keeps n_ctx rows for each.)"""
 
     def __init__(self, n_pages: int, page_size: int, width: int, batch: int, max_pages: int, device="cuda"):
         import torch
@@ -158,6 +159,11 @@ class PagedLayer:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _decides(self, what):
+        import torch
+        if self.k.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise ConfigRefused(f"kv_cache.PagedLayer.{what} decides on the host: a captured one would not when it is replayed")
+
     def _send_table(self):
         # (a copy that is ours alone: the host's table may change before the device has read it)
         self.table.copy_(self._table.clone(), non_blocking=True)
@@ -167,6 +173,7 @@ class PagedLayer:
         Full, writing nothing, when a sequence has no place left in the table or the pool no page.  Returns the rows' bounds
         cu_rows on the device (None for one row each), which attn_rows takes."""
         import torch
+        self._decides("append")
         given = [1] * self.batch if counts is None else [int(n) for n in counts]
         if len(given) != self.batch or min(given) < 0:
             raise DimensionMismatch("kv_cache.PagedLayer.append takes a count for every sequence")
@@ -188,7 +195,10 @@ class PagedLayer:
 
     def reserve(self, counts) -> None:
         """Pages for counts[b] more rows of each sequence, for all of them or (Full) for none."""
-        wanted = []
+        self._decides("reserve")
+        counts, wanted = list(counts), []
+        if len(counts) != self.batch:
+            raise DimensionMismatch("kv_cache.PagedLayer.reserve takes a count for every sequence")
         for b, n in enumerate(counts):
             if n < 0:
                 raise DimensionMismatch("kv_cache.PagedLayer.reserve")
@@ -205,6 +215,7 @@ class PagedLayer:
 
     def release(self, b: int) -> None:
         """The sequence ends: its pages go back to the pool and its place is empty again."""
+        self._decides("release")
         self._give_back(b, range(self.max_pages))
         self._len[b] = 0
         self.len[b].zero_()
@@ -213,6 +224,7 @@ class PagedLayer:
         """Gives back the pages that no coming query of `window` and `sinks` sees; returns how many."""
         if window < 1 or sinks < 0:
             raise DimensionMismatch("kv_cache.PagedLayer.trim")
+        self._decides("trim")
         before, ps = len(self._free), self.page_size
         for b, n in enumerate(self._len):
             # the next query stands at n and sees slots from n - window + 1 on
