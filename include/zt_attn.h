@@ -150,7 +150,8 @@ void zt_attn_set_verbose(int on);
  * earlier forms: up to head_dim 128 two kernels (dQ's, then dK/dV's) instead of the fused one --
  * slower by a quarter, and the only form whose dq is bit-reproducible run to run (the fused kernel
  * adds every key tile's share of dq in memory, in no fixed order: equal to rounding) -- and at 192
- * and 256 the scores kernel that loads every operand per tile.  Any other value selects 0.  For
+ * and 256 the scores kernel that loads every operand per tile (with a window at any width: the CUDA-core
+ * backward).  Any other value selects 0.  For
  * tests, for bisecting a parity failure, and for a caller that needs run-to-run identical dq;
  * returns the previous value. */
 int zt_attn_set_path(int path);
@@ -359,8 +360,15 @@ int zt_kv_append(float *k_cache, float *v_cache, int *n_keys, const float *k_new
  * position t sees key j where j <= t and (j > t - window or j < sinks).  window 0: no window, every key up to t.
  * Layouts, lse, delta, the gradients and the backward's workspace (zt_attn_backward_workspace_bytes, the same rules) are
  * those of zt_attn_forward_batched and zt_attn_backward_batched; out and lse handed to the backward are this forward's.
- * Key tiles that no query of a tile sees are not visited, so the time goes with the pairs that are seen.  The forward takes
- * no scratch.  Non-finite values: see "non-finite" in the notes on operands; a window's masks are masks in that sense.
+ * Key tiles that no query of a tile sees are not visited, so the time goes with the pairs that are seen.
+ * Scratch: where several tiles of rows visit the same keys the forward converts these beforehand, into scratch that is taken
+ * and given back in the order of the stream (see "Scratch" above; captured, it is a pair of memory nodes); where there is none
+ * to be had, it does without.  The backward takes the caller's workspace and nothing else.
+ * Non-finite values: in the forward a key or value that is not finite reaches the rows that see it, and no others; in the
+ * backward it may reach the gradients of its tiles, as in zt_attn_backward_batched.
+ * out and lse come out the same bit for bit from run to run, whether keys were converted beforehand or not aside; dq and, with
+ * sinks or above 128 columns, dk and dv are sums made in memory.  zt_attn_set_path(1) and (8) give the CUDA-core backward, whose
+ * gradients are bit for bit the same too.
  * Refusals: those of the batched calls; window < 0; sinks < 0.
  * No reference counterpart (src/attention.zig:60-153 sees the whole prefix). */
 int zt_attn_forward_window_batched(const float *q, const float *k, const float *v, float *out, float *lse, int batch,
@@ -394,8 +402,9 @@ int zt_attn_backward_window_batched(const float *q, const float *k, const float 
  * workspace: zt_attn_paged_workspace_bytes(batch, rows, max_keys, ...), 256-byte aligned, max_keys = max_pages * page_size; a call
  * with a smaller batch, fewer rows or a smaller table may use it too.  Calls that may overlap on the GPU take one each.
  * Refusals of both: batch outside 1 .. 65535; degenerate pages; a width (n_kv_heads * dim) that is no multiple of four, heads that
- * are no group, a dim outside 32 .. 256 or no multiple of four; rows < 0; cu_rows NULL and rows != batch; null pointers; tensors off a 16-byte boundary; window or sinks < 0; a
- * missing, short or misaligned workspace.  rows 0 is nothing to do.
+ * are no group, a dim outside 32 .. 256 or no multiple of four; rows < 0; cu_rows NULL and rows != batch; null pointers; tensors
+ * off a 16-byte boundary; window or sinks < 0; a missing, short or misaligned workspace.  rows 0 is nothing to do.
+ * zt_attn_set_path does not concern them: there is one form, and out and lse come out the same bit for bit from run to run.
  * No reference counterpart (src/kv_cache.zig:60-95 keeps a sequence's rows contiguous). */
 int zt_kv_append_paged(float *k_pages, float *v_pages, const int *table, int *n_keys, const float *k_new,
                        const float *v_new, const int *cu_rows, int *skipped, int batch, int rows, int n_pages,

@@ -2,7 +2,9 @@
 //
 // This file holds only argument checking and dispatch; the kernels live in
 // simt_kernels.cuh (CUDA-core, any admissible shape), decode_kernels.cuh
-// (bandwidth-bound split-K decode) and tc_fwd.cuh (tcgen05/TMEM forward).
+// (bandwidth-bound split-K decode, over pages too), paged_kernels.cuh (pages
+// and what is appended to them), tc_rows.cuh (tcgen05/TMEM: rows over pages,
+// windows), and the other tc_*.cuh (tcgen05/TMEM: whole sequences and gradients).
 // There is no CPU path: every launching entry point needs a CUDA device.
 //
 // The refusal order and wording follow the reference's launchers
