@@ -619,16 +619,20 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                 // a warp fetches its 32 half rows whole lines at a time (each thread its own half row took 10000 clocks)
                 constexpr int N = TD / 8;  // chunks of a half row
                 uint8_t *staged = smem + C::kQ + half * (TD * 2);
-#pragma unroll
+                // (wide heads' by asynchronous copies: a half row on its way would be 128 registers.  2 sequences of T 1024, window 256, 16/4 heads of
+                // 256, us: 60 / 55; of 64 columns 195 / 198)
+#pragma unroll(C::kWide ? 1 : N)
                 for (int i = 0; i < N; ++i) {
                     // (the row's place is known to its own thread; a division each cost 4000 clocks)
                     const int r = (i * 32 + lane) / N, col = half * (TD / 2) + (i * 32 + lane) % N * 4;
                     const long long row = __shfl_sync(0xffffffffu, rh, r);
                     const bool in = (warp & 3) * 32 + r < n_rows && col < p.dim;
-                    x[i] = in ? *reinterpret_cast<const float4 *>(p.q + row * p.dim + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (C::kWide) copy16_async(smem_u32(staged + ((warp & 3) * 32 + r) * C::RS + (i * 32 + lane) % N * 16), in ? p.q + row * p.dim + col : p.q, in);
+                    else x[i] = in ? *reinterpret_cast<const float4 *>(p.q + row * p.dim + col) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
+                if (C::kWide) copy_async_commit(), copy_async_wait<0>();
 #pragma unroll
-                for (int i = 0; i < N; ++i)
+                for (int i = 0; !C::kWide && i < N; ++i)
                     *reinterpret_cast<float4 *>(staged + ((warp & 3) * 32 + (i * 32 + lane) / N) * C::RS + (i * 32 + lane) % N * 16) = x[i];
                 __syncwarp();
 #pragma unroll
