@@ -844,11 +844,17 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const Params p, float *o
     w /= sum;
     for (int c = lane; c - lane < n4; c += 32) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i < p.parts; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            if (wi == 0.f || c >= n4) continue;
-            const float4 x = *(reinterpret_cast<const float4 *>(p.out + i * p.out_part + row * p.dim) + c);
-            a.x = fmaf(wi, x.x, a.x), a.y = fmaf(wi, x.y, a.y), a.z = fmaf(wi, x.z, a.z), a.w = fmaf(wi, x.w, a.w);
+        for (int i0 = 0; i0 < p.parts; i0 += 8) {  // (eight of the parts' chunks under way; beyond the last, a weight of zero)
+            float wi[8];
+            float4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                wi[i] = __shfl_sync(0xffffffffu, w, i0 + i);
+                x[i] = wi[i] != 0.f && c < n4 ? *(reinterpret_cast<const float4 *>(p.out + (i0 + i) * p.out_part + row * p.dim) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                a.x = fmaf(wi[i], x[i].x, a.x), a.y = fmaf(wi[i], x[i].y, a.y), a.z = fmaf(wi[i], x[i].z, a.z), a.w = fmaf(wi[i], x[i].w, a.w);
         }
         if (c < n4) *(reinterpret_cast<float4 *>(out + row * p.dim) + c) = a;
     }
@@ -1012,14 +1018,18 @@ inline int launch_join(const Params &p, float *out, float *lse, cudaStream_t str
 
 // Row tiles, at most, of `rows` new rows of `batch` sequences.
 inline long long row_slots(int batch, int rows, int group) { return (long long)rows * group / 128 + batch; }
-// How many parts the keys of a row tile are split into, where a CTA an SM is more than there are row tiles: a part keeps
-// 256 keys of the longest sequence at least.
-inline int row_parts(int batch, int rows, int max_seen, int n_heads, int n_kv_heads) {
+// How many parts the keys of a row tile are split into, where a CTA an SM is more than there are row tiles: a part keeps a key tile
+// of the longest sequence at least.  One sequence, us with the join, parts of 256 / 128 / 64 keys at least: 77 rows, the last of 1000, 32/8
+// heads of 128 25.8 / 20.9 / 20.9, 16 of 516 22.1 / 19.0 / 17.2, 30 of 630, 16/4 heads of 256 63 / 43.5 / 36.0; with a tile, and eight
+// parts' chunks under way in the join, 19.7, 15.1, 28.5.
+inline int converted_keys(int dim) { return dim > 128 ? Cfg<256, false>::BN : dim > 64 ? Cfg<128, false>::BN : Cfg<64, false>::BN; }
+inline int row_parts(int batch, int rows, int max_seen, int n_heads, int n_kv_heads, int dim) {
     const int group = n_heads / n_kv_heads;
     // (sequences share the rows: a tile each, and one more for every 128 rows)
     const long long full = (long long)rows * group, tiles = full / 128 + (full < batch ? full : batch);
     long long n = split_sm_count() / (tiles * n_kv_heads < 1 ? 1 : tiles * n_kv_heads);
-    if (n > max_seen / 256) n = max_seen / 256;
+    const long long key_tiles = ((long long)max_seen + converted_keys(dim) - 1) / converted_keys(dim);
+    if (n > key_tiles) n = key_tiles;
     return n < 2 ? 1 : (n > 32 ? 32 : (int)n);
 }
 // The most floats of the parts' rows, of a call of at most so many rows: what row_parts splits is at most a CTA's 128 rows an SM.

@@ -1287,7 +1287,7 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     p.seen = Seen{window, sinks};
     p.scale_log2 = kLog2e / sqrtf((float)dim);
     const long long keys = window > 0 ? (long long)window + sinks + rows : capacity;
-    p.parts = tcr::row_parts(batch, rows, (int)(keys < capacity ? keys : capacity), n_heads, n_kv_heads);
+    p.parts = tcr::row_parts(batch, rows, (int)(keys < capacity ? keys : capacity), n_heads, n_kv_heads, dim);
     const long long slots = tcr::row_slots(batch, rows, n_heads / n_kv_heads);
     const size_t planes = tcr::paged_planes_bytes(batch, rows, capacity, n_heads, n_kv_heads, dim);
     if (planes > 0) p.parts = 1, tcr::place_planes(p, static_cast<char *>(workspace) + kDecodeHeaderBytes, capacity);
