@@ -1021,7 +1021,8 @@ inline long long row_slots(int batch, int rows, int group) { return (long long)r
 // How many parts the keys of a row tile are split into, where a CTA an SM is more than there are row tiles: a part keeps a key tile
 // of the longest sequence at least.  One sequence, us with the join, parts of 256 / 128 / 64 keys at least: 77 rows, the last of 1000, 32/8
 // heads of 128 25.8 / 20.9 / 20.9, 16 of 516 22.1 / 19.0 / 17.2, 30 of 630, 16/4 heads of 256 63 / 43.5 / 36.0; with a tile, and eight
-// parts' chunks under way in the join, 19.7, 15.1, 28.5.
+// parts' chunks under way in the join, 19.7, 15.1, 28.5.  Keys converted beforehand, whole / in parts: 500 of 8500, 4/2 heads of 128 138 / 40,
+// 200 of 1700, 16/4 of 256 91 / 42, 200 of 4200, 32/8 of 128 99 / 76.
 inline int converted_keys(int dim) { return dim > 128 ? Cfg<256, false>::BN : dim > 64 ? Cfg<128, false>::BN : Cfg<64, false>::BN; }
 inline int row_parts(int batch, int rows, int max_seen, int n_heads, int n_kv_heads, int dim) {
     const int group = n_heads / n_kv_heads;

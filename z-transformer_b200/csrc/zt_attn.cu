@@ -1245,7 +1245,7 @@ size_t zt_attn_paged_workspace_bytes(int batch, int rows, int max_keys, int n_he
     if (batch < 1 || rows < 0 || max_keys < 1 || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || !zt_attn_dim_ok(dim) || dim % 4 != 0)
         return 0;
     const size_t parts = tcr::row_parts_bound(rows, n_heads, dim) * sizeof(float), planes = tcr::paged_planes_bound(batch, rows, max_keys, n_heads, n_kv_heads, dim);
-    return most(decode_bytes_bound(batch, max_keys, n_heads, n_kv_heads, dim), kDecodeHeaderBytes + most(parts, planes));
+    return most(decode_bytes_bound(batch, max_keys, n_heads, n_kv_heads, dim), kDecodeHeaderBytes + parts + planes);
 }
 
 int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, const int *n_keys,
@@ -1290,10 +1290,12 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     p.parts = tcr::row_parts(batch, rows, (int)(keys < capacity ? keys : capacity), n_heads, n_kv_heads, dim);
     const long long slots = tcr::row_slots(batch, rows, n_heads / n_kv_heads);
     const size_t planes = tcr::paged_planes_bytes(batch, rows, capacity, n_heads, n_kv_heads, dim);
-    if (planes > 0) p.parts = 1, tcr::place_planes(p, static_cast<char *>(workspace) + kDecodeHeaderBytes, capacity);
+    float *const parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + kDecodeHeaderBytes);  // (the planes lie behind them)
+    const long long pairs = (long long)rows * n_heads;
+    if (planes > 0) tcr::place_planes(p, parts + (p.parts > 1 ? p.parts * pairs * (dim + 1) : 0), capacity);
     if (p.parts == 1) return tcr::launch(p, slots, (cudaStream_t)stream);
-    p.lse_part = (long long)rows * n_heads, p.out_part = p.lse_part * dim;
-    p.out = reinterpret_cast<float *>(static_cast<char *>(workspace) + kDecodeHeaderBytes), p.lse = p.out + p.parts * p.out_part;
+    p.lse_part = pairs, p.out_part = pairs * dim;
+    p.out = parts, p.lse = p.out + p.parts * p.out_part;
     if (tcr::launch(p, slots, (cudaStream_t)stream)) return 1;
     return tcr::launch_join(p, out, lse, (cudaStream_t)stream);
 }
