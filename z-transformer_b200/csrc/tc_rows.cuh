@@ -824,6 +824,10 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
     if (warp == kIssuer) tmem_dealloc(tmem, 512);
 }
 
+// Whether the join reads part i of a row: of the parts that there are those with a weight (one that saw none of the row's keys wrote
+// nothing).  A row whose sum is NaN has NaN for every part's weight, so that the weight alone does not say which parts there are.
+__host__ __device__ inline bool join_reads(int i, int parts, float weight) { return i < parts && weight != 0.f; }
+
 // out, lse <- the parts'.  A warp per (row, head); a row that belongs to no sequence is left as it is.
 __global__ void __launch_bounds__(256) rows_join_kernel(const Params p, float *out, float *lse) {
     pdl_wait();
@@ -841,7 +845,7 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const Params p, float *o
     float w = (mine == -INFINITY) ? 0.f : ex2((mine - top) * kLog2e), sum = w;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    w /= sum;
+    w = lane < p.parts ? w / sum : 0.f;
     for (int c = lane; c - lane < n4; c += 32) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int i0 = 0; i0 < p.parts; i0 += 8) {  // (eight of the parts' chunks under way; beyond the last, a weight of zero)
@@ -850,7 +854,7 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const Params p, float *o
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 wi[i] = __shfl_sync(0xffffffffu, w, i0 + i);
-                x[i] = wi[i] != 0.f && c < n4 ? *(reinterpret_cast<const float4 *>(p.out + (i0 + i) * p.out_part + row * p.dim) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                x[i] = join_reads(i0 + i, p.parts, wi[i]) && c < n4 ? *(reinterpret_cast<const float4 *>(p.out + (i0 + i) * p.out_part + row * p.dim) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
