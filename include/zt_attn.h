@@ -388,8 +388,9 @@ int zt_attn_backward_window_batched(const float *q, const float *k, const float 
  *
  * zt_kv_append_paged copies the new rows into slots n_keys[b], n_keys[b] + 1, ... and advances n_keys[b].  A sequence
  * whose rows do not all have a place -- more than max_pages * page_size slots, a page number outside [0, n_pages), bounds
- * that do not ascend within [0, rows] -- is left untouched and counted in *skipped (device int, may be NULL).  No two
- * sequences of a call may append to the same page.
+ * that do not ascend within [0, rows] -- is left untouched and counted in *skipped (device int, may be NULL).  Each sequence
+ * is judged by its own two bounds: a row that several sequences' bounds hold, as only bounds that descend somewhere make
+ * it, is appended to each of them.  No two sequences of a call may append to the same page.
  *
  * zt_attn_paged: q, out [rows, n_heads*dim], lse [rows, n_heads] (may be NULL); the new rows, appended before, are the last of
  * their sequence: row cu_rows[b] + i stands at position n_keys[b] - (cu_rows[b + 1] - cu_rows[b]) + i and sees slot j where

@@ -84,42 +84,51 @@ __device__ __forceinline__ bool rows_fit(const AppendParams &p, const NewRows &r
         }
     return __syncthreads_and(fits);
 }
-// The sequence that row `row` belongs to, -1 if to none (called by whole blocks).
-__device__ __forceinline__ int sequence_of(const int *cu_rows, int batch, int row, int *found) {
-    if (!cu_rows) return row < batch ? row : -1;
-    if (threadIdx.x == 0) *found = -1;
+// The last of the first `batch` sequences that row `row` belongs to (-1: it belongs to none), and how many of them it belongs to: one, where
+// the bounds ascend (called by whole blocks).
+struct Owners {
+    int last, n;
+};
+__device__ __forceinline__ Owners owners_of(const int *cu_rows, int batch, int row, Owners *found) {
+    if (!cu_rows) return row < batch ? Owners{row, 1} : Owners{-1, 0};
+    if (threadIdx.x == 0) *found = Owners{-1, 0};
     __syncthreads();
     for (int b = threadIdx.x; b < batch; b += blockDim.x)
-        if (cu_rows[b] <= row && row < cu_rows[b + 1]) atomicMax(found, b);
+        if (cu_rows[b] <= row && row < cu_rows[b + 1]) atomicMax(&found->last, b), atomicAdd(&found->n, 1);
     __syncthreads();
     return *found;
 }
 
 // A block per new row.  Where a sequence has one row only (cu_rows null) its block also advances the count; elsewhere rows of
-// other blocks still read it, and advance_kernel follows.  Bound by a launch's latency: 2048 rows of 2 x 4 KB take 13 us and the counts 6.
+// other blocks still read it, and advance_kernel follows.  A row in the bounds of several sequences, which do not ascend then, goes to
+// each of them: their counts take it in.  Bound by a launch's latency: 2048 rows of 2 x 4 KB take 13 us and the counts 6.
 __global__ void __launch_bounds__(256) append_paged_kernel(const AppendParams p) {
-    __shared__ int found;
+    __shared__ Owners found;
     pdl_wait();
     pdl_launch();
     const int row = blockIdx.x;
-    const int b = sequence_of(p.cu_rows, p.batch, row, &found);
-    if (b < 0) return;
-    const NewRows r = new_rows(p.cu_rows, p.n_keys, b, p.rows, p.pg, false);
-    const bool fits = rows_fit(p, r, b);
-    if (fits) {
-        const long long at = p.pg.row(b, r.pos + (row - r.begin));
-        const float *ks = p.k_new + (long long)row * p.pg.width, *vs = p.v_new + (long long)row * p.pg.width;
-        float *kd = p.k_pages + at, *vd = p.v_pages + at;
-        for (int j = threadIdx.x * 4; j < p.pg.width; j += 1024) {
-            const float4 kx = *reinterpret_cast<const float4 *>(ks + j), vx = *reinterpret_cast<const float4 *>(vs + j);
-            *reinterpret_cast<float4 *>(kd + j) = kx, *reinterpret_cast<float4 *>(vd + j) = vx;
+    for (int below = p.batch, left = 1; left > 0;) {
+        const Owners own = owners_of(p.cu_rows, below, row, &found);
+        const int b = own.last;
+        if (b < 0) return;
+        const NewRows r = new_rows(p.cu_rows, p.n_keys, b, p.rows, p.pg, false);
+        const bool fits = rows_fit(p, r, b);  // (behind its barrier everyone has read `found`)
+        if (fits) {
+            const long long at = p.pg.row(b, r.pos + (row - r.begin));
+            const float *ks = p.k_new + (long long)row * p.pg.width, *vs = p.v_new + (long long)row * p.pg.width;
+            float *kd = p.k_pages + at, *vd = p.v_pages + at;
+            for (int j = threadIdx.x * 4; j < p.pg.width; j += 1024) {
+                const float4 kx = *reinterpret_cast<const float4 *>(ks + j), vx = *reinterpret_cast<const float4 *>(vs + j);
+                *reinterpret_cast<float4 *>(kd + j) = kx, *reinterpret_cast<float4 *>(vd + j) = vx;
+            }
         }
-    }
-    if (p.cu_rows) return;
-    __syncthreads();  // (every thread has read the count)
-    if (threadIdx.x == 0) {
-        if (fits) p.n_keys[b] = r.pos + 1;
-        else if (p.skipped) atomicAdd(p.skipped, 1);
+        left = own.n - 1, below = b;
+        if (p.cu_rows) continue;
+        __syncthreads();  // (every thread has read the count)
+        if (threadIdx.x == 0) {
+            if (fits) p.n_keys[b] = r.pos + 1;
+            else if (p.skipped) atomicAdd(p.skipped, 1);
+        }
     }
 }
 // A block per sequence, behind append_paged_kernel: the counts take in the rows that it wrote.
