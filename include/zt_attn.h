@@ -398,8 +398,9 @@ int zt_attn_backward_window_batched(const float *q, const float *k, const float 
  * read, nor are their places in the table, so a page that has left the window may be given to another sequence.  A row that
  * sees a slot on a page number outside [0, n_pages) is NaN.  A sequence whose counts contradict each other (fewer keys
  * than new rows, more than max_pages * page_size, bounds that do not ascend within [0, rows]) is not computed: its rows
- * are NaN, and zt_attn_decode_status(workspace) counts it after a synchronisation.  Rows that belong to nobody are left as
- * they are.  A non-finite key or value reaches the rows that see it, and no others.
+ * are NaN, and zt_attn_decode_status(workspace) counts it after a synchronisation.  Where bounds descend somewhere, the
+ * rows that several sequences' bounds hold, or that the descent passes over, are NaN too.  Rows that belong to nobody (below the
+ * least bound or from the greatest on) are left as they are.  A non-finite key or value reaches the rows that see it, and no others.
  * workspace: zt_attn_paged_workspace_bytes(batch, rows, max_keys, ...), 256-byte aligned, max_keys = max_pages * page_size; a call
  * with a smaller batch, fewer rows or a smaller table may use it too.  Calls that may overlap on the GPU take one each.
  * Refusals of both: batch outside 1 .. 65535; degenerate pages; a width (n_kv_heads * dim) that is no multiple of four, heads that

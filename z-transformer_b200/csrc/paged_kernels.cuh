@@ -64,6 +64,42 @@ __device__ __forceinline__ NewRows new_rows(const int *cu_rows, const int *n_key
     return r;
 }
 
+// The rows that sequence b answers for in an attention over pages, where a tile of 128 (row, head of a KV group) pairs belongs to one
+// sequence: [begin, end), of which it computes those in front of `upto` and makes the rest NaN.  Where the bounds ascend they are its own.
+// Elsewhere b answers from the greatest bound up to its own on (the first sequence from the least of all) to the greatest up to the
+// next one, and those behind the least bound to come are other sequences' as well, or only a descent passes over them: so every
+// row between the least and the greatest bound is one block's, and no row is computed that belongs to two sequences.
+struct RowSpan {
+    int b, begin, end, upto;  // b: -1 where the tile is nobody's
+};
+__host__ __device__ __forceinline__ int row_bound(const int *cu_rows, int rows, int i) {
+    const int c = cu_rows[i];
+    return c < 0 ? 0 : (c > rows ? rows : c);
+}
+// The first tile of a sequence that answers for rows from `begin` on: as many as it needs, or one more, lie in front of the next one's.
+__host__ __device__ __forceinline__ long long first_row_tile(int begin, int group, int b) { return (long long)begin * group / 128 + b; }
+// Whom tile `slot` belongs to, found one sequence after the other: for bounds that do not ascend.
+__host__ __device__ inline RowSpan row_span(const int *cu_rows, int batch, int rows, int group, int slot) {
+    RowSpan s{0, rows, 0, rows};
+    for (int i = 0; i <= batch; ++i) {
+        const int c = row_bound(cu_rows, rows, i);
+        s.begin = c < s.begin ? c : s.begin;
+    }
+    s.end = row_bound(cu_rows, rows, 0);
+    for (s.b = slot < first_row_tile(s.begin, group, 0) ? batch : 0; s.b < batch; ++s.b) {
+        const int c = row_bound(cu_rows, rows, s.b + 1);
+        s.end = c > s.end ? c : s.end;
+        if (slot < first_row_tile(s.end, group, s.b + 1)) break;
+        s.begin = s.end;
+    }
+    if (s.b == batch) return RowSpan{-1, 0, 0, 0};
+    for (int i = s.b + 1; i <= batch; ++i) {
+        const int c = row_bound(cu_rows, rows, i);
+        s.upto = c < s.upto ? c : s.upto;
+    }
+    return s;
+}
+
 // ---- append ----------------------------------------------------------------------------------------------------------
 
 struct AppendParams {

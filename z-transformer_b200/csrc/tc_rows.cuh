@@ -97,6 +97,7 @@ struct Shared {
     uint32_t tmem_base;
     volatile int abort;
     int found;
+    RowSpan span;
     float mk[16], mv[16];       // one over the scales of tiles j & 15 (powers of two)
     uint32_t odd[16][4];        // which values' rows of tile j & 15 hold something that is not finite
     alignas(16) uint32_t top[2][2][4];  // [group][unit & 1][warp]: the largest hi piece; or max |x|
@@ -202,8 +203,8 @@ struct Tiles {
 // The rows of a tile: flat rows [f0, f0 + 128) of a sequence's (token, head of the group) pairs.
 struct RowTile {
     int b, begin, count, pos;  // sequence; its first row in q, its rows, the first one's position
+    int computed;              // so many of its rows; the rest are NaN
     int f0;
-    bool bad;
 };
 
 template <int TD, bool PAGED, bool PLANES>
@@ -227,39 +228,52 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             bad = __reduce_add_sync(0xffffffffu, bad);
             if (lane == 0) *p.bad_count = bad;
         }
-        // Sequence b has the tiles from floor(cu_rows[b] group / 128) + b on: as many as it needs, or one more.
+        // Sequence b has the tiles from first_row_tile(cu_rows[b]) on: as many as it needs, or one more.
         if (threadIdx.x == 0) sh->found = -1;
         __syncthreads();
-        const auto clipped = [&](int i) { const int c = p.cu_rows[i]; return c < 0 ? 0 : (c > p.rows ? p.rows : c); };
-        const auto first_tile = [&](int i) { return (int)((long long)clipped(i) * group / 128) + i; };
-        for (int i = threadIdx.x; i < p.batch; i += kThreads)
-            if (first_tile(i) <= slot && slot < first_tile(i + 1)) atomicMax(&sh->found, i);
+        bool ascend = true;
+        for (int i = threadIdx.x; i < p.batch; i += kThreads) {
+            const int lo = row_bound(p.cu_rows, p.rows, i), hi = row_bound(p.cu_rows, p.rows, i + 1);
+            ascend &= lo <= hi;
+            if (first_row_tile(lo, group, i) <= slot && slot < first_row_tile(hi, group, i + 1)) atomicMax(&sh->found, i);
+        }
+        ascend = __syncthreads_and(ascend);
+        if (threadIdx.x == 0) {  // (one thread, into shared memory: what the others hold of it costs no registers)
+            const int b = sh->found;
+            if (!ascend) sh->span = row_span(p.cu_rows, p.batch, p.rows, group, slot);
+            else if (b < 0) sh->span.b = b;
+            else sh->span = RowSpan{b, row_bound(p.cu_rows, p.rows, b), row_bound(p.cu_rows, p.rows, b + 1), p.rows};
+        }
         __syncthreads();
-        t.b = sh->found;
+        const RowSpan span = sh->span;
+        t.b = span.b;
         if (t.b < 0) return;
         const NewRows r = new_rows(p.cu_rows, p.n_keys, t.b, p.rows, p.pg, true);
-        t.begin = clipped(t.b), t.count = clipped(t.b + 1) - t.begin, t.pos = r.pos, t.bad = r.bad;
-        t.f0 = (slot - first_tile(t.b)) * 128;
+        t.begin = span.begin, t.count = span.end - span.begin, t.pos = r.pos + (span.begin - r.begin);
+        t.computed = r.bad || span.upto < span.begin ? 0 : (span.upto < span.end ? span.upto : span.end) - span.begin;
+        t.f0 = (int)(slot - first_row_tile(span.begin, group, t.b)) * 128;
     } else {
         const int per = (int)(((long long)p.T * group + 127) / 128);
-        t.b = slot / per, t.begin = t.b * p.T, t.count = p.T, t.f0 = (slot - t.b * per) * 128;
+        t.b = slot / per, t.begin = t.b * p.T, t.count = t.computed = p.T, t.f0 = (slot - t.b * per) * 128;
     }
     const long long flat = (long long)t.count * group;
     if (t.f0 >= flat) return;
-    const int n_rows = flat - t.f0 < 128 ? (int)(flat - t.f0) : 128;
+    const auto of_tile = [&](long long end) { return end - t.f0 < 128 ? (int)(end - t.f0) : 128; };
+    const int n_rows = of_tile((long long)t.computed * group);
     // a row's place in q, out and lse
     const auto row_head = [&](int r) -> long long {
         const int f = t.f0 + r, i = f / group;
         return (long long)(t.begin + i) * p.n_heads + g * group + (f - i * group);
     };
-    if (PAGED && t.bad) {
+    if (PAGED && t.computed < t.count) {
         const float nan = __int_as_float(0x7fc00000);
-        for (int i = threadIdx.x; i < n_rows * p.dim; i += kThreads) {
+        const int nan0 = n_rows < 0 ? 0 : n_rows, nan1 = of_tile(flat);
+        for (int i = nan0 * p.dim + threadIdx.x; i < nan1 * p.dim; i += kThreads) {
             const int r = i / p.dim;
             p.out[part * p.out_part + row_head(r) * p.dim + (i - r * p.dim)] = nan;
         }
-        if (p.lse && threadIdx.x < n_rows) p.lse[part * p.lse_part + row_head(threadIdx.x)] = nan;
-        return;
+        if (p.lse && (int)threadIdx.x >= nan0 && (int)threadIdx.x < nan1) p.lse[part * p.lse_part + row_head(threadIdx.x)] = nan;
+        if (n_rows <= 0) return;
     }
     const int pos_first = t.pos + t.f0 / group, pos_last = t.pos + (t.f0 + n_rows - 1) / group;
     const Tiles tiles(p.seen, pos_first, pos_last, BN);
@@ -835,9 +849,9 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const Params p, float *o
     const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= p.lse_part) return;
     const int lane = threadIdx.x & 31, token = (int)(row / p.n_heads), n4 = p.dim >> 2;
-    bool owned = false;
-    for (int b = lane; b < p.batch; b += 32) owned |= p.cu_rows[b] <= token && token < p.cu_rows[b + 1];
-    if (!__any_sync(0xffffffffu, owned)) return;
+    bool from = false, to = false;  // (between the least bound and the greatest)
+    for (int b = lane; b <= p.batch; b += 32) from |= p.cu_rows[b] <= token, to |= p.cu_rows[b] > token;
+    if (!__any_sync(0xffffffffu, from) || !__any_sync(0xffffffffu, to)) return;
     const float mine = lane < p.parts ? p.lse[lane * p.lse_part + row] : -INFINITY;
     float top = mine;
 #pragma unroll
