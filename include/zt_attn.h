@@ -405,7 +405,8 @@ int zt_attn_backward_window_batched(const float *q, const float *k, const float 
  * with a smaller batch, fewer rows or a smaller table may use it too.  Calls that may overlap on the GPU take one each.
  * Refusals of both: batch outside 1 .. 65535; degenerate pages; a width (n_kv_heads * dim) that is no multiple of four, heads that
  * are no group, a dim outside 32 .. 256 or no multiple of four; rows < 0; cu_rows NULL and rows != batch; null pointers; tensors
- * off a 16-byte boundary; window or sinks < 0; a missing, short or misaligned workspace.  rows 0 is nothing to do.
+ * off a 16-byte boundary; window or sinks < 0; a missing, short or misaligned workspace.  rows 0 is nothing to do (and no
+ * sequence is counted).
  * zt_attn_set_path does not concern them: there is one form, and out and lse come out the same bit for bit from run to run.
  * No reference counterpart (src/kv_cache.zig:60-95 keeps a sequence's rows contiguous). */
 int zt_kv_append_paged(float *k_pages, float *v_pages, const int *table, int *n_keys, const float *k_new,

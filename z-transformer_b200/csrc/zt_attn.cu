@@ -1265,7 +1265,11 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     if (need_device()) return 1;
     const DeviceInfo *d = device_info();
     if (d->cc_major != 10 || !tc_takes_dim(dim)) return refuse("paged attention needs an sm_100 device.");
-    if (rows == 0) return 0;
+    if (rows == 0) {  // (no sequence is looked at: the count that zt_attn_decode_status reads is this call's all the same)
+        if (cudaMemsetAsync(workspace, 0, sizeof(int), (cudaStream_t)stream) == cudaSuccess) return 0;
+        cudaGetLastError();
+        return refuse("could not clear the workspace's count of sequences.");
+    }
     const int capacity = max_pages * page_size;
     normal_window(capacity, &window, &sinks);
     if (!cu_rows) {
