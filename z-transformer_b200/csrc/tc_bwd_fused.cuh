@@ -60,7 +60,7 @@ constexpr size_t kFusedSmem = 3 * (size_t)(128 * 128 * 2) + 2 * (size_t)(128 * 1
 constexpr int kFusedThreads = (kKvRowWarps + 3) * 32;
 // PARTS: the walk is split, or the blocks go tile by tile (tc_split.cuh).  A variant of its own: large launches are 1-2 % slower
 // with the code in it.
-// WIN: a window (BwdWindow); the blocks along y are window_block's.  A walk ends with the window, so the time goes with the pairs seen:
+// WIN: a window (BwdWindow); the blocks along x are window_block's, times the KV heads.  A walk ends with the window, so the time goes with the pairs seen:
 // T 8192, 32/8 heads of 128, window 1024 1290 us, 250 TFLOP/s of the pairs seen (two of a tile's nine visits are
 // half masked, and the accumulators are flushed four times as often as without a window).
 template <bool PARTS, bool PAD, bool WIN>
@@ -82,8 +82,10 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
 
     const int warp = threadIdx.x >> 5;
     // (the slowest index is the sequence, or the tile: see tile_by_tile)
-    const WindowBlock mine_of = WIN ? window_block(p.win, p.T, (int)blockIdx.y, BQ) : WindowBlock{};
-    const int g = blockIdx.x, kt = WIN ? mine_of.kt : PARTS && p.by_tile ? (int)blockIdx.z : (int)blockIdx.y, bp = PARTS && p.by_tile ? (int)blockIdx.y : (int)blockIdx.z;
+    // (a window's blocks lie along x with the KV heads: they may be more than y takes)
+    const int along = WIN ? (int)blockIdx.x / p.n_kv_heads : 0;
+    const WindowBlock mine_of = WIN ? window_block(p.win, p.T, along, BQ) : WindowBlock{};
+    const int g = WIN ? (int)blockIdx.x - along * p.n_kv_heads : (int)blockIdx.x, kt = WIN ? mine_of.kt : PARTS && p.by_tile ? (int)blockIdx.z : (int)blockIdx.y, bp = PARTS && p.by_tile ? (int)blockIdx.y : (int)blockIdx.z;
     const int b = PARTS ? bp / p.parts.n() : bp, part = PARTS ? bp - b * p.parts.n() : 0;
     const int group = p.n_heads / p.n_kv_heads;
     const int s0 = kt * 128;
@@ -658,8 +660,8 @@ inline int launch_bwd_fused(const CUtensorMap &k128, const CUtensorMap &v128, co
     const auto kernel = win ? (head_steps(p.dim_out) < 8 ? attn_bwd_fused_tc<false, true, true> : attn_bwd_fused_tc<false, false, true>)
                             : with_flags([](auto parts, auto pad) { return attn_bwd_fused_tc<parts.value, pad.value, false>; }, p.parts.n() > 1 || p.by_tile, head_steps(p.dim_out) < 8);
     if (optin_smem((const void *)kernel, kFusedSmem)) return 1;
-    const unsigned tiles = (unsigned)(win ? window_blocks(p.win, p.T, 64) : (p.T + 127) / 128), seqs = (unsigned)(p.batch * p.parts.n()), kv = (unsigned)p.n_kv_heads;
-    const dim3 grid = p.by_tile ? dim3(kv, seqs, tiles) : dim3(kv, tiles, seqs);
+    const unsigned tiles = (unsigned)((p.T + 127) / 128), seqs = (unsigned)(p.batch * p.parts.n()), kv = (unsigned)p.n_kv_heads;
+    const dim3 grid = win ? dim3((unsigned)window_grid(p.win, p.T, 64, p.n_kv_heads), 1, seqs) : p.by_tile ? dim3(kv, seqs, tiles) : dim3(kv, tiles, seqs);
     return launch_after("attn_bwd_fused_tc", kernel, grid, dim3(kFusedThreads), kFusedSmem, stream, 1, k128, v128, qs64, g64, p);
 }
 
@@ -726,6 +728,8 @@ inline int launch_bwd_tc(const float *q, const float *k, const float *v, const f
     if (fused) pass_fill(pa, dq, (long long)batch * T * n_heads * dim);
     const int rows = fused && td == 64 ? tcf::fused64_rows(T) : 64;  // of a query tile
     const BwdWindow win{window, sinks, (window + 127) / rows + 2};
+    if (window > 0 && window_grid(win, T, rows, n_kv_heads) > 0x7fffffffll)
+        return refuse("T %d with a window of %d keys and %d sinks is refused: its backward is more blocks than a launch holds.", T, window, sinks);
     if (window > 0 && zero_added_rows(win, dk, dv, batch, T, n_kv_heads * dim, rows, stream)) return 1;
     if (launch_pass_backward(pa, w, fused, !fused, qkv_planes_kept, stream)) return 1;
     BwdMaps m;

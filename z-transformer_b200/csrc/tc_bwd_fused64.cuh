@@ -86,8 +86,10 @@ __global__ void __launch_bounds__(kFused64Threads, 1)
 
     const int warp = threadIdx.x >> 5;
     // (the slowest index is the sequence, or the tile: see tile_by_tile)
-    const WindowBlock mine_of = WIN ? window_block(p.win, p.T, (int)blockIdx.y, BQ) : WindowBlock{};
-    const int g = blockIdx.x, kt = WIN ? mine_of.kt : PARTS && p.by_tile ? (int)blockIdx.z : (int)blockIdx.y, bp = PARTS && p.by_tile ? (int)blockIdx.y : (int)blockIdx.z;
+    // (a window's blocks lie along x with the KV heads: they may be more than y takes)
+    const int along = WIN ? (int)blockIdx.x / p.n_kv_heads : 0;
+    const WindowBlock mine_of = WIN ? window_block(p.win, p.T, along, BQ) : WindowBlock{};
+    const int g = WIN ? (int)blockIdx.x - along * p.n_kv_heads : (int)blockIdx.x, kt = WIN ? mine_of.kt : PARTS && p.by_tile ? (int)blockIdx.z : (int)blockIdx.y, bp = PARTS && p.by_tile ? (int)blockIdx.y : (int)blockIdx.z;
     const int b = PARTS ? bp / p.parts.n() : bp, part = PARTS ? bp - b * p.parts.n() : 0;
     const int group = p.n_heads / p.n_kv_heads;
     const int s0 = kt * 128;
@@ -624,8 +626,8 @@ inline int launch_bwd_fused64(const CUtensorMap &k128, const CUtensorMap &v128, 
                         : win ? (pad ? attn_bwd_fused64_tc<false, true, 128, true> : attn_bwd_fused64_tc<false, false, 128, true>)
                               : with_flags([](auto parts, auto pad) { return attn_bwd_fused64_tc<parts.value, pad.value, 128, false>; }, p.parts.n() > 1 || p.by_tile, pad);
     if (optin_smem((const void *)kernel, kFused64Smem)) return 1;
-    const unsigned tiles = (unsigned)(win ? window_blocks(p.win, p.T, fused64_rows(p.T)) : (p.T + 127) / 128), seqs = (unsigned)(p.batch * p.parts.n()), kv = (unsigned)p.n_kv_heads;
-    const dim3 grid = p.by_tile ? dim3(kv, seqs, tiles) : dim3(kv, tiles, seqs);
+    const unsigned tiles = (unsigned)((p.T + 127) / 128), seqs = (unsigned)(p.batch * p.parts.n()), kv = (unsigned)p.n_kv_heads;
+    const dim3 grid = win ? dim3((unsigned)window_grid(p.win, p.T, fused64_rows(p.T), p.n_kv_heads), 1, seqs) : p.by_tile ? dim3(kv, seqs, tiles) : dim3(kv, tiles, seqs);
     return launch_after("attn_bwd_fused64_tc", kernel, grid, dim3(kFused64Threads), kFused64Smem, stream, 1, k128, v128, qs128, g128, dqmap, dkmap, dvmap, p);
 }
 

@@ -130,11 +130,12 @@ __host__ __device__ inline WindowBlock window_block(const BwdWindow &w, int T, i
     const int near = near_tiles(w, T, i, rows);
     return WindowBlock{i, i * (128 / rows), near, i * 128 < w.sinks && near < all};
 }
-inline int window_blocks(const BwdWindow &w, int T, int rows) {
+// All of them, times the KV heads: what a launch has along x (with many sinks, more than the 65535 along y).
+inline long long window_grid(const BwdWindow &w, int T, int rows, int n_kv_heads) {
     const int all = (T + rows - 1) / rows;
-    int n = (T + 127) / 128;
+    long long n = (T + 127) / 128;
     for (int kt = 0; kt * 128 < T && kt * 128 < w.sinks; ++kt) n += (all - near_tiles(w, T, kt, rows) + w.far - 1) / w.far;
-    return n;
+    return n * n_kv_heads;
 }
 // Whether query t sees key j, of those at or before it.
 __host__ __device__ inline bool window_sees(const BwdWindow &w, int j, int t) { return j > t - w.window || j < w.sinks; }
