@@ -1,0 +1,27 @@
+"""How exact windows' outputs are, as the norm of the error over the norm of the result.  The tensor core adds with truncation: an addition to a
+sum that has grown loses half a step of 2^-23 on average, 2^-24 of the sum, which on its way is two thirds of what it becomes.  The small terms
+of the f16 pieces cost nothing while they come first."""
+import pytest
+import torch
+from test_gpu_window import backward64, make
+
+pytestmark = pytest.mark.gpu
+
+
+def errors(zt, B, T, H, G, D, window, sinks):
+    q, k, v, dout = make(B, T, H, G, D, seed=T + D)
+    ref = backward64(q, k, v, dout, H, G, D, window, sinks)
+    out, lse = zt.attention_forward_window(q, k, v, H, G, D, window, sinks=sinks, want_lse=True)
+    got = zt.attention_backward_window(q, k, v, out, lse, dout, H, G, D, window, sinks=sinks)
+    return {n: float((a.double() - b).norm() / b.norm()) for n, a, b in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *got), ref)}
+
+
+@pytest.mark.parametrize("B,T,H,G,D,window,sinks", [(4, 1000, 16, 4, 80, 200, 3), (1, 1000, 16, 4, 128, 300, 4), (1, 1000, 16, 4, 128, 1000, 0), (1, 2000, 8, 2, 128, 600, 4)])
+def test_heads_of_65_to_128_columns(zt, B, T, H, G, D, window, sinks):
+    """S: eight additions to a growing sum, 8 * 2^-24 * 2/3 = 3.2e-7 of S, which is near one, and so of a weight; out sums weighted values whose errors
+    are partly their common bias, which the softmax takes out: 4.2e-7 with a third for P's pieces and P V.  (With the small terms of the second half behind the
+    hi ones of the first it is sixteen additions, and 4.7e-7 to 5.5e-7 were measured.)  dv: 128 rows between two flushes, in two steps: 4 + 12 additions,
+    16 * 2^-24 * 2/3 = 6.4e-7.  Its weights' error is 3.2e-7 of S less the row's mean under P; where they count, by their squares, a score of variance one
+    stands at two and the mean at one: sqrt(1 + 1) * 3.2e-7 = 4.5e-7; pieces, 2^-23: 1.2e-7.  Together 1.21e-6 at most."""
+    e = errors(zt, B, T, H, G, D, window, sinks)
+    assert e["out"] <= 4.2e-7 and e["dv"] <= 1.25e-6, e

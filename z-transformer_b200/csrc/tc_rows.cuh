@@ -326,22 +326,25 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                     const uint32_t cS = C::cS + (j % SB) * BN;
                     const uint64_t bkh = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP)), bkl = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP + KP));
                     const uint64_t bql = desc_kmajor(ql_u32);
-// (64 columns at a time the two small terms first, while there is little to truncate.  The backward forms S in the same
-                    // order: where a softmax is saturated, what its dP and delta leave of each other is as good as the two S agree.)
+                    // (the two small terms first, while there is little to truncate: of the whole contraction, above 128 columns of 64 at a time, as
+                    // the backward has them.  It forms S in the same order: where a softmax is saturated, what its dP and delta leave of
+                    // each other is as good as the two S agree.  Of 128 columns, in two halves / at once: out's error at T 8192, window 1024
+                    // 5.5e-7 / 3.6e-7; a prompt of 16384, window 4096, 538 / 524 us.)
+                    constexpr int kSpan = C::kWide ? 4 : TD / 16;
 #pragma unroll
-                    for (int c = 0; c < TD / 64; ++c) {
+                    for (int c = 0; c < TD / 16; c += kSpan) {
 #pragma unroll
-                        for (int kk = 4 * c; kk < 4 * c + 4; ++kk) {
+                        for (int kk = c; kk < c + kSpan; ++kk) {
                             if (kk >= steps) break;
-                            const uint32_t bo = (uint32_t)(c * (BN * 128) + (kk & 3) * 32);
+                            const uint32_t bo = (uint32_t)((kk >> 2) * (BN * 128) + (kk & 3) * 32);
                             mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, desc_advance(bkl, bo), id_s, kk > 0);
-                            if (C::kWide) mma_ss_f16(tmem + cS, desc_advance(bql, (uint32_t)(c * (128 * 128) + (kk & 3) * 32)), desc_advance(bkh, bo), id_s, 1);
+                            if (C::kWide) mma_ss_f16(tmem + cS, desc_advance(bql, (uint32_t)((kk >> 2) * (128 * 128) + (kk & 3) * 32)), desc_advance(bkh, bo), id_s, 1);
                             else mma_ts_f16(tmem + cS, tmem + C::cQl + kk * 8, desc_advance(bkh, bo), id_s, 1);
                         }
 #pragma unroll
-                        for (int kk = 4 * c; kk < 4 * c + 4; ++kk) {
+                        for (int kk = c; kk < c + kSpan; ++kk) {
                             if (kk >= steps) break;
-                            mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, desc_advance(bkh, (uint32_t)(c * (BN * 128) + (kk & 3) * 32)), id_s, 1);
+                            mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, desc_advance(bkh, (uint32_t)((kk >> 2) * (BN * 128) + (kk & 3) * 32)), id_s, 1);
                         }
                     }
                     mma_commit(&sh->k_free[s]);
