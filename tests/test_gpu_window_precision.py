@@ -25,3 +25,12 @@ def test_heads_of_65_to_128_columns(zt, B, T, H, G, D, window, sinks):
     stands at two and the mean at one: sqrt(1 + 1) * 3.2e-7 = 4.5e-7; pieces, 2^-23: 1.2e-7.  Together 1.21e-6 at most."""
     e = errors(zt, B, T, H, G, D, window, sinks)
     assert e["out"] <= 4.2e-7 and e["dv"] <= 1.25e-6, e
+
+
+@pytest.mark.parametrize("B,T,H,G,D,window,sinks", [(1, 2000, 4, 2, 192, 900, 4), (1, 3000, 4, 2, 256, 1500, 4), (2, 1024, 16, 4, 256, 256, 0), (1, 700, 4, 1, 160, 300, 5)])
+def test_heads_above_128_columns(zt, B, T, H, G, D, window, sinks):
+    """dk and dv: pieces of 256 rows in four steps, 4 + 3 * 12 additions to a growing sum: 40 * 2^-24 * 2/3 = 1.6e-6.  S and dP: four blocks of 64
+    columns, as many additions, 1.6e-6 of each; of S what a weight notices is sqrt(2) times that (see above), 2.3e-6.  In quadrature: dk 3.2e-6,
+    dv 2.8e-6, dq (pieces of 512: 88 additions, 3.5e-6) 4.5e-6.  (Pieces of 1024: 192 additions, and 5.4e-6 to 6.1e-6 were measured.)"""
+    e = errors(zt, B, T, H, G, D, window, sinks)
+    assert e["dk"] <= 3.2e-6 and e["dv"] <= 2.8e-6 and e["dq"] <= 4.5e-6, e

@@ -52,6 +52,11 @@ constexpr int kScoreThreads = 10 * 32;  // TMA producer, MMA issuer, eight epilo
 constexpr int kResThreads = 18 * 32;    // TMA producer, MMA issuer, sixteen row warps
 constexpr int kTriThreads = 6 * 32;     // TMA producer, MMA issuer, four epilogue warps
 constexpr int kPiece = 1024;            // contraction depth of one unit of wide_products
+// Of a window, whose gradients are held to what plain f32 sums give (see kFlushRowsWin): of dQ, which wants to be stored, 512, of dK and dV
+// 256.  Error of dk / dv, us of wide_products at T 1024, window 256, 16/4 heads of 256: one piece of 1024, hi terms first 2.5e-6 / 1.9e-6 (66.8);
+// 384 2.4e-6 / 1.8e-6 (67.9), 256 2.2e-6 / 1.6e-6 (72.5; 74.5, and 3 for zeros, with dQ in pieces of 256 too), 128 1.8e-6 / 1.2e-6 (93.7); at T 3000,
+// window 1500 6.1e-6 / 5.7e-6, 2.9e-6 / 2.3e-6, 2.3e-6 / 1.7e-6, 1.9e-6 / 1.2e-6; plain f32 0.8e-6 and 1.3e-6.  What is left at 128 is S's and dP's.
+__host__ __device__ constexpr int win_depth(int which) { return which == 0 ? 512 : 256; }
 
 // Of a window, tiles of 128 on both sides: query tile m visits the key tiles that hold sinks and those from `low` on, numbered
 // through; key tile n is visited by the query tiles from n on up to `last`.
@@ -96,7 +101,8 @@ struct WideParams {
     int batch, T, Tp, n_heads, n_kv_heads;
     int dim_out, td;                   // the tensors' head_dim, the planes' (192 or 256)
     int unit0, unit_cap;               // the chunk: units (b * n_heads + h) from unit0; planes allocated for unit_cap
-    int units, pieces;                 // wide_products: units of the chunk, pieces of kPiece along one head's contraction
+    int units, pieces;                 // wide_products: units of the chunk, pieces (kPiece, win_depth) along one head's contraction
+    bool dq_whole;                     // a tile of dQ is one unit's
     bool in_turn;                      // and the order of its units (products_in_turn)
     BwdWindow win;                     // window 0: none
     float scale, scale_log2, p_scale;
@@ -641,6 +647,23 @@ __host__ __device__ inline bool products_in_turn(int pieces, int nt, int heads, 
     return pieces == 1 && 5LL * heads * drift >= 6LL * blocks;
 }
 
+// Pieces of the longest contraction.
+struct WidePieces {
+    int n, dq;  // of dQ alone
+};
+inline WidePieces wide_pieces(const BwdWindow &w, int Tp) {
+    const int all = (Tp + kPiece - 1) / kPiece;
+    if (w.window == 0) return WidePieces{all, all};
+    int keys = 0, rows = 0;
+    for (int m = 0; m < Tp / 128; ++m) {
+        const int k = WideTiles(w, m).n * 128, r = (wide_last(w, m, Tp / 128) + 1 - m) * 128;
+        keys = k > keys ? k : keys;
+        rows = r > rows ? r : rows;
+    }
+    const int dq = (keys + win_depth(0) - 1) / win_depth(0), dkv = (rows + win_depth(1) - 1) / win_depth(1);
+    return WidePieces{dq > dkv ? dq : dkv, dq};
+}
+
 struct TriUnit {
     int which, u, m0, b, h, k_begin, n_steps;  // which: 0 dQ, 1 dK, 2 dV; n_steps <= 0: nothing to do
     int sinks_end, skip;                       // (a window's dQ) from contraction index sinks_end on, `skip` keys are left out
@@ -664,8 +687,9 @@ struct TriUnit {
         const int ug = p.unit0 + u;
         b = ug / p.n_heads, h = ug - b * p.n_heads;
         m0 = m * 128;
-        k_begin = piece * kPiece;
-        int k_end = k_begin + kPiece;
+        const int depth = p.win.window > 0 ? win_depth(which) : kPiece;
+        k_begin = piece * depth;
+        int k_end = k_begin + depth;
         sinks_end = 0, skip = 0;
         if (p.win.window > 0) {  // pieces of what is visited
             if (which == 0) {
@@ -751,6 +775,7 @@ __global__ void __launch_bounds__(kTriThreads, 1)
         if (elect_one() && !sh->abort) {
             const uint32_t s_u32 = smem_u32(smem_raw);
             int it = 0, n = 0;  // steps, units with something to do
+            const bool win = p.win.window > 0;  // (the small terms of a step first)
             for (int i = blockIdx.x; i < n_units && !sh->abort; i += gridDim.x) {
                 const TriUnit w(p, i);
                 if (w.n_steps <= 0) continue;
@@ -771,10 +796,13 @@ __global__ void __launch_bounds__(kTriThreads, 1)
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint64_t dah = desc_advance(ah, kk * a_step), dal = desc_advance(al, kk * a_step);
                         const uint64_t dbh = desc_advance(bh, kk * 2048), dbl = desc_advance(bl, kk * 2048);
-                        mma_ss_f16(acc, dah, dbh, idesc, (s > 0 || kk > 0) ? 1 : 0);
-                        mma_ss_f16(acc, dah, dbl, idesc, 1);
+                        if (!win) mma_ss_f16(acc, dah, dbh, idesc, (s > 0 || kk > 0) ? 1 : 0);
+                        mma_ss_f16(acc, dah, dbl, idesc, (!win || s > 0 || kk > 0) ? 1 : 0);
                         mma_ss_f16(acc, dal, dbh, idesc, 1);
                     }
+                    if (win)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) mma_ss_f16(acc, desc_advance(ah, kk * a_step), desc_advance(bh, kk * 2048), idesc, 1);
                     mma_commit(&sh->freed[st]);
                 }
                 mma_commit(&sh->acc_full[n & 1]);
@@ -807,7 +835,7 @@ __global__ void __launch_bounds__(kTriThreads, 1)
             tc_fence_after();
             const long long ld = (long long)(w.which == 0 ? p.n_heads : p.n_kv_heads) * p.dim_out;
             const int row0 = t - j8;  // the first of this lane's eight rows
-            const bool whole = w.which == 0 && p.pieces == 1;
+            const bool whole = w.which == 0 && p.dq_whole;
             float *dst = (w.which == 0 ? p.dq : w.which == 1 ? p.dk : p.dv) + ((long long)w.b * p.T + row0) * ld +
                          (long long)(w.which == 0 ? w.h : g) * p.dim_out + 4 * j8;
 #pragma unroll 1
@@ -952,8 +980,8 @@ inline int launch_bwd_wide(const float *q, const float *k, const float *v, const
         pass_add(pa, k, batch, T, n_kv_heads, 1, w.part[1], w.amax_k, nullptr, w.k_planes);
         pass_add(pa, v, batch, T, n_kv_heads, 1, w.part[2], w.amax_v, w.vnmax, w.v_planes);
     }
-    const int pieces = (ww.Tp + kPiece - 1) / kPiece;
-    if (pieces > 1) pass_fill(pa, dq, (long long)batch * T * n_heads * dim);  // (a whole contraction's dQ is stored)
+    const WidePieces pieces = wide_pieces(BwdWindow{window, sinks, 0}, ww.Tp);
+    if (pieces.dq > 1) pass_fill(pa, dq, (long long)batch * T * n_heads * dim);  // (a whole contraction's dQ is stored)
     pass_fill(pa, dk, (long long)batch * T * n_kv_heads * dim);
     pass_fill(pa, dv, (long long)batch * T * n_kv_heads * dim);
     if (launch_pass_backward(pa, w, true, true, qkv_planes_kept, stream)) return 1;
@@ -990,7 +1018,7 @@ inline int launch_bwd_wide(const float *q, const float *k, const float *v, const
     p.dim_out = dim, p.td = td;
     p.unit_cap = cap;
     p.dq = dq, p.dk = dk, p.dv = dv;
-    p.pieces = pieces;
+    p.pieces = pieces.n, p.dq_whole = pieces.dq == 1;
     p.win = BwdWindow{window, sinks, 0};
     p.scale = 1.0f / sqrtf((float)dim), p.scale_log2 = kLog2e / sqrtf((float)dim);
     p.p_scale = ldexpf(1.0f, 10);
