@@ -606,8 +606,9 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             sync();
             const uint4 tops = *reinterpret_cast<const uint4 *>(sh->top[gi][u & 1]);
             top = max(max(tops.x, tops.y), max(tops.z, tops.w));
-            // The largest hi piece below 2^-3 (its lo piece would lose bits), or none, or not finite: with care.
-            const bool care = top < 0x3000u || top >= 0x7c00u || (is_k && hole);
+            // The largest hi piece below 2^4, or none, or not finite: with care.  What is taken as it is has the tile's largest at 2^4 at least, so
+            // that lo pieces, to the nearest 2^-24, are off by 2^-29 of it at most, and elements down to 2^-7 of it keep their 22 bits.
+            const bool care = top < 0x4c00u || top >= 0x7c00u || (is_k && hole);
             if (care) m = with_care(dst, is_k, j, u);
             if (ct == 0) {
                 (is_k ? sh->mk : sh->mv)[j & 15] = pow2_inverse(m);
