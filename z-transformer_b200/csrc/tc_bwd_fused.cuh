@@ -761,7 +761,7 @@ inline int launch_bwd_tc(const float *q, const float *k, const float *v, const f
     p.batch = batch, p.T = T, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads;
     p.dim_out = dim;
     p.rope_t = rope_t;
-    p.scale = 1.0f / sqrtf((float)dim), p.scale_log2 = kLog2e / sqrtf((float)dim);
+    p.scale = grad_scale(dim, window, sinks), p.scale_log2 = kLog2e / sqrtf((float)dim);
     // P in [0, 1] is split after a multiplication by 2^10 (its low piece then stays a normal f16 down to p ~ 2^-14).
     // dS is scaled inside the kernels (see "The scale of dS" in tc_bwd.cuh and the head of this file).
     p.p_scale = ldexpf(1.0f, 10);

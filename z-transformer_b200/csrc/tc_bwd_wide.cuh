@@ -1020,7 +1020,7 @@ inline int launch_bwd_wide(const float *q, const float *k, const float *v, const
     p.dq = dq, p.dk = dk, p.dv = dv;
     p.pieces = pieces.n, p.dq_whole = pieces.dq == 1;
     p.win = BwdWindow{window, sinks, 0};
-    p.scale = 1.0f / sqrtf((float)dim), p.scale_log2 = kLog2e / sqrtf((float)dim);
+    p.scale = grad_scale(dim, window, sinks), p.scale_log2 = kLog2e / sqrtf((float)dim);
     p.p_scale = ldexpf(1.0f, 10);
     g_last_path = "tcgen05";
     const int nt = Tp / 128;

@@ -335,7 +335,7 @@ static int backward_impl(const float *q, const float *k, const float *v, const f
     p.q_batch_stride = (long long)T * n_heads * dim;
     p.kv_batch_stride = (long long)T * n_kv_heads * dim;
     p.lse_batch_stride = (long long)T * n_heads;
-    p.scale = 1.0f / sqrtf((float)dim);
+    p.scale = grad_scale(dim, window, sinks);
     p.scale_log2 = kLog2e / sqrtf((float)dim);
     p.window = window, p.sinks = sinks;
     return launch_bwd_simt(p, batch, stream);

@@ -129,6 +129,10 @@ inline const DeviceInfo *device_info() {
     return &d;
 }
 
+// The factor of dq and dk behind dS.  With a window of one key and no sinks a query sees itself alone: P is one, delta is dP, dS is zero and so are
+// dq and dk, of which the arithmetic would leave the rounding of dP and delta.
+inline float grad_scale(int dim, int window, int sinks) { return window == 1 && sinks == 0 ? 0.f : 1.0f / sqrtf((float)dim); }
+
 // Function attributes are set once per (kernel, device, value): asking the driver on every launch costs more host time
 // than the launch's own bookkeeping.  Returns whether `value` is already known to hold.
 inline bool attribute_known(const void *fn, int attr, size_t value, bool record) {
