@@ -140,7 +140,7 @@ class PagedLayer:
     """A layer's cache for `batch` sequences whose rows lie in pages of a common pool: k, v [n_pages, page_size, width], a table
     [batch, max_pages] of every sequence's pages (-1: none) and per-sequence len.  Which pages are whose is decided on the host, from
     counts kept there; no step reads the device.  So what changes them is refused inside a stream capture, whose replays would not: a graph
-    calls paged_append and attn_rows, over pages that reserve() has found beforehand.  (kv_cache.Layer, src/kv_cache.zig:60-135, keeps n_ctx rows for each.)"""
+    calls paged_append and attn_rows, over pages that reserve() has found beforehand, and set_lens() says afterwards how far it went.  (kv_cache.Layer, src/kv_cache.zig:60-135, keeps n_ctx rows for each.)"""
 
     def __init__(self, n_pages: int, page_size: int, width: int, batch: int, max_pages: int, device="cuda"):
         import torch
@@ -192,6 +192,22 @@ class PagedLayer:
         paged_append(self.k, self.v, self.table, self.len, k_rows, v_rows, cu_rows=cu, skipped=self.skipped)
         self._len = [n + m for n, m in zip(self._len, given)]
         return cu
+
+    def set_lens(self, lens) -> None:
+        """Start from given per-sequence fill counts: rows were written directly, or by the replays of a captured paged_append, of which the host's
+        counts know nothing.  Refuses a count whose rows lie beyond the table or, behind those that were known, on no page."""
+        import torch
+        self._decides("set_lens")
+        lens = torch.as_tensor(lens, dtype=torch.int32)
+        given = lens.tolist() if lens.shape == (self.batch,) else [-1]
+        if min(given) < 0 or max(given) > self.max_pages * self.page_size:
+            raise DimensionMismatch("kv_cache.PagedLayer.set_lens")
+        for b, n in enumerate(given):
+            new = self._table[b, self._len[b] // self.page_size:-(-n // self.page_size)]
+            if n > self._len[b] and bool((new < 0).any()):
+                raise DimensionMismatch("kv_cache.PagedLayer.set_lens: rows on no page")
+        self._len = given
+        self.len.copy_(torch.tensor(given, dtype=torch.int32), non_blocking=True)  # (host memory of its own: see Layer.set_lens)
 
     def reserve(self, counts) -> None:
         """Pages for counts[b] more rows of each sequence, for all of them or (Full) for none."""
