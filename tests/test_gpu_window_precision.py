@@ -1,8 +1,11 @@
 """How exact windows' outputs are, as the norm of the error over the norm of the result.  The tensor core adds with truncation: an addition to a
 sum that has grown loses half a step of 2^-23 on average, 2^-24 of the sum, which on its way is two thirds of what it becomes.  The small terms
 of the f16 pieces cost nothing while they come first."""
+import math
+
 import pytest
 import torch
+from test_gpu_paged import Case
 from test_gpu_window import backward64, make
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +37,17 @@ def test_heads_above_128_columns(zt, B, T, H, G, D, window, sinks):
     dv 2.8e-6, dq (pieces of 512: 88 additions, 3.5e-6) 4.5e-6.  (Pieces of 1024: 192 additions, and 5.4e-6 to 6.1e-6 were measured.)"""
     e = errors(zt, B, T, H, G, D, window, sinks)
     assert e["dk"] <= 3.2e-6 and e["dv"] <= 2.8e-6 and e["dq"] <= 4.5e-6, e
+
+
+@pytest.mark.parametrize("H,G,D", [(8, 2, 256), (8, 2, 192), (16, 4, 128), (8, 2, 160)])
+@pytest.mark.parametrize("rows", [25, 300])
+def test_rows_over_pages(zt, H, G, D, rows):
+    """S: as many additions to a growing sum as the head has sixteens of columns, n * 2^-24 * 2/3 of S.  What out notices of it is S less the row's mean
+    under P, where weights count by their squares: sqrt(2) of that (see above), 9.0e-7 at 256.  In quadrature with 4.8e-7: P V, four additions a tile, 1.6e-7;
+    P's pieces 1.2e-7; the tiles' sums in registers 1e-7; the exponent, a number near eight rounded at 2^-24 of itself, 4.2e-7.  (With the small terms of
+    64 columns behind the hi ones of the last 8.4e-7 at 160, 9.1e-7 at 192 and 1.2e-6 at 256 were measured.)"""
+    c = Case([rows], [1500], H, G, D, 16, seed=D)
+    out, _ = c.call(zt)
+    ref = c.reference(0)[0]
+    bound = math.hypot(math.sqrt(2) * D / 16 * 2.0**-24 * 2 / 3, 4.8e-7)
+    assert float((out.double() - ref).norm() / ref.norm()) <= bound

@@ -326,11 +326,12 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                     const uint32_t cS = C::cS + (j % SB) * BN;
                     const uint64_t bkh = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP)), bkl = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP + KP));
                     const uint64_t bql = desc_kmajor(ql_u32);
-                    // (the two small terms first, while there is little to truncate: of the whole contraction, above 128 columns of 64 at a time, as
-                    // the backward has them.  It forms S in the same order: where a softmax is saturated, what its dP and delta leave of
-                    // each other is as good as the two S agree.  Of 128 columns, in two halves / at once: out's error at T 8192, window 1024
-                    // 5.5e-7 / 3.6e-7; a prompt of 16384, window 4096, 538 / 524 us.)
-                    constexpr int kSpan = C::kWide ? 4 : TD / 16;
+                    // (the two small terms first, while there is little to truncate: of the whole contraction, but above 128 columns of whole
+                    // sequences of 64 at a time, as the backward has them.  It forms S in the same order: where a softmax is saturated, what its
+                    // dP and delta leave of each other is as good as the two S agree.  Of 128 columns, in two halves / at once: out's error at
+                    // T 8192, window 1024 5.5e-7 / 3.6e-7; a prompt of 16384, window 4096, 538 / 524 us.  Of 256 over pages, in four / at once:
+                    // 1.2e-6 / 6.5e-7.  Whole sequences of 256 at once: out's 9.8e-7 / 4.8e-7, but dk's 2.2e-6 / 2.5e-6.)
+                    constexpr int kSpan = C::kWide && !PAGED ? 4 : TD / 16;
 #pragma unroll
                     for (int c = 0; c < TD / 16; c += kSpan) {
 #pragma unroll
