@@ -9,8 +9,8 @@
 //           same keys, so a short chunk fills a tile, and a window of W keys costs a tile W + 128 / group keys and not W + 128.
 //   keys    come as they are.  Converting warps copy a tile's rows into shared memory (cp.async, row by row: each has its
 //           page) and write the pieces, scaled by a power of two of the tile's own, as the operand tiles that the MMAs
-//           read.  No launch before this one converts anything and nothing is kept in memory.  The power of two is the one that
-//           the tile before would have had, so that a row is converted as soon as it is there; where it turns out to be off by
+//           read: in that form nothing is converted before the launch and nothing is kept in memory.  The power of two is the one
+//           that the tile before would have had, so that a row is converted as soon as it is there; where it turns out to be off by
 //           more than the pieces can bear, or something is not finite, the tile is converted again with care.
 //   scales  K's goes into the tile's scores; V's, and the reference maximum of the tile's exponentials, into the factor with
 //           which the row threads add the tile's P V to the row: O leaves TMEM after every tile and is summed in registers,
@@ -27,8 +27,8 @@
 // come by bulk copies, and the converting warps' place is taken by row warps, of which some make P and others sum.
 // TMEM: Q hi, Q lo (above 128 columns in shared memory), one O buffer (up to 64 columns two), four S/P buffers (of tiles of 128
 // keys two): S runs ahead of the rows, so that a set finds the next tile's when it has made P of one and summed those before.
-// What bounds it.  Keys converted beforehand: the products.  Four chunks of 512 rows over 8192 keys of 32/8 heads of 128 605 us, 81 % of
-// what three f16 products of every seen pair take at the rate of a large bf16 GEMM; a prompt of 16384 with a window of 4096 550 us (81 %).
+// What bounds it.  Keys converted beforehand: the products.  Four chunks of 512 rows over 8192 keys of 32/8 heads of 128 581 us, 84 % of
+// what three f16 products of every seen pair take at the rate of a large bf16 GEMM; a prompt of 16384 with a window of 4096 520 us (86 %).
 // A tile's rows need some 19000 clocks besides, one CTA an SM: 13000 until the first product (the query rows' way in 8000 of them), 3500
 // for the rows' way out; at T 8192, 32/8 heads, window 1024 that is why the 380 us are 1.6 times their products'.  Keys that
 // the CTA converts: the converting warps' instructions and their waits for rows: 32 ragged sequences, window 2048, 16/16 heads of 64,
@@ -460,8 +460,9 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
             const bool hole = PAGED && __any_sync(0xffffffffu, at == kNoPage);
             if (lane == 0) sh->holes[place(j)][cw] = hole;
         };
-        // Sixteen rows by eight threads each, a thread the chunks (ct & 7) + 8 i of its row: one look-up and one address a row, whole 128-byte lines a row, and sixteen threads write eight bytes each of two rows whose chunks lie in
-        // different banks (rows four apart, see the swizzle).
+        // Sixteen rows by eight threads each, a thread the chunks (ct & 7) + 8 i of its row: one look-up and one address a row, whole
+        // 128-byte lines a row, and sixteen threads write eight bytes each of two rows whose chunks lie in different banks (rows four
+        // apart, see the swizzle).
         const int pr = (ct >> 3 & 1) << 2 | (ct >> 4 & 3) | (ct >> 6) << 3, pc = ct & 7;
         constexpr int CPT = TD / 32;                     // chunks that a thread has of a row
         const int my_chunks = (p.dim / 4 - pc + 7) / 8;  // of the head's columns; the rest of the tile's are zeros
