@@ -34,6 +34,10 @@ def test_pages_behind_a_window_may_be_gone(zt):
     assert c.trim(window=3) == 2  # slots 10 and 11 are seen and 12: pages 0 and 1 go
     c.set_lens([15, 0])
     assert c._len == [15, 0]
+    with pytest.raises(zt.ops.DimensionMismatch):  # slots 4 and 5 went with their page, and 6 would share a new one with them
+        c.set_lens([6, 0])
+    c.set_lens([9, 0])
+    assert c._len == [9, 0]
 
 
 @pytest.mark.gpu

@@ -204,7 +204,9 @@ class PagedLayer:
             raise DimensionMismatch("kv_cache.PagedLayer.set_lens")
         for b, n in enumerate(given):
             new = self._table[b, self._len[b] // self.page_size:-(-n // self.page_size)]
-            if n > self._len[b] and bool((new < 0).any()):
+            # (going back, the page that the next row shares with older ones has to be there still)
+            shared = n % self.page_size > 0 and int(self._table[b, n // self.page_size]) < 0
+            if shared or n > self._len[b] and bool((new < 0).any()):
                 raise DimensionMismatch("kv_cache.PagedLayer.set_lens: rows on no page")
         self._len = given
         self.len.copy_(torch.tensor(given, dtype=torch.int32), non_blocking=True)  # (host memory of its own: see Layer.set_lens)
