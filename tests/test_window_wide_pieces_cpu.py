@@ -30,7 +30,7 @@ int main() {
         for (int i = 0; i < 3 * nt * p.units * p.pieces; ++i) {
             const tcw::TriUnit w(p, i);
             if (w.n_steps <= 0) continue;
-            if (w.n_steps * 64 > tcw::win_depth(w.which)) ++bad;
+            if (w.n_steps * 64 > tcw::kPiece) ++bad;
             const size_t of = ((size_t)w.which * 2 + w.u) * nt + w.m0 / 128;
             ++units[of];
             for (int s = 0; s < w.n_steps; ++s) {

@@ -51,12 +51,13 @@ constexpr int kSB = 4 * kTB;       // a stage: A hi, A lo, B hi, B lo
 constexpr int kScoreThreads = 10 * 32;  // TMA producer, MMA issuer, eight epilogue warps
 constexpr int kResThreads = 18 * 32;    // TMA producer, MMA issuer, sixteen row warps
 constexpr int kTriThreads = 6 * 32;     // TMA producer, MMA issuer, four epilogue warps
+constexpr int kTriThreadsWin = 10 * 32; // (a window's: eight)
+// Of a window, whose gradients are held to what plain f32 sums give (see kFlushRowsWin): an accumulator takes 128 contraction rows, two steps, and the
+// epilogue warps add them up in registers, with rounding.  Error of dq / dk / dv in 1e-7, us of wide_products at T 1024, window 256, 16/4 heads of
+// 256: one accumulator a unit, hi terms first 21 / 25 / 19 (66.8), with the scores' small terms first pieces of 256 rows added in memory 12 / 14 / 12 (71.0), 128 rows
+// 9 / 10 / 8 (68.6), 64 rows 8 / 8 / 6 (77.3); T 3000, window 1500 30 / 61 / 57, 16 / 15 / 13, 10 / 10 / 8, 8 / 9 / 6; plain f32 6 / 8 / 8 and 7 / 13 / 13.
+constexpr int kWinSteps = 2;
 constexpr int kPiece = 1024;            // contraction depth of one unit of wide_products
-// Of a window, whose gradients are held to what plain f32 sums give (see kFlushRowsWin): of dQ, which wants to be stored, 512, of dK and dV
-// 256.  Error of dk / dv, us of wide_products at T 1024, window 256, 16/4 heads of 256: one piece of 1024, hi terms first 2.5e-6 / 1.9e-6 (66.8);
-// 384 2.4e-6 / 1.8e-6 (67.9), 256 2.2e-6 / 1.6e-6 (72.5; 74.5, and 3 for zeros, with dQ in pieces of 256 too), 128 1.8e-6 / 1.2e-6 (93.7); at T 3000,
-// window 1500 6.1e-6 / 5.7e-6, 2.9e-6 / 2.3e-6, 2.3e-6 / 1.7e-6, 1.9e-6 / 1.2e-6; plain f32 0.8e-6 and 1.3e-6.  What is left at 128 is S's and dP's.
-__host__ __device__ constexpr int win_depth(int which) { return which == 0 ? 512 : 256; }
 
 // Of a window, tiles of 128 on both sides: query tile m visits the key tiles that hold sinks and those from `low` on, numbered
 // through; key tile n is visited by the query tiles from n on up to `last`.
@@ -101,7 +102,7 @@ struct WideParams {
     int batch, T, Tp, n_heads, n_kv_heads;
     int dim_out, td;                   // the tensors' head_dim, the planes' (192 or 256)
     int unit0, unit_cap;               // the chunk: units (b * n_heads + h) from unit0; planes allocated for unit_cap
-    int units, pieces;                 // wide_products: units of the chunk, pieces (kPiece, win_depth) along one head's contraction
+    int units, pieces;                 // wide_products: units of the chunk, pieces of kPiece along one head's contraction
     bool dq_whole;                     // a tile of dQ is one unit's
     bool in_turn;                      // and the order of its units (products_in_turn)
     BwdWindow win;                     // window 0: none
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1)
 // 32/8 of 256 623 -> 606 (the planes' DRAM traffic next).
 // ---------------------------------------------------------------------------------------------------
 struct ResShared {
-    uint64_t full[4], freed[4], qh_full, ql_full, a_ready, s_full, s_free, dp_full, dp_free;
+    uint64_t full[5], freed[5], full_lo[3], freed_lo[3], qh_full, ql_full, a_ready, s_full, s_free, dp_full, dp_free;
     uint32_t tmem_base;
     volatile int abort;
 };
@@ -352,17 +353,26 @@ __device__ __forceinline__ void store_rows_quad(__half *dst, long long ld, const
 // Slots of the ring of K and V blocks: what shared memory leaves beside the lo planes of Q and dO.
 template <int D>
 __host__ __device__ constexpr int res_slots() { return D == 256 ? 3 : 4; }
+// A window's, whose scores want the small terms of the whole contraction first: its K and V blocks are needed twice, the hi planes until the end,
+// the lo planes once, so they have rings of their own in the same place.  T 78, heads of 256, in 1e-7, 64 columns at a time / so: out's error 7.4 / 3.6,
+// dq's 14 / 7.0, dk's 15 / 7.5; us of the scores at T 1024, window 256, 16/4 heads 58.7 / 67.6: between two contractions the first hi plane is waited for.
+template <int D>
+__host__ __device__ constexpr int res_hi_slots() { return D == 256 ? 4 : 5; }
+template <int D>
+__host__ __device__ constexpr int res_lo_slots() { return 2 * res_slots<D>() - res_hi_slots<D>(); }
 
 template <int D, bool WIN>
 __global__ void __launch_bounds__(kResThreads, 1)
     bwd_wide_scores_res(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap gmap, const __grid_constant__ CUtensorMap vmap, const WideParams p) {
-    constexpr int NB = D / 64, NR = res_slots<D>();
+    constexpr int NB = D / 64, NR = res_slots<D>(), NH = res_hi_slots<D>(), NL = res_lo_slots<D>();
+    static_assert(NH >= NB && NH <= 5 && NL >= 1 && NL <= 3, "a contraction's hi planes are all there; ResShared");
     constexpr int BT = 128 * 64 * 2;          // one 64-column block of a 128-row tile, one plane: 16 KB
     constexpr int cQh = 0, cGh = 128, cS = 256, cDP = 384;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *sQl = smem_raw, *sGl = smem_raw + NB * BT;   // lo planes of Q and dO: NB blocks each (hi planes first, staged)
-    uint8_t *ring = smem_raw + 2 * NB * BT;                   // slot s: block hi, block lo at ring + s * 2 BT + {0, 1} BT
+    uint8_t *ring = smem_raw + 2 * NB * BT;                   // slot s: block hi, block lo at ring + s * 2 BT + {0, 1} BT (WIN: NH hi ones, NL lo ones)
+    uint8_t *ring_lo = ring + NH * BT;
     ResShared *sh = reinterpret_cast<ResShared *>(ring + NR * 2 * BT);
     const int warp = threadIdx.x >> 5;
     // launch order (x fastest): every unit's last query tile, then every unit's last but one, ...: the longest
@@ -379,7 +389,8 @@ __global__ void __launch_bounds__(kResThreads, 1)
     const int n_blocks = 2 * NB * n_tiles;  // per tile: K's blocks, then V's
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < NR; ++i) mbar_init(&sh->full[i], 1), mbar_init(&sh->freed[i], 1);
+        for (int i = 0; i < (WIN ? NH : NR); ++i) mbar_init(&sh->full[i], 1), mbar_init(&sh->freed[i], 1);
+        for (int i = 0; WIN && i < NL; ++i) mbar_init(&sh->full_lo[i], 1), mbar_init(&sh->freed_lo[i], 1);
         mbar_init(&sh->qh_full, 1), mbar_init(&sh->ql_full, 1);
         mbar_init(&sh->a_ready, 16);
         mbar_init(&sh->s_full, 1), mbar_init(&sh->s_free, 16);
@@ -408,6 +419,19 @@ __global__ void __launch_bounds__(kResThreads, 1)
             }
             int issued = 0;
             bool live = true;
+            // (WIN) load i is the lo plane (even) or the hi plane of block i / 2
+            auto load_plane = [&](int i) {
+                const int j = i >> 1, n = j / (2 * NB), in_tile = j - n * 2 * NB, hi = i & 1;
+                const bool is_v = in_tile >= NB;
+                const int st = hi ? j % NH : j % NL, round = hi ? j / NH : j / NL;
+                uint64_t *full = hi ? &sh->full[st] : &sh->full_lo[st];
+                if (round > 0 && !rwait(hi ? &sh->freed[st] : &sh->freed_lo[st], (uint32_t)((round & 1) ^ 1), sh)) { rgive_up(sh, 91), live = false; return; }
+                mbar_arrive_expect_tx(full, BT);
+                tma_load_4d(hi ? ring + st * BT : ring_lo + st * BT, is_v ? &vmap : &kmap, full, 0, key_tile(n) * 128, g * NB + (is_v ? in_tile - NB : in_tile), hi ? b : B + b);
+                ++issued;
+            };
+            const int at_first = WIN ? (2 * NL < 2 * n_blocks ? 2 * NL : 2 * n_blocks) : 0;  // (what finds its slot empty)
+            for (int i = 0; i < at_first; ++i) load_plane(i);
             auto load_block = [&](int j) {
                 const int st = j % NR;
                 if (j >= NR && !rwait(&sh->freed[st], (uint32_t)(((j / NR) & 1) ^ 1), sh)) { rgive_up(sh, 91), live = false; return; }
@@ -421,7 +445,7 @@ __global__ void __launch_bounds__(kResThreads, 1)
                 tma_load_4d(base + BT, mp, &sh->full[st], 0, key_tile(n) * 128, g * NB + blk, B + b);
                 ++issued;
             };
-            for (int j = 0; j < NR && j < n_blocks; ++j) load_block(j);
+            for (int j = 0; !WIN && j < NR && j < n_blocks; ++j) load_block(j);
             if (!rwait(&sh->a_ready, 0, sh)) rgive_up(sh, 91), live = false;
             if (live) {
                 mbar_arrive_expect_tx(&sh->ql_full, 2 * NB * BT);
@@ -430,11 +454,18 @@ __global__ void __launch_bounds__(kResThreads, 1)
                     tma_load_4d(sGl + blk * BT, &gmap, &sh->ql_full, 0, m0, h * NB + blk, B + b);
                 }
             }
-            for (int j = NR; live && j < n_blocks; ++j) load_block(j);
+            for (int i = at_first; WIN && live && i < 2 * n_blocks; ++i) load_plane(i);
+            for (int j = NR; !WIN && live && j < n_blocks; ++j) load_block(j);
             if (sh->abort) {
                 mbar_wait(&sh->qh_full, 0);
                 if (live) mbar_wait(&sh->ql_full, 0);
-                for (int j = (issued > NR ? issued - NR : 0); j < issued; ++j) mbar_wait(&sh->full[j % NR], (uint32_t)((j / NR) & 1));
+                if (WIN) {
+                    const int n_lo = (issued + 1) >> 1, n_hi = issued >> 1;
+                    for (int j = (n_hi > NH ? n_hi - NH : 0); j < n_hi; ++j) mbar_wait(&sh->full[j % NH], (uint32_t)((j / NH) & 1));
+                    for (int j = (n_lo > NL ? n_lo - NL : 0); j < n_lo; ++j) mbar_wait(&sh->full_lo[j % NL], (uint32_t)((j / NL) & 1));
+                } else {
+                    for (int j = (issued > NR ? issued - NR : 0); j < issued; ++j) mbar_wait(&sh->full[j % NR], (uint32_t)((j / NR) & 1));
+                }
             }
         }
         __syncwarp();
@@ -456,7 +487,33 @@ __global__ void __launch_bounds__(kResThreads, 1)
                     tc_fence_after();
                     const uint32_t acc = tmem + (prod ? cDP : cS), a_hi = tmem + (prod ? cGh : cQh);
                     const uint32_t a_lo = prod ? gl_u32 : ql_u32;
-                    for (int blk = 0; blk < NB; ++blk, ++j) {
+                    if (WIN) {  // (S as the forward has it, attn_rows_tc)
+                        for (int blk = 0; blk < NB; ++blk) {
+                            const int i = j + blk, sth = i % NH, stl = i % NL;
+                            if (!rwait(&sh->full_lo[stl], (uint32_t)((i / NL) & 1), sh) || !rwait(&sh->full[sth], (uint32_t)((i / NH) & 1), sh)) { rgive_up(sh, 94); ok = false; break; }
+                            tc_fence_after();
+                            const uint64_t bh = desc_kmajor(ring_u32 + (uint32_t)(sth * BT)), bl = desc_kmajor(ring_u32 + (uint32_t)((NH + stl) * BT));
+                            const uint64_t al = desc_kmajor(a_lo + (uint32_t)(blk * BT));
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                if (blk * 4 + kk >= steps) break;
+                                mma_ts_f16(acc, a_hi + (uint32_t)((blk * 4 + kk) * 8), desc_advance(bl, kk * 32), idesc, (blk > 0 || kk > 0) ? 1 : 0);
+                                mma_ss_f16(acc, desc_advance(al, kk * 32), desc_advance(bh, kk * 32), idesc, 1);
+                            }
+                            mma_commit(&sh->freed_lo[stl]);
+                        }
+                        for (int blk = 0; ok && blk < NB; ++blk, ++j) {
+                            const int sth = j % NH;
+                            const uint64_t bh = desc_kmajor(ring_u32 + (uint32_t)(sth * BT));
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                if (blk * 4 + kk >= steps) break;
+                                mma_ts_f16(acc, a_hi + (uint32_t)((blk * 4 + kk) * 8), desc_advance(bh, kk * 32), idesc, 1);
+                            }
+                            mma_commit(&sh->freed[sth]);
+                        }
+                    }
+                    for (int blk = 0; !WIN && blk < NB; ++blk, ++j) {
                         const int st = j % NR;
                         if (!rwait(&sh->full[st], (uint32_t)((j / NR) & 1), sh)) { rgive_up(sh, 94); ok = false; break; }
                         tc_fence_after();
@@ -464,26 +521,13 @@ __global__ void __launch_bounds__(kResThreads, 1)
                         const uint64_t bh = desc_kmajor(base), bl = desc_kmajor(base + BT);
                         const uint64_t al = desc_kmajor(a_lo + (uint32_t)(blk * BT));
 #pragma unroll
-                        for (int kk = 0; !WIN && kk < 4; ++kk) {
+                        for (int kk = 0; kk < 4; ++kk) {
                             if (blk * 4 + kk >= steps) break;
                             const uint64_t dbh = desc_advance(bh, kk * 32), dbl = desc_advance(bl, kk * 32);
                             const uint32_t at = a_hi + (uint32_t)((blk * 4 + kk) * 8);
                             mma_ts_f16(acc, at, dbh, idesc, (blk > 0 || kk > 0) ? 1 : 0);
                             mma_ts_f16(acc, at, dbl, idesc, 1);
                             mma_ss_f16(acc, desc_advance(al, kk * 32), dbh, idesc, 1);
-                        }
-                        // (a window's in the order of its forward, attn_rows_tc, where the small terms go first)
-#pragma unroll
-                        for (int i = 0; WIN && i < 8; ++i) {
-                            const int kk = i & 3;
-                            if (blk * 4 + kk >= steps) continue;
-                            const uint32_t at = a_hi + (uint32_t)((blk * 4 + kk) * 8);
-                            if (i & 4) {
-                                mma_ts_f16(acc, at, desc_advance(bh, kk * 32), idesc, 1);
-                            } else {
-                                mma_ts_f16(acc, at, desc_advance(bl, kk * 32), idesc, (blk > 0 || kk > 0) ? 1 : 0);
-                                mma_ss_f16(acc, desc_advance(al, kk * 32), desc_advance(bh, kk * 32), idesc, 1);
-                            }
                         }
                         mma_commit(&sh->freed[st]);
                     }
@@ -660,7 +704,7 @@ inline WidePieces wide_pieces(const BwdWindow &w, int Tp) {
         keys = k > keys ? k : keys;
         rows = r > rows ? r : rows;
     }
-    const int dq = (keys + win_depth(0) - 1) / win_depth(0), dkv = (rows + win_depth(1) - 1) / win_depth(1);
+    const int dq = (keys + kPiece - 1) / kPiece, dkv = (rows + kPiece - 1) / kPiece;
     return WidePieces{dq > dkv ? dq : dkv, dq};
 }
 
@@ -687,9 +731,8 @@ struct TriUnit {
         const int ug = p.unit0 + u;
         b = ug / p.n_heads, h = ug - b * p.n_heads;
         m0 = m * 128;
-        const int depth = p.win.window > 0 ? win_depth(which) : kPiece;
-        k_begin = piece * depth;
-        int k_end = k_begin + depth;
+        k_begin = piece * kPiece;
+        int k_end = k_begin + kPiece;
         sinks_end = 0, skip = 0;
         if (p.win.window > 0) {  // pieces of what is visited
             if (which == 0) {
@@ -710,8 +753,8 @@ struct TriUnit {
     }
 };
 
-template <int D>
-__global__ void __launch_bounds__(kTriThreads, 1)
+template <int D, bool WIN>
+__global__ void __launch_bounds__(WIN ? kTriThreadsWin : kTriThreads, 1)
     wide_products(const __grid_constant__ CUtensorMap ds_k, const __grid_constant__ CUtensorMap ds_m, const __grid_constant__ CUtensorMap p_m,
                   const __grid_constant__ CUtensorMap k_n, const __grid_constant__ CUtensorMap qs_n, const __grid_constant__ CUtensorMap g_n,
                   const WideParams p, int n_units) {
@@ -727,7 +770,7 @@ __global__ void __launch_bounds__(kTriThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh->full[i], 1), mbar_init(&sh->freed[i], 1);
-            mbar_init(&sh->acc_full[i], 1), mbar_init(&sh->acc_free[i], 4);
+            mbar_init(&sh->acc_full[i], 1), mbar_init(&sh->acc_free[i], WIN ? 8 : 4);
         }
         sh->abort = (smem_u32(smem_raw) & 1023u) ? 84 : 0;
         if (sh->abort) atomicMax(&g_tc_status, 84);
@@ -774,17 +817,17 @@ __global__ void __launch_bounds__(kTriThreads, 1)
         // ------------------------------------------------------------------ MMA issuer
         if (elect_one() && !sh->abort) {
             const uint32_t s_u32 = smem_u32(smem_raw);
-            int it = 0, n = 0;  // steps, units with something to do
-            const bool win = p.win.window > 0;  // (the small terms of a step first)
+            int it = 0, n = 0;  // steps; accumulators handed over: one a unit with something to do (WIN: one every kWinSteps steps)
             for (int i = blockIdx.x; i < n_units && !sh->abort; i += gridDim.x) {
                 const TriUnit w(p, i);
                 if (w.n_steps <= 0) continue;
                 const uint32_t idesc = idesc_f16(128, 16 * head_steps(p.dim_out), w.which != 0, true);
                 const uint32_t a_step = w.which ? 2048 : 32;
-                const uint32_t acc = tmem + (n & 1) * 256;
-                if (n >= 2 && !twait(&sh->acc_free[n & 1], (uint32_t)(((n >> 1) & 1) ^ 1), sh)) { tgive_up(sh, 86); break; }
+                if (!WIN && n >= 2 && !twait(&sh->acc_free[n & 1], (uint32_t)(((n >> 1) & 1) ^ 1), sh)) { tgive_up(sh, 86); break; }
                 for (int s = 0; s < w.n_steps; ++s, ++it) {
                     const int st = it & 1;
+                    const uint32_t acc = tmem + (n & 1) * 256;
+                    if (WIN && s % kWinSteps == 0 && n >= 2 && !twait(&sh->acc_free[n & 1], (uint32_t)(((n >> 1) & 1) ^ 1), sh)) { tgive_up(sh, 86); break; }
                     if (!twait(&sh->full[st], (uint32_t)((it >> 1) & 1), sh)) { tgive_up(sh, 86); break; }
                     tc_fence_after();
                     const uint32_t base = s_u32 + (uint32_t)(st * kStage);
@@ -796,22 +839,23 @@ __global__ void __launch_bounds__(kTriThreads, 1)
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint64_t dah = desc_advance(ah, kk * a_step), dal = desc_advance(al, kk * a_step);
                         const uint64_t dbh = desc_advance(bh, kk * 2048), dbl = desc_advance(bl, kk * 2048);
-                        if (!win) mma_ss_f16(acc, dah, dbh, idesc, (s > 0 || kk > 0) ? 1 : 0);
-                        mma_ss_f16(acc, dah, dbl, idesc, (!win || s > 0 || kk > 0) ? 1 : 0);
+                        if (!WIN) mma_ss_f16(acc, dah, dbh, idesc, (s > 0 || kk > 0) ? 1 : 0);
+                        mma_ss_f16(acc, dah, dbl, idesc, (!WIN || s % kWinSteps > 0 || kk > 0) ? 1 : 0);
                         mma_ss_f16(acc, dal, dbh, idesc, 1);
                     }
-                    if (win)
+                    if (WIN) {  // (the small terms first)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) mma_ss_f16(acc, desc_advance(ah, kk * a_step), desc_advance(bh, kk * 2048), idesc, 1);
+                    }
                     mma_commit(&sh->freed[st]);
+                    if (WIN && (s % kWinSteps == kWinSteps - 1 || s == w.n_steps - 1)) mma_commit(&sh->acc_full[n++ & 1]);
                 }
-                mma_commit(&sh->acc_full[n & 1]);
-                ++n;
+                if (!WIN) mma_commit(&sh->acc_full[n++ & 1]);
             }
         }
         __syncwarp();
     } else {
-        // ------------------------------------------------------------------ epilogue: a thread per output row
+        // ------------------------------------------------------------------ epilogue: a thread per output row (WIN: and half of its columns)
         const int lane = threadIdx.x & 31, j8 = lane & 7;
         const int lane_grp = warp & 3;
         const uint32_t lane_base = (uint32_t)(lane_grp * 32) << 16;
@@ -831,21 +875,55 @@ __global__ void __launch_bounds__(kTriThreads, 1)
             } else {
                 f = 1.0f / (p.p_scale * block_mult(p.amax_do[bg]));
             }
-            if (!__all_sync(0xffffffffu, twait(&sh->acc_full[n & 1], (uint32_t)((n >> 1) & 1), sh))) { tgive_up(sh, 87); break; }
-            tc_fence_after();
+            // a window's: what the steps leave, added up with rounding
+            constexpr int CW = WIN ? D / 2 : 32;
+            const int col0 = WIN ? ((int)(warp - 2) >> 2) * CW : 0;
+            float2 sum[CW / 2];
+            if (WIN) {
+                bool ok = true;
+#pragma unroll
+                for (int c = 0; c < CW / 2; ++c) sum[c] = make_float2(0.f, 0.f);
+                for (int s = 0; ok && s < w.n_steps; s += kWinSteps, ++n) {
+                    ok = __all_sync(0xffffffffu, twait(&sh->acc_full[n & 1], (uint32_t)((n >> 1) & 1), sh));
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < CW; c += 32) {
+                        uint32_t r[32];
+                        tmem_ld32(tmem + lane_base + (n & 1) * 256 + col0 + c, r);
+                        tmem_wait_ld();
+                        if (c + 32 == CW) {
+                            tc_fence_before();
+                            mbar_arrive_warp_relaxed(&sh->acc_free[n & 1]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) sum[(c + e) / 2] = tcb::add2(sum[(c + e) / 2], tcb::floats2(r[e], r[e + 1]));
+                    }
+                }
+                if (!ok) { tgive_up(sh, 87); break; }
+            } else {
+                if (!__all_sync(0xffffffffu, twait(&sh->acc_full[n & 1], (uint32_t)((n >> 1) & 1), sh))) { tgive_up(sh, 87); break; }
+                tc_fence_after();
+            }
             const long long ld = (long long)(w.which == 0 ? p.n_heads : p.n_kv_heads) * p.dim_out;
             const int row0 = t - j8;  // the first of this lane's eight rows
             const bool whole = w.which == 0 && p.dq_whole;
             float *dst = (w.which == 0 ? p.dq : w.which == 1 ? p.dk : p.dv) + ((long long)w.b * p.T + row0) * ld +
                          (long long)(w.which == 0 ? w.h : g) * p.dim_out + 4 * j8;
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+#pragma unroll(WIN ? CW / 32 : 1)
+            for (int i32 = 0; i32 < (WIN ? CW : D); i32 += 32) {
+                const int c = col0 + i32;
                 uint32_t r[32];
-                tmem_ld32(tmem + lane_base + (n & 1) * 256 + c, r);
-                tmem_wait_ld();
-                if (c + 32 == D) {  // all read: the MMAs may have the buffer while the last columns are on their way
-                    tc_fence_before();
-                    mbar_arrive_warp_relaxed(&sh->acc_free[n & 1]);
+                if (WIN) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) r[e] = __float_as_uint(sum[(WIN ? i32 + e : e) / 2].x), r[e + 1] = __float_as_uint(sum[(WIN ? i32 + e : e) / 2].y);
+                } else {
+                    tmem_ld32(tmem + lane_base + (n & 1) * 256 + c, r);
+                    tmem_wait_ld();
+                    if (c + 32 == D) {  // all read: the MMAs may have the buffer while the last columns are on their way
+                        tc_fence_before();
+                        mbar_arrive_warp_relaxed(&sh->acc_free[n & 1]);
+                    }
                 }
                 if (c >= p.dim_out) continue;
 #pragma unroll
@@ -877,7 +955,7 @@ __global__ void __launch_bounds__(kTriThreads, 1)
                     }
                 }
             }
-            ++n;
+            if (!WIN) ++n;
         }
     }
     tc_fence_before();
@@ -1005,7 +1083,7 @@ inline int launch_bwd_wide(const float *q, const float *k, const float *v, const
     const size_t smem_r = td == 192 ? res_smem_bytes<192>() : res_smem_bytes<256>();
     const auto scores = window > 0 ? (td == 192 ? bwd_wide_scores_res<192, true> : bwd_wide_scores_res<256, true>)
                                    : (td == 192 ? bwd_wide_scores_res<192, false> : bwd_wide_scores_res<256, false>);
-    const auto products = td == 192 ? wide_products<192> : wide_products<256>;
+    const auto products = window > 0 ? (td == 192 ? wide_products<192, true> : wide_products<256, true>) : (td == 192 ? wide_products<192, false> : wide_products<256, false>);
     if (optin_smem((const void *)bwd_wide_scores, smem) || optin_smem((const void *)scores, smem_r) ||
         optin_smem((const void *)products, smem_t))
         return 1;
@@ -1039,7 +1117,7 @@ inline int launch_bwd_wide(const float *q, const float *k, const float *v, const
         const long long n_units = 3LL * nt * units * p.pieces;
         const dim3 gp((unsigned)(n_units < split_sm_count() ? n_units : split_sm_count()));
         p.in_turn = products_in_turn(p.pieces, nt, units, split_sm_count());
-        if (launch_after("wide_products", products, gp, dim3(kTriThreads), smem_t, stream, 1, ds_k, ds_m, p_m, k_n, qs_n, g_n, p, (int)n_units))
+        if (launch_after("wide_products", products, gp, dim3(window > 0 ? kTriThreadsWin : kTriThreads), smem_t, stream, 1, ds_k, ds_m, p_m, k_n, qs_n, g_n, p, (int)n_units))
             return 1;
     }
     return 0;

@@ -326,27 +326,22 @@ __global__ void __launch_bounds__(Cfg<TD, PLANES>::kThreads, 1) attn_rows_tc(con
                     const uint32_t cS = C::cS + (j % SB) * BN;
                     const uint64_t bkh = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP)), bkl = desc_kmajor(k_u32 + (uint32_t)(s * 2 * KP + KP));
                     const uint64_t bql = desc_kmajor(ql_u32);
-                    // (the two small terms first, while there is little to truncate: of the whole contraction, but above 128 columns of whole
-                    // sequences of 64 at a time, as the backward has them.  It forms S in the same order: where a softmax is saturated, what its
-                    // dP and delta leave of each other is as good as the two S agree.  Of 128 columns, in two halves / at once: out's error at
-                    // T 8192, window 1024 5.5e-7 / 3.6e-7; a prompt of 16384, window 4096, 538 / 524 us.  Of 256 over pages, in four / at once:
-                    // 1.2e-6 / 6.5e-7.  Whole sequences of 256 at once: out's 9.8e-7 / 4.8e-7, but dk's 2.2e-6 / 2.5e-6.)
-                    constexpr int kSpan = C::kWide && !PAGED ? 4 : TD / 16;
+                    // (the two small terms of the whole contraction first, while there is little to truncate.  The backward forms S in the same
+                    // order: where a softmax is saturated, what its dP and delta leave of each other is as good as the two S agree.  64 columns
+                    // at a time / at once: out's error at T 8192, window 1024, heads of 128 5.5e-7 / 3.6e-7, at T 1024, window 256, heads of 256
+                    // 9.8e-7 / 4.8e-7; a prompt of 16384, window 4096, heads of 128 538 / 524 us.)
 #pragma unroll
-                    for (int c = 0; c < TD / 16; c += kSpan) {
+                    for (int kk = 0; kk < TD / 16; ++kk) {
+                        if (kk >= steps) break;
+                        const uint32_t bo = (uint32_t)((kk >> 2) * (BN * 128) + (kk & 3) * 32);
+                        mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, desc_advance(bkl, bo), id_s, kk > 0);
+                        if (C::kWide) mma_ss_f16(tmem + cS, desc_advance(bql, (uint32_t)((kk >> 2) * (128 * 128) + (kk & 3) * 32)), desc_advance(bkh, bo), id_s, 1);
+                        else mma_ts_f16(tmem + cS, tmem + C::cQl + kk * 8, desc_advance(bkh, bo), id_s, 1);
+                    }
 #pragma unroll
-                        for (int kk = c; kk < c + kSpan; ++kk) {
-                            if (kk >= steps) break;
-                            const uint32_t bo = (uint32_t)((kk >> 2) * (BN * 128) + (kk & 3) * 32);
-                            mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, desc_advance(bkl, bo), id_s, kk > 0);
-                            if (C::kWide) mma_ss_f16(tmem + cS, desc_advance(bql, (uint32_t)((kk >> 2) * (128 * 128) + (kk & 3) * 32)), desc_advance(bkh, bo), id_s, 1);
-                            else mma_ts_f16(tmem + cS, tmem + C::cQl + kk * 8, desc_advance(bkh, bo), id_s, 1);
-                        }
-#pragma unroll
-                        for (int kk = c; kk < c + kSpan; ++kk) {
-                            if (kk >= steps) break;
-                            mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, desc_advance(bkh, (uint32_t)((kk >> 2) * (BN * 128) + (kk & 3) * 32)), id_s, 1);
-                        }
+                    for (int kk = 0; kk < TD / 16; ++kk) {
+                        if (kk >= steps) break;
+                        mma_ts_f16(tmem + cS, tmem + C::cQh + kk * 8, desc_advance(bkh, (uint32_t)((kk >> 2) * (BN * 128) + (kk & 3) * 32)), id_s, 1);
                     }
                     mma_commit(&sh->k_free[s]);
                     mma_commit(&sh->s_full[j % SB]);
