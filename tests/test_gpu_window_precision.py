@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 from test_gpu_paged import Case
-from test_gpu_window import backward64, make
+from test_gpu_window import backward64, make, seen
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,25 @@ def test_rows_over_pages(zt, H, G, D, rows):
     ref = c.reference(0)[0]
     bound = math.hypot(math.sqrt(2) * D / 16 * 2.0**-24 * 2 / 3, 4.8e-7)
     assert float((out.double() - ref).norm() / ref.norm()) <= bound
+
+
+@pytest.mark.parametrize("B,T,H,G,D,window,sinks", [(4, 1000, 16, 4, 80, 200, 3), (1, 1000, 16, 4, 128, 300, 4), (1, 700, 8, 2, 112, 150, 0), (2, 500, 4, 4, 128, 400, 2), (1, 1000, 16, 4, 192, 300, 4), (2, 1024, 16, 4, 256, 256, 0)])
+def test_gradients_beside_a_plain_form_in_32_bits(zt, B, T, H, G, D, window, sinks):
+    """At most half as much again as what sums in 32 bits leave, or 1e-6."""
+    q, k, v, dout = make(B, T, H, G, D, seed=T + D)
+    ref = backward64(q, k, v, dout, H, G, D, window, sinks)
+    R, scale = H // G, 1.0 / math.sqrt(D)
+    qs, gs = (x.view(B, T, G, R, D) for x in (q, dout))
+    ks, vs = (x.view(B, T, G, D) for x in (k, v))
+    assert not torch.backends.cuda.matmul.allow_tf32
+    s = (torch.einsum("btgrd,bsgd->bgrts", qs, ks) * scale).masked_fill(~seen(T, window, sinks), -math.inf)
+    p = torch.exp(s - s.amax(-1, keepdim=True))
+    p = p / p.sum(-1, keepdim=True)
+    delta = (gs * torch.einsum("bgrts,bsgd->btgrd", p, vs)).sum(-1).permute(0, 2, 3, 1)[..., None]
+    ds = p * (torch.einsum("btgrd,bsgd->bgrts", gs, vs) - delta)
+    plain = {"dq": (torch.einsum("bgrts,bsgd->btgrd", ds, ks) * scale).reshape(B, T, H * D), "dk": (torch.einsum("bgrts,btgrd->bsgd", ds, qs) * scale).reshape(B, T, G * D),
+             "dv": torch.einsum("bgrts,btgrd->bsgd", p, gs).reshape(B, T, G * D)}
+    e = errors(zt, B, T, H, G, D, window, sinks)
+    for name, want in zip(("dq", "dk", "dv"), ref[2:]):
+        theirs = float((plain[name].double() - want).norm() / want.norm())
+        assert e[name] <= max(1e-6, 1.5 * theirs), (name, e[name], theirs)

@@ -117,6 +117,10 @@ constexpr int kFlushRows = 512;  // query rows between flushes
 // heads of 128, window 1024 6.2e-6, 3.4e-6, 2.1e-6 (1171, 1223, 1288), batch 4, T 2048, 32/8 of 64, window 512 4.4e-6, 2.6e-6,
 // 1.6e-6 (334, 338, 347); a plain form in f32 2.1e-6 and 1.2e-6.
 constexpr int kFlushRowsWin = 128;
+// At 65 to 128 columns, where 128 rows are two steps, every step where a key's sums are short, and a plain form's good for it: dk's error in 1e-7,
+// us of the kernel, 128 / 64 rows / plain: T 1000, window 200, 16/4 heads of 80 12 / 7.9 / 7.0 (136, 142), window 300, heads of 128 12 / 8.6 / 8.3; T 8192,
+// window 1024, 8/2 heads of 128 17 / 10 / 15 (32/8 heads 1295, 1377).
+inline bool flushes_often(const BwdWindow &w, int group) { return ((long long)w.window + 127) * group <= 2048; }
 // An iterator: step `it` is (head hh of the group, query tile qi of ROWS rows); `flush` says the accumulators are
 // flushed after it, `fresh` that they restart from zero at it.  No divisions per step: every role of
 // the kernel walks it in lockstep.

@@ -60,10 +60,10 @@ constexpr size_t kFusedSmem = 3 * (size_t)(128 * 128 * 2) + 2 * (size_t)(128 * 1
 constexpr int kFusedThreads = (kKvRowWarps + 3) * 32;
 // PARTS: the walk is split, or the blocks go tile by tile (tc_split.cuh).  A variant of its own: large launches are 1-2 % slower
 // with the code in it.
-// WIN: a window (BwdWindow); the blocks along x are window_block's, times the KV heads.  A walk ends with the window, so the time goes with the pairs seen:
+// WIN: a window (BwdWindow), and the query rows between its flushes; the blocks along x are window_block's, times the KV heads.  A walk ends with the window, so the time goes with the pairs seen:
 // T 8192, 32/8 heads of 128, window 1024 1290 us, 250 TFLOP/s of the pairs seen (two of a tile's nine visits are
 // half masked, and the accumulators are flushed four times as often as without a window).
-template <bool PARTS, bool PAD, bool WIN>
+template <bool PARTS, bool PAD, int WIN>
 __global__ void __launch_bounds__(kFusedThreads, 1)
     attn_bwd_fused_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                       const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
     const int per_head = n_q - qi0;
     const int n_it = n_heads_mine * per_head;
     const int B = p.batch;
-    using Walk = WalkOf<BQ, WIN ? kFlushRowsWin : kFlushRows>;
+    using Walk = WalkOf<BQ, WIN ? WIN : kFlushRows>;
     Walk walk(n_heads_mine, per_head, qi0, n_q);
 
     if (threadIdx.x == 0) {
@@ -665,8 +665,9 @@ __global__ void __launch_bounds__(kFusedThreads, 1)
 inline int launch_bwd_fused(const CUtensorMap &k128, const CUtensorMap &v128, const CUtensorMap &qs64, const CUtensorMap &g64,
                             const BwdParams &p, cudaStream_t stream) {
     const bool win = p.win.window > 0;
-    const auto kernel = win ? (head_steps(p.dim_out) < 8 ? attn_bwd_fused_tc<false, true, true> : attn_bwd_fused_tc<false, false, true>)
-                            : with_flags([](auto parts, auto pad) { return attn_bwd_fused_tc<parts.value, pad.value, false>; }, p.parts.n() > 1 || p.by_tile, head_steps(p.dim_out) < 8);
+    const bool pad = head_steps(p.dim_out) < 8;
+    const auto kernel = win ? with_flags([](auto often, auto pad) { return attn_bwd_fused_tc<false, pad.value, often.value ? 64 : kFlushRowsWin>; }, flushes_often(p.win, p.n_heads / p.n_kv_heads), pad)
+                            : with_flags([](auto parts, auto pad) { return attn_bwd_fused_tc<parts.value, pad.value, 0>; }, p.parts.n() > 1 || p.by_tile, pad);
     if (optin_smem((const void *)kernel, kFusedSmem)) return 1;
     const unsigned tiles = (unsigned)((p.T + 127) / 128), seqs = (unsigned)(p.batch * p.parts.n()), kv = (unsigned)p.n_kv_heads;
     const dim3 grid = win ? dim3((unsigned)window_grid(p.win, p.T, 64, p.n_kv_heads), 1, seqs) : p.by_tile ? dim3(kv, seqs, tiles) : dim3(kv, tiles, seqs);
